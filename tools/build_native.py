@@ -53,7 +53,8 @@ def write_ninja(debug=False, diag=False):
     opt = '-O0 -g' if debug else '-O3'
     hipcc = osp.join(ROCM, 'bin', 'hipcc')
     hip_flags = ('{} {} -x hip --offload-arch={} -fno-gpu-rdc '
-                 '-munsafe-fp-atomics -I{}{}'.format(
+                 '-munsafe-fp-atomics -Xclang -target-feature -Xclang '
+                 '-packed-fp32-ops -I{}{}'.format(
                      opt, common, ARCH, osp.join(ROOT, 'csrc', 'hip'),
                      ' -DDGMC_DIAG=1' if diag else ''))
     host_flags = '{} {} -fopenmp -Wall -Wno-unused-function -I{}'.format(
