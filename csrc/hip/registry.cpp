@@ -5,6 +5,25 @@
 #include <torch/library.h>
 
 namespace dgmc {
+namespace segattn {
+std::tuple<at::Tensor, at::Tensor> segment_attention_fwd(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+    const at::Tensor& ptr_q, const at::Tensor& ptr_k, double scale,
+    double cap, const c10::optional<at::Tensor>& bias,
+    const c10::optional<at::Tensor>& pos_q,
+    const c10::optional<at::Tensor>& pos_k, int64_t half, int64_t mbits,
+    double dmax, bool with_lse);
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+segment_attention_bwd(const at::Tensor& dout, const at::Tensor& q,
+                      const at::Tensor& k, const at::Tensor& v,
+                      const at::Tensor& out, const at::Tensor& lse,
+                      const at::Tensor& ptr_q, const at::Tensor& ptr_k,
+                      double scale, double cap,
+                      const c10::optional<at::Tensor>& bias,
+                      const c10::optional<at::Tensor>& pos_q,
+                      const c10::optional<at::Tensor>& pos_k, int64_t half,
+                      int64_t mbits, double dmax);
+}  // namespace segattn
 void relconv_fwd(const at::Tensor& ptr, const at::Tensor& col,
                  const at::Tensor& split, const at::Tensor& hub,
                  const at::Tensor& xa, const c10::optional<at::Tensor>& xb,
@@ -613,6 +632,16 @@ TORCH_LIBRARY(dgmc_amd, m) {
       "sinkhorn_transport_bwd(Tensor? grad_P, Tensor grad_joint, Tensor r_s, "
       "Tensor S_hat, Tensor ptr_s, Tensor ptr_t, Tensor a_hist, Tensor "
       "b_hist, int iters, float tau, Tensor? add) -> Tensor");
+  m.def(
+      "segment_attention_fwd(Tensor q, Tensor k, Tensor v, Tensor ptr_q, "
+      "Tensor ptr_k, float scale, float cap, Tensor? bias, Tensor? pos_q, "
+      "Tensor? pos_k, int half, int mbits, float dmax, bool with_lse) -> "
+      "(Tensor, Tensor)");
+  m.def(
+      "segment_attention_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, "
+      "Tensor out, Tensor lse, Tensor ptr_q, Tensor ptr_k, float scale, "
+      "float cap, Tensor? bias, Tensor? pos_q, Tensor? pos_k, int half, int "
+      "mbits, float dmax) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(dgmc_amd, CompositeExplicitAutograd, m) {
@@ -707,4 +736,6 @@ TORCH_LIBRARY_IMPL(dgmc_amd, CUDA, m) {
   m.impl("sinkhorn_bwd", &dgmc::sinkhorn_bwd);
   m.impl("sinkhorn_transport", &dgmc::sinkhorn_transport);
   m.impl("sinkhorn_transport_bwd", &dgmc::sinkhorn_transport_bwd);
+  m.impl("segment_attention_fwd", &dgmc::segattn::segment_attention_fwd);
+  m.impl("segment_attention_bwd", &dgmc::segattn::segment_attention_bwd);
 }

@@ -1,0 +1,320 @@
+// Attention inside the segments (graphs) of a packed node batch, gfx950:
+// shared pieces of the forward and backward kernels.
+//
+//   z_ij = cap tanh(scale <q_i, k_j> / cap) + T[h, bucket(pos_j - pos_i)]
+//   p_i  = softmax_j z_ij over the keys j of row i's segment,  o_i = p_i v
+//
+// (cap and the bias table T are optional; a row without keys, or whose
+// scores are all -inf, gives 0).  Heads h share key head h / G.
+//
+// Packed rows.  The G query heads of one key head are rows of the same
+// tile: row c of a wave's 32 is query c / G, head c % G (c < RW = G floor(32
+// / G)), so every K / V tile staged in LDS serves all of them, a single new
+// query fills G rows, and dK / dV sum over the group inside one workgroup.
+//
+// Work list without a plan.  Segment b's tiles occupy the slots from
+// f(b) = ptr[b] / TQ + b on (TQ queries per tile): f grows by at least
+// ceil(n_b / TQ) per segment, so floor(N / TQ) + B + 1 slots always suffice
+// and the grid depends on N and B only - no host copy of ptr, no sort, and
+// a captured graph may change ptr between replays.  A wave finds its
+// segment by a 64-way search (two dependent loads for B <= 4096).  Slots
+// without a tile end at once.
+//
+// Matrix products.  32 x 32 accumulators: lane l holds column l & 31 and
+// rows 8 (r / 4) + 4 (l >> 5) + r % 4.  Scores are formed TRANSPOSED to the
+// axis that is reduced next (the forward keeps one query per lane, so a
+// row's maximum and sum are in-lane plus one exchange), and the
+// accumulator's rows then serve directly as the K index of the second
+// product: its other operand is read from LDS in that same row order
+// (bf16: ds_read_b64_tr_b16, 4 rows a time; fp32: one value a lane), no
+// lane exchange of P.  bf16 runs on v_mfma_f32_32x32x16_bf16, fp32 on
+// v_mfma_f32_32x32x2_f32 (exact products, fp32 sums).
+//
+// Bucket of an offset d = pos_j - pos_i on one axis: b(|d|) with `steps` =
+// 2^m buckets per octave, read off the float 2 (|d| / steps + 1): its
+// exponent and top m mantissa bits ARE the bucket number (exact integer
+// arithmetic up to 2^23; larger distances fall into the last bucket).  The
+// sign selects the upper or lower half.  The table sits in LDS with one
+// unused slot between the halves (so the sign is one xor-add).
+#pragma once
+
+#include "common.h"
+
+namespace dgmc {
+namespace segattn {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kSlots = 64;            // LDS slots of one head's bias table
+// Finite biases below this count as it: times log2(e) they stay finite, so
+// a row masked everywhere by a type's lowest value is uniform, not empty.
+constexpr float kLowest = -1e38f;
+
+struct Args {
+  const void *q, *k, *v, *o, *dout;
+  void *out, *dq, *dk, *dv;
+  float *lse, *delta;                 // [Nq, H]
+  float *part_o, *part_ml;            // splits: [S][Nq, H, D], [S][Nq, H, 2]
+  float *part_bias;                   // [blocks][KV][G][kSlots]
+  const int *ptr_q, *ptr_k;
+  const float* bias;                  // [H, nb]
+  const int *pos_q, *pos_k;           // [N, axes]
+  int64_t q_sn, q_sh, k_sn, k_sh, v_sn, v_sh, o_sn, o_sh, g_sn, g_sh;
+  int B, Nq, Nk, H, KV, G, D, nb, half, mbits, slots;
+  float scale, cap, dmax, dmul;
+  int vec_q, vec_k, vec_v, vec_o, vec_g;   // 16-byte rows
+  int splits;
+};
+
+// Segment `b` rows (clamped to [0, N]; the first segment starts at row 0,
+// "segment" B is the tail behind the last one).
+__device__ __forceinline__ int seg_begin(const int* ptr, int b, int N) {
+  return b == 0 ? 0 : min(max(ptr[b], 0), N);
+}
+__device__ __forceinline__ void seg_range(const int* ptr, int b, int B, int N,
+                                          int& lo, int& hi) {
+  lo = seg_begin(ptr, b, N);
+  hi = b >= B ? N : min(max(ptr[b + 1], lo), N);
+}
+
+// Largest b in [0, B] with f(b) <= slot (wave-uniform result).
+__device__ __forceinline__ int find_segment(const int* ptr, int B, int N,
+                                            int per, int slot) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = B + 1;
+  while (n > 1) {
+    const int step = (n + 63) >> 6;
+    const int idx = lo + lane * step;
+    bool ok = lane * step < n;
+    if (ok) ok = seg_begin(ptr, idx, N) / per + idx <= slot;
+    const int c = max(__popcll(__ballot(ok)), 1);
+    const int adv = (c - 1) * step;
+    lo += adv;
+    n = min(step, n - adv);
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// 16-byte chunk swizzle of an LDS tile row with CH chunks: both 16-byte
+// column reads over 16 rows and transposing reads of 4 rows spread over all
+// banks.
+template <int CH>
+__device__ __forceinline__ int swz(int row) {
+  if constexpr (CH >= 16) return ((row & 3) << 2) | ((row >> 2) & 3);
+  else if constexpr (CH == 8)
+    return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  else return (row >> 2) & 3;
+}
+
+__device__ __forceinline__ float max_half(float v) {   // over lanes l, l ^ 32
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float sum_half(float v) {
+  return v + __shfl_xor(v, 32);
+}
+__device__ __forceinline__ float exp2_(float x) {
+  return __builtin_amdgcn_exp2f(x);
+}
+
+// One 16-byte chunk of a row of D elements (zeros outside).
+template <typename T>
+__device__ __forceinline__ u32x4 load_chunk(const T* row, int ch, int D,
+                                            bool valid, int vec) {
+  constexpr int E = 16 / sizeof(T);
+  u32x4 r = {0u, 0u, 0u, 0u};
+  const int d0 = ch * E;
+  if (!valid || d0 >= D) return r;
+  if (vec) return *reinterpret_cast<const u32x4*>(row + d0);
+  T tmp[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) tmp[e] = d0 + e < D ? row[d0 + e] : T(0.f);
+  __builtin_memcpy(&r, tmp, 16);
+  return r;
+}
+
+// --------------------------------------------------------------------------
+// Matrix core policies
+// --------------------------------------------------------------------------
+template <typename T> struct Mma;
+
+template <> struct Mma<__bf16> {
+  // acc += A B for one pair of 16-byte chunks (K = 16).
+  __device__ __forceinline__ static f32x16 dot(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+        __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+        0);
+  }
+  // acc[blk] += tile^T p: rows of `tile` (32 from row0) are the K index, in
+  // the accumulator's row order.
+  template <int DP>
+  __device__ __forceinline__ static void accum(f32x16 (&acc)[DP / 32],
+                                               const DGMC_LDS char* tile,
+                                               int row0, f32x16 p) {
+    constexpr int CH = DP / 8;
+    const int lane = threadIdx.x & 63;
+    const int h = lane >> 5, ds = (lane >> 4) & 1, q = (lane >> 2) & 3,
+              pp = lane & 3;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      bf16x8 b;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) b[i] = (__bf16)p[8 * c + i];
+      const int r0 = row0 + 16 * c + 4 * h + q, r1 = r0 + 8;
+#pragma unroll
+      for (int k = 0; k < DP / 32; ++k) {
+        const int ch = 4 * k + 2 * ds + (pp >> 1);
+        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (DGMC_LDS i16x4*)(tile + (r0 * CH + (ch ^ swz<CH>(r0))) * 16 +
+                              8 * (pp & 1)));
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (DGMC_LDS i16x4*)(tile + (r1 * CH + (ch ^ swz<CH>(r1))) * 16 +
+                              8 * (pp & 1)));
+        const i16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5,
+                                                   6, 7);
+        acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            __builtin_bit_cast(bf16x8, both), b, acc[k], 0, 0, 0);
+      }
+    }
+  }
+  __device__ __forceinline__ static float chunk_dot(u32x4 a, u32x4 b) {
+    const bf16x8 x = __builtin_bit_cast(bf16x8, a),
+                 y = __builtin_bit_cast(bf16x8, b);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += (float)x[i] * (float)y[i];
+    return s;
+  }
+};
+
+template <> struct Mma<float> {
+  __device__ __forceinline__ static f32x16 dot(u32x4 a, u32x4 b, f32x16 c) {
+    const f32x4 x = __builtin_bit_cast(f32x4, a),
+                y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
+    return c;
+  }
+  template <int DP>
+  __device__ __forceinline__ static void accum(f32x16 (&acc)[DP / 32],
+                                               const DGMC_LDS char* tile,
+                                               int row0, f32x16 p) {
+    constexpr int CH = DP / 4;
+    const int lane = threadIdx.x & 63, h = lane >> 5, d = lane & 31;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = row0 + 8 * (r >> 2) + 4 * h + (r & 3);
+#pragma unroll
+      for (int k = 0; k < DP / 32; ++k) {
+        const int ch = 8 * k + (d >> 2);
+        const float a = *(const DGMC_LDS float*)(
+            tile + (row * CH + (ch ^ swz<CH>(row))) * 16 + 4 * (d & 3));
+        acc[k] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[k], 0, 0,
+                                                      0);
+      }
+    }
+  }
+  __device__ __forceinline__ static float chunk_dot(u32x4 a, u32x4 b) {
+    const f32x4 x = __builtin_bit_cast(f32x4, a),
+                y = __builtin_bit_cast(f32x4, b);
+    return (x[0] * y[0] + x[1] * y[1]) + (x[2] * y[2] + x[3] * y[3]);
+  }
+};
+
+// Chunk (row, ch) of a swizzled LDS tile.
+template <int CH>
+__device__ __forceinline__ u32x4 lds_chunk(const DGMC_LDS char* tile, int row,
+                                           int ch) {
+  return *(const DGMC_LDS u32x4*)(tile + (row * CH + (ch ^ swz<CH>(row))) *
+                                             16);
+}
+
+// --------------------------------------------------------------------------
+// Scores
+// --------------------------------------------------------------------------
+// tanh: v_exp / v_rcp (about 1 ulp each) of 1 - 2 / (e^2x + 1), whose
+// cancellation leaves an absolute error of 1e-7 near 0 - below a bf16
+// product's rounding.  fp32 (EXACT) takes the odd series up to |x| < 0.25
+// (to x^9; the next term is 8.5e-9 of x there) so small scores keep their
+// relative precision.
+template <bool EXACT>
+__device__ __forceinline__ float tanh_(float x) {
+  const float e = exp2_(x * (2.f * kLog2e));
+  const float t = fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
+  if constexpr (EXACT) {
+    const float y = x * x;
+    float s = fmaf(y, 62.f / 2835.f, -17.f / 315.f);
+    s = fmaf(y, s, 2.f / 15.f);
+    s = fmaf(y, s, -1.f / 3.f);
+    const float small = fmaf(x * y, s, x);
+    return fabsf(x) < 0.25f ? small : t;
+  } else {
+    return t;
+  }
+}
+
+// Bucket slot of offset d (float, exact) on one axis: 0 .. 2 half + 1.
+struct Bucket {
+  float dmax, dmul;
+  int shift, width, K;
+  __device__ __forceinline__ explicit Bucket(const Args& a)
+      : dmax(a.dmax), dmul(a.dmul), shift(23 - a.mbits), width(5 + a.mbits),
+        K(a.half + 1) {}
+  __device__ __forceinline__ int slot(float d) const {
+    const float c = __builtin_amdgcn_fmed3f(d, -dmax, dmax);
+    const float x = fmaf(fabsf(c), dmul, 2.f);
+    const int t = __builtin_amdgcn_ubfe(__builtin_bit_cast(unsigned, x),
+                                        shift, width);
+    const int s = __builtin_bit_cast(int, c) >> 31;
+    return (t ^ s) + K;
+  }
+};
+
+// Positions as floats, clamped to +-2^23 (their differences are exact).
+__device__ __forceinline__ float load_pos(const int* pos, int64_t i, int axes,
+                                          int axis) {
+  const int p = pos[i * axes + axis];
+  return (float)min(max(p, -(1 << 23)), 1 << 23);
+}
+
+// Dynamic LDS past 64 KB has to be asked for.
+inline void allow_lds(const void* kernel, size_t bytes) {
+  TORCH_CHECK(bytes <= 160 * 1024, "segment_attention: ", bytes,
+              " bytes of LDS");
+  if (bytes > 64 * 1024)
+    DGMC_CHECK_HIP(hipFuncSetAttribute(
+        kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+}
+
+// The group's bias tables -> LDS slots, times log2(e).
+__device__ __forceinline__ void load_table(const Args& a, int kvh,
+                                           DGMC_LDS float* tab, int axes) {
+  const int W = 2 * a.half + 2, w = 2 * a.half + 1;
+  for (int e = threadIdx.x; e < a.G * kSlots; e += blockDim.x) {
+    const int g = e / kSlots, s = e % kSlots;
+    int c = -1;
+    if (axes == 1) {
+      if (s < W && s != a.half) c = s < a.half ? s : s - 1;
+    } else if (s < W * W) {
+      const int x = s / W, y = s % W;
+      if (x != a.half && y != a.half)
+        c = (x < a.half ? x : x - 1) * w + (y < a.half ? y : y - 1);
+    }
+    float v = 0.f;
+    if (c >= 0) {
+      v = a.bias[(int64_t)(kvh * a.G + g) * a.nb + c];
+      if (v < kLowest && v > -INFINITY) v = kLowest;
+      v *= kLog2e;
+    }
+    tab[e] = v;
+  }
+}
+
+}  // namespace segattn
+}  // namespace dgmc

@@ -1,0 +1,11 @@
+// fp32 instances of the segment attention backward.
+#include "segment_attention_bwd.h"
+
+namespace dgmc {
+namespace segattn {
+void bwd_f32(const Args& a, int axes, int nwq, int nwk, int nblk,
+              hipStream_t st) {
+  run_bwd<float>(a, axes, nwq, nwk, nblk, st);
+}
+}  // namespace segattn
+}  // namespace dgmc

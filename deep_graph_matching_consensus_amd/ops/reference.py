@@ -129,3 +129,62 @@ def top_k(x_s, x_t, k):
     """Indices of the k largest inner products, best first (dgmc.py:85-94)."""
     S_ij = x_s @ x_t.transpose(-1, -2)
     return S_ij.topk(k, dim=2)[1]
+
+
+# --------------------------------------------------------------------------
+# Attention inside the segments of a packed batch
+# --------------------------------------------------------------------------
+def position_buckets(pos_q, pos_k, starts):
+    """``[n_q, n_k]`` column of the bias table of every pair of positions
+    (``[n, axes]``): ``half +- b`` per axis, the first axis most significant;
+    ``b`` is the last bucket of ``starts`` not beyond the distance."""
+    half = len(starts) - 1
+    edges = torch.tensor(starts[1:], dtype=torch.long, device=pos_q.device)
+    lim = 1 << 23
+    out = torch.zeros((pos_q.size(0), pos_k.size(0)), dtype=torch.long,
+                      device=pos_q.device)
+    for x in range(pos_q.size(1)):
+        d = pos_k[:, x].long().clamp(-lim, lim).view(1, -1) - \
+            pos_q[:, x].long().clamp(-lim, lim).view(-1, 1)
+        b = (d.abs().unsqueeze(-1) >= edges).sum(-1)
+        out = out * (2 * half + 1) + half + torch.sign(d) * b
+    return out
+
+
+def segment_attention(q, k, v, ptr_q, ptr_k, scale, cap=0.0, bias=None,
+                      pos_q=None, pos_k=None, starts=(0, )):
+    """Attention of every segment's rows over its keys, in fp32 (fp64 for
+    fp64 inputs), rounded once to ``q``'s dtype."""
+    acc = torch.float64 if q.dtype == torch.float64 else torch.float32
+    G = q.size(1) // k.size(1)
+    qa, ka, va = q.to(acc), k.to(acc), v.to(acc)
+    pq, pk = ptr_q.tolist(), ptr_k.tolist()
+    outs, rows = [], 0
+    never = torch.ones((), dtype=torch.bool, device=q.device)
+    for b in range(len(pq) - 1):
+        sq, sk = slice(pq[b], pq[b + 1]), slice(pk[b], pk[b + 1])
+        rows = pq[b + 1]
+        if pq[b + 1] == pq[b]:
+            continue
+        if pk[b + 1] == pk[b]:
+            outs.append(qa[sq].masked_fill(never, 0))
+            continue
+        qs = qa[sq].transpose(0, 1)
+        ks = ka[sk].repeat_interleave(G, dim=1).transpose(0, 1)
+        vs = va[sk].repeat_interleave(G, dim=1).transpose(0, 1)
+        z = scale * (qs @ ks.transpose(1, 2))
+        if cap:
+            z = cap * torch.tanh(z / cap)
+        if bias is not None:
+            z = z + bias.to(acc).clamp(min=-1e38).where(
+                bias > -float('inf'), bias.to(acc))[
+                    :, position_buckets(pos_q[sq], pos_k[sk], starts)]
+        # (a row of -inf everywhere gives 0, not NaN)
+        top = z.detach().amax(dim=-1, keepdim=True)
+        dead = top == -float('inf')
+        e = torch.exp(z - top.masked_fill(dead, 0))
+        p = e / e.sum(dim=-1, keepdim=True).masked_fill(dead, 1)
+        outs.append((p @ vs).transpose(0, 1))
+    if rows < q.size(0) or not outs:
+        outs.append(qa[rows:].masked_fill(never, 0))
+    return torch.cat(outs, dim=0).to(q.dtype)
