@@ -6,18 +6,18 @@
 
 namespace dgmc {
 namespace segattn {
-std::tuple<at::Tensor, at::Tensor> segment_attention_fwd(
+std::tuple<at::Tensor, at::Tensor, at::Tensor> segment_attention_fwd(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& ptr_q, const at::Tensor& ptr_k, double scale,
     double cap, const c10::optional<at::Tensor>& bias,
     const c10::optional<at::Tensor>& pos_q,
     const c10::optional<at::Tensor>& pos_k, int64_t half, int64_t mbits,
-    double dmax, bool with_lse);
+    double dmax, bool train);
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>
 segment_attention_bwd(const at::Tensor& dout, const at::Tensor& q,
                       const at::Tensor& k, const at::Tensor& v,
-                      const at::Tensor& out, const at::Tensor& lse,
-                      const at::Tensor& ptr_q, const at::Tensor& ptr_k,
+                      const at::Tensor& out, const at::Tensor& lo,
+                      const at::Tensor& lse, const at::Tensor& ptr_q, const at::Tensor& ptr_k,
                       double scale, double cap,
                       const c10::optional<at::Tensor>& bias,
                       const c10::optional<at::Tensor>& pos_q,
@@ -635,11 +635,11 @@ TORCH_LIBRARY(dgmc_amd, m) {
   m.def(
       "segment_attention_fwd(Tensor q, Tensor k, Tensor v, Tensor ptr_q, "
       "Tensor ptr_k, float scale, float cap, Tensor? bias, Tensor? pos_q, "
-      "Tensor? pos_k, int half, int mbits, float dmax, bool with_lse) -> "
-      "(Tensor, Tensor)");
+      "Tensor? pos_k, int half, int mbits, float dmax, bool train) -> "
+      "(Tensor, Tensor, Tensor)");
   m.def(
       "segment_attention_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, "
-      "Tensor out, Tensor lse, Tensor ptr_q, Tensor ptr_k, float scale, "
+      "Tensor out, Tensor lo, Tensor lse, Tensor ptr_q, Tensor ptr_k, float scale, "
       "float cap, Tensor? bias, Tensor? pos_q, Tensor? pos_k, int half, int "
       "mbits, float dmax) -> (Tensor, Tensor, Tensor, Tensor)");
 }

@@ -58,9 +58,10 @@ constexpr float kLowest = -1e38f;
 
 struct Args {
   const void *q, *k, *v, *o, *dout;
-  void *out, *dq, *dk, *dv;
+  void *out, *out_lo, *dq, *dk, *dv;  // out_lo: bf16 rest of out (training)
   float *lse, *delta;                 // [Nq, H]
-  float *part_o, *part_ml;            // splits: [S][Nq, H, D], [S][Nq, H, 2]
+  // Splits: [S][Nq, H, D] (dk, dv: [2][S][Nk, KV, D]) and [S][Nq, H, 2].
+  float *part_o, *part_ml;
   float *part_bias;                   // [blocks][KV][G][kSlots]
   const int *ptr_q, *ptr_k;
   const float* bias;                  // [H, nb]
@@ -69,8 +70,14 @@ struct Args {
   int B, Nq, Nk, H, KV, G, D, nb, half, mbits, slots;
   float scale, cap, dmax, dmul;
   int vec_q, vec_k, vec_v, vec_o, vec_g;   // 16-byte rows
-  int splits;
+  int splits, chunk;                  // most splits, least tiles of one
 };
+
+// Tiles of one split of an axis of n tiles: an even share of the splits, at
+// least `chunk` (a join costs more than a short split gains).
+__device__ __forceinline__ int split_tiles(const Args& a, int n) {
+  return max(a.chunk, (n + a.splits - 1) / a.splits);
+}
 
 // Segment `b` rows (clamped to [0, N]; the first segment starts at row 0,
 // "segment" B is the tail behind the last one).
@@ -139,6 +146,99 @@ __device__ __forceinline__ u32x4 load_chunk(const T* row, int ch, int D,
 }
 
 // --------------------------------------------------------------------------
+// Staging.  A tile is ROWS x CH 16-byte chunks, chunk ch of row r at slot
+// (r, ch ^ swz(r)).  Rows of 16-byte chunks go straight from global memory
+// to LDS (buffer_load_dwordx4 ... lds: no register in between, the loads of
+// the next tile stay in flight over the current one's products); a lane
+// fills slot (r, s) with chunk s ^ swz(r) and lanes without a row (or past
+// the width) carry an offset beyond the buffer's range, which reads zeros.
+// Other layouts are loaded value by value and written with ds_write.
+// --------------------------------------------------------------------------
+constexpr unsigned kNoRow = 0x80000000u;   // past every buffer's range
+
+template <typename T, int ROWS, int CH, int NT>
+struct Stager {
+  static constexpr int E = 16 / (int)sizeof(T);
+  static constexpr int N = (ROWS * CH + NT - 1) / NT;
+  static constexpr bool kFull = N * NT == ROWS * CH;
+
+  // Slot i of thread `tid`: its row and (global) chunk.
+  __device__ __forceinline__ static int row(int tid, int i) {
+    return (tid + i * NT) / CH;
+  }
+  __device__ __forceinline__ static int chunk(int tid, int i) {
+    return ((tid + i * NT) % CH) ^ swz<CH>(row(tid, i));
+  }
+  // `ok(row)`: the row is there, at `off(row)` bytes from `base` (below 2^31
+  // where vec is set).
+  template <typename Ok, typename Off>
+  __device__ __forceinline__ static void fill(const T* base, int D, int vec,
+                                              DGMC_LDS char* tile, Ok ok,
+                                              Off off) {
+    const int wave = threadIdx.x >> 6;
+    if (vec) {
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<T*>(base), 0, 0x80000000u, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (!kFull && i * NT + wave * 64 >= ROWS * CH) continue;
+        const int ch = chunk(threadIdx.x, i), r = row(threadIdx.x, i);
+        const unsigned o =
+            ok(r) && ch * E < D ? (unsigned)off(r) + ch * 16 : kNoRow;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rs, (DGMC_LDS void*)(tile + (i * NT + wave * 64) * 16), 16, o, 0,
+            0, 0);
+      }
+    } else {
+      // (opaque: nothing of this path is kept in registers over the loop)
+      int tid = threadIdx.x;
+      asm volatile("" : "+v"(tid));
+#pragma unroll 1
+      for (int i = 0; i < N; ++i) {
+        if (!kFull && tid + i * NT >= ROWS * CH) continue;
+        const int ch = chunk(tid, i), r = row(tid, i);
+        const u32x4 v = load_chunk<T>(
+            (const T*)((const char*)base + off(r)), ch, D, ok(r), 0);
+        *(DGMC_LDS u32x4*)(tile + (tid + i * NT) * 16) = v;
+      }
+    }
+  }
+};
+
+// The 16-byte chunks h, h + 2, .. of this lane's own row (an MFMA operand):
+// at `off` bytes from the wave-uniform `base`, zeros where it is not `live`.
+// All loads are issued before the first is needed (no branch around them).
+template <typename T, int N>
+__device__ __forceinline__ void load_frags(u32x4 (&f)[N], const T* base,
+                                           int64_t off, bool live, int D,
+                                           int vec) {
+  constexpr int E = 16 / (int)sizeof(T);
+  const int h = (threadIdx.x >> 5) & 1;
+  if (vec) {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<T*>(base), 0, 0x80000000u, 0x00020000);
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+      const int ch = 2 * s + h;
+      f[s] = __builtin_amdgcn_raw_buffer_load_b128(
+          rs, live && ch * E < D ? (unsigned)off + ch * 16 : kNoRow, 0, 0);
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < N; ++s)
+      f[s] = load_chunk<T>((const T*)((const char*)base + off), 2 * s + h, D,
+                           live, 0);
+  }
+}
+
+// Every wave's staged data (and LDS reads) done, then the barrier.
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// --------------------------------------------------------------------------
 // Matrix core policies
 // --------------------------------------------------------------------------
 template <typename T> struct Mma;
@@ -151,8 +251,8 @@ template <> struct Mma<__bf16> {
         0);
   }
   // acc[blk] += tile^T p: rows of `tile` (32 from row0) are the K index, in
-  // the accumulator's row order.
-  template <int DP>
+  // the accumulator's row order.  FINE: p as the sum of two bf16 terms.
+  template <int DP, bool FINE = false>
   __device__ __forceinline__ static void accum(f32x16 (&acc)[DP / 32],
                                                const DGMC_LDS char* tile,
                                                int row0, f32x16 p) {
@@ -162,9 +262,14 @@ template <> struct Mma<__bf16> {
               pp = lane & 3;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      bf16x8 b;
+      bf16x8 b, lo_b;
 #pragma unroll
       for (int i = 0; i < 8; ++i) b[i] = (__bf16)p[8 * c + i];
+      if constexpr (FINE) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          lo_b[i] = (__bf16)(p[8 * c + i] - (float)b[i]);
+      }
       const int r0 = row0 + 16 * c + 4 * h + q, r1 = r0 + 8;
 #pragma unroll
       for (int k = 0; k < DP / 32; ++k) {
@@ -179,6 +284,9 @@ template <> struct Mma<__bf16> {
                                                    6, 7);
         acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
             __builtin_bit_cast(bf16x8, both), b, acc[k], 0, 0, 0);
+        if constexpr (FINE)
+          acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              __builtin_bit_cast(bf16x8, both), lo_b, acc[k], 0, 0, 0);
       }
     }
   }
@@ -201,7 +309,7 @@ template <> struct Mma<float> {
       c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
     return c;
   }
-  template <int DP>
+  template <int DP, bool FINE = false>
   __device__ __forceinline__ static void accum(f32x16 (&acc)[DP / 32],
                                                const DGMC_LDS char* tile,
                                                int row0, f32x16 p) {
@@ -226,6 +334,20 @@ template <> struct Mma<float> {
     return (x[0] * y[0] + x[1] * y[1]) + (x[2] * y[2] + x[3] * y[3]);
   }
 };
+
+// Four values of an output row of D at d (d % 4 == 0).
+template <typename T>
+__device__ __forceinline__ void put4(T* row, int d, int D, const T* v) {
+  if (D % 4 == 0) {
+    if (d < D)
+      __builtin_memcpy(__builtin_assume_aligned(row + d, 4 * sizeof(T)), v,
+                       4 * sizeof(T));
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (d + r < D) row[d + r] = v[r];
+  }
+}
 
 // Chunk (row, ch) of a swizzled LDS tile.
 template <int CH>
@@ -281,6 +403,13 @@ __device__ __forceinline__ float load_pos(const int* pos, int64_t i, int axes,
                                           int axis) {
   const int p = pos[i * axes + axis];
   return (float)min(max(p, -(1 << 23)), 1 << 23);
+}
+
+// Keys of a forward tile: 64 while both buffers of K and V fit 64 KB of LDS
+// (128 KB at dim 128, fp32: 32).
+inline int fwd_keys(int D, int nw, bool f32) {
+  const int DP = D <= 32 ? 32 : D <= 64 ? 64 : 128;
+  return nw > 1 && DP * (f32 ? 4 : 2) <= 256 ? 64 : 32;
 }
 
 // Dynamic LDS past 64 KB has to be asked for.

@@ -7,68 +7,168 @@ namespace dgmc {
 namespace segattn {
 
 void fwd_bf16(const Args& a, int axes, int nw, hipStream_t st);
+void fwd_bf16_fine(const Args& a, int axes, int nw, hipStream_t st);
 void fwd_f32(const Args& a, int axes, int nw, hipStream_t st);
-void bwd_bf16(const Args& a, int axes, int nwq, int nwk, int nblk,
-              hipStream_t st);
-void bwd_f32(const Args& a, int axes, int nwq, int nwk, int nblk,
-             hipStream_t st);
+void dq_bf16(const Args& a, int axes, int nw, int nblk, hipStream_t st);
+void dq_f32(const Args& a, int axes, int nw, int nblk, hipStream_t st);
+void dkv_bf16(const Args& a, int axes, int nw, hipStream_t st);
+void dkv_f32(const Args& a, int axes, int nw, hipStream_t st);
 
-constexpr int kMaxSplits = 64;        // one per lane of the joining wave
+constexpr int kMaxSplits = 64;
 
-// One wave per (row, head): o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s
-// over the splits in order.
-template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(const Args a) {
-  const int64_t rows = (int64_t)a.Nq * a.H;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 63;
-  float m = -INFINITY, l = 0.f;
-  if (lane < a.splits) {
-    m = a.part_ml[(lane * rows + row) * 2];
-    l = a.part_ml[(lane * rows + row) * 2 + 1];
-  }
-  const float M = wave_max(m);
-  // (a split without a finite score has l = 0: weight 0)
-  const float w = l == 0.f ? 0.f : exp2_(m - M);
-  const float L = wave_sum(w * l);
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  float o[2] = {0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
-    const float ws = lane_of(w, s);
-    const float* p = a.part_o + (s * rows + row) * a.D;
+// Join of the split rows (FWD: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M)
+// l_s; DQ, DKV: plain sums), in order of the splits.  A workgroup takes the
+// rows of one tile of the kernel whose splits it joins; 16 threads a row, 8
+// values each (dim <= 128), and where a tile has few rows the splits of a row are shared
+// out to several such groups (their sums added in order).
+enum { FWD, DQ, DKV };
+
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void join_kernel(const Args a, int per_tile,
+                                                   int key_tile) {
+  __shared__ float red[256][9];
+  __shared__ float wsum[16];
+  const int kvh = blockIdx.x % a.KV, slot = blockIdx.x / a.KV;
+  const int* own = MODE == DKV ? a.ptr_k : a.ptr_q;
+  const int* other = MODE == DKV ? a.ptr_q : a.ptr_k;
+  const int N = MODE == DKV ? a.Nk : a.Nq, No = MODE == DKV ? a.Nq : a.Nk;
+  const int seg = find_segment(own, a.B, N, per_tile, slot);
+  if (seg >= a.B) return;
+  int lo, hi, o_lo, o_hi;
+  seg_range(own, seg, a.B, N, lo, hi);
+  lo += (slot - (seg_begin(own, seg, N) / per_tile + seg)) * per_tile;
+  if (lo >= hi) return;
+  seg_range(other, seg, a.B, No, o_lo, o_hi);
+  const int ntile = (o_hi - o_lo + key_tile - 1) / key_tile;
+  const int per = split_tiles(a, ntile);
+  if (per >= ntile) return;
+  const int ns = (ntile + per - 1) / per;
+
+  const int G = MODE == DKV ? 1 : a.G, heads = G * a.KV;
+  const int rows = min(per_tile, hi - lo) * G;
+  const int64_t all = (int64_t)N * heads;
+  const int grp = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
+  // `ways` (a power of two) groups share a row; 16 / ways rows a round.
+  int ways = 1;
+  while (ways < 16 && 2 * ways * rows <= 16 && ways < ns) ways *= 2;
+  const int rpr = 16 / ways, rr = grp / ways, way = grp % ways;
+  const float* part =
+      a.part_o + (MODE == DKV ? blockIdx.y * a.splits * all * a.D : 0);
+  for (int r0 = blockIdx.z * rpr; r0 < rows; r0 += rpr * gridDim.z) {
+    const int r = r0 + rr;
+    const bool live = r < rows;
+    const int64_t row =
+        (int64_t)(lo + r / G) * heads + kvh * G + r % G;
+    float M = -INFINITY, L = 0.f, o[8];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-      if (lane + 64 * k < a.D && ws != 0.f) o[k] += ws * p[lane + 64 * k];
-  }
-  T* out = (T*)a.out + row * a.D;
+    for (int k = 0; k < 8; ++k) o[k] = 0.f;
+    if (live) {
+      if (MODE == FWD) {
+#pragma unroll 4
+        for (int s = 0; s < ns; ++s)
+          M = fmaxf(M, a.part_ml[(s * all + row) * 2]);
+        if (M == -INFINITY) M = 0.f;
+      }
+#pragma unroll 4
+      for (int s = way; s < ns; s += ways) {
+        float w = 1.f;
+        if (MODE == FWD) {
+          w = exp2_(a.part_ml[(s * all + row) * 2] - M);
+          L += w * a.part_ml[(s * all + row) * 2 + 1];
+        }
+        const float* p = part + (s * all + row) * a.D;
+        if (a.D % 4 == 0 && d0 + 8 <= a.D) {
+          const f32x4 x = *(const f32x4*)(p + d0),
+                      y = *(const f32x4*)(p + d0 + 4);
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (lane + 64 * k < a.D) out[lane + 64 * k] = (T)(o[k] * inv);
-  if (lane == 0 && a.lse) a.lse[row] = L == 0.f ? INFINITY : M + log2f(L);
+          for (int k = 0; k < 4; ++k) {
+            o[k] += w * x[k];
+            o[4 + k] += w * y[k];
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (d0 + k < a.D) o[k] += w * p[d0 + k];
+        }
+      }
+    }
+    if (ways > 1) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) red[threadIdx.x][k] = o[k];
+      if ((threadIdx.x & 15) == 0) wsum[grp] = L;
+      __syncthreads();
+      if (way == 0) {
+        for (int w = 1; w < ways; ++w) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) o[k] += red[threadIdx.x + 16 * w][k];
+          L += wsum[grp + w];
+        }
+      }
+      __syncthreads();
+    }
+    if (!live || way != 0) continue;
+    const float f = MODE == FWD ? (L == 0.f ? 0.f : 1.f / L)
+                    : MODE == DKV && blockIdx.y == 1 ? 1.f
+                                                     : a.scale;
+    T* out = (T*)(MODE == FWD  ? a.out
+                  : MODE == DQ ? a.dq
+                               : (blockIdx.y ? a.dv : a.dk)) +
+             row * a.D;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (d0 + k < a.D) {
+        const T v = (T)(o[k] * f);
+        out[d0 + k] = v;
+        if (MODE == FWD && a.out_lo)
+          ((T*)a.out_lo)[row * a.D + d0 + k] = (T)(o[k] * f - (float)v);
+      }
+    if (MODE == FWD && a.lse && d0 == 0)
+      a.lse[row] = L == 0.f ? INFINITY : M + log2f(L);
+  }
 }
 
-// dT[head][c] = sum over the workgroups' parts, in order.  One workgroup per
-// head: 4 lanes groups of 64 slots each take every fourth part.
-__global__ __launch_bounds__(256) void bias_sum_kernel(
+template <int MODE>
+static void join(const Args& a, bool f32, int per_tile, int key_tile) {
+  const int N = MODE == DKV ? a.Nk : a.Nq;
+  // (workgroups along z share a tile's rows, 16 a round)
+  const int G = MODE == DKV ? 1 : a.G;
+  const dim3 grid((N / per_tile + a.B + 1) * a.KV, MODE == DKV ? 2 : 1,
+                  (per_tile * G + 15) / 16);
+  if (f32)
+    join_kernel<float, MODE><<<grid, 256, 0, stream()>>>(a, per_tile,
+                                                         key_tile);
+  else
+    join_kernel<__bf16, MODE><<<grid, 256, 0, stream()>>>(a, per_tile,
+                                                          key_tile);
+  DGMC_CHECK_LAUNCH();
+}
+
+// dT[head][c] = sum over the workgroups' parts, in a fixed order: one
+// workgroup per head, 16 threads a slot, each of which takes every 16th part
+// (eight loads in flight); their sums are added in order.
+constexpr int kSumWays = 16;
+
+__global__ __launch_bounds__(kSlots * kSumWays) void bias_sum_kernel(
     const float* __restrict__ part, float* __restrict__ out, int nblk, int KV,
     int G, int slots, int nb, int half, int axes) {
-  __shared__ float red[4][kSlots];
+  __shared__ float red[kSumWays][kSlots];
   const int head = blockIdx.x, kvh = head / G, g = head % G;
   const int s = threadIdx.x & 63, p = threadIdx.x >> 6;
+  const float* src = part + ((int64_t)kvh * G + g) * slots + min(s, slots - 1);
+  const int64_t step = (int64_t)KV * G * slots;
   float sum = 0.f;
-  if (s < slots)
-    for (int b = p; b < nblk; b += 4)
-      sum += part[(((int64_t)b * KV + kvh) * G + g) * slots + s];
+#pragma unroll 8
+  for (int b = p; b < nblk; b += kSumWays) sum += src[b * step];
   red[p][s] = sum;
   __syncthreads();
-  if (threadIdx.x >= nb) return;
+  if ((int)threadIdx.x >= nb) return;
   const int c = threadIdx.x, w = 2 * half + 1, W = w + 1;
   const int y = c % w, x = axes == 1 ? 0 : c / w;
   const int ys = y < half ? y : y + 1, xs = x < half ? x : x + 1;
   const int t = axes == 1 ? ys : xs * W + ys;
-  out[(int64_t)head * nb + c] =
-      (red[0][t] + red[1][t]) + (red[2][t] + red[3][t]);
+  sum = 0.f;
+  for (int k = 0; k < kSumWays; ++k) sum += red[k][t];
+  out[(int64_t)head * nb + c] = sum;
 }
 
 static void check_heads(const at::Tensor& t, const char* name,
@@ -93,11 +193,14 @@ static void check_index(const at::Tensor& t, const char* name, int dim,
 }
 
 // 16-byte loads of whole rows: base, row and head strides and the width are
-// multiples of 16 bytes.
+// multiples of 16 bytes, and a tile (64 rows, 32 heads) spans less than the
+// 2^31 bytes of a buffer's offsets.
 static int rows16(const at::Tensor& t) {
   const int64_t e = 16 / t.element_size();
   return t.size(2) % e == 0 && t.stride(0) % e == 0 && t.stride(1) % e == 0 &&
-         aligned16(t.data_ptr());
+         aligned16(t.data_ptr()) &&
+         (64 * t.stride(0) + 32 * t.stride(1) + 128) * t.element_size() <
+             ((int64_t)1 << 31);
 }
 
 static Args make_args(const at::Tensor& q, const at::Tensor& k,
@@ -184,59 +287,61 @@ static int waves_for(int64_t rows, int64_t B) {
   return rows > 64 * std::max<int64_t>(B, 1) ? 4 : 1;
 }
 
-std::tuple<at::Tensor, at::Tensor> segment_attention_fwd(
+// Splits of the other axis (`n` rows in tiles of `tile`) where the `tiles`
+// of the own axis are too few or too uneven to fill the chip: up to 1024
+// workgroups, no split under kChunk tiles.  False: none.
+constexpr int kChunk = 8;
+static bool split_axis(Args& a, int64_t tiles, int64_t n, int tile) {
+  tiles = std::max<int64_t>(tiles, 1) * a.KV;
+  a.chunk = kChunk;
+  a.splits = (int)std::max<int64_t>(
+      1, std::min<int64_t>({(1024 + tiles - 1) / tiles,
+                            n / ((int64_t)tile * kChunk), kMaxSplits}));
+  return a.splits > 1;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> segment_attention_fwd(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& ptr_q, const at::Tensor& ptr_k, double scale,
     double cap, const c10::optional<at::Tensor>& bias,
     const c10::optional<at::Tensor>& pos_q,
     const c10::optional<at::Tensor>& pos_k, int64_t half, int64_t mbits,
-    double dmax, bool with_lse) {
+    double dmax, bool train) {
   int axes;
   Args a = make_args(q, k, v, ptr_q, ptr_k, scale, cap, bias, pos_q, pos_k,
                      half, mbits, dmax, axes);
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   const auto f32 = q.options().dtype(at::kFloat);
   at::Tensor out = at::empty({a.Nq, a.H, a.D}, q.options());
-  at::Tensor lse = at::empty({with_lse ? a.Nq : 0, a.H}, f32);
-  if (a.Nq == 0) return {out, lse};
+  at::Tensor lse = at::empty({train ? a.Nq : 0, a.H}, f32);
+  // bf16 training keeps the rest of the output's rounding for delta.
+  const bool f = q.scalar_type() == at::kFloat, fine = train && !f;
+  at::Tensor lo = at::empty({fine ? a.Nq : 0, a.H, a.D}, q.options());
+  if (a.Nq == 0) return {out, lo, lse};
   a.out = out.data_ptr();
-  a.lse = with_lse ? lse.data_ptr<float>() : nullptr;
+  a.out_lo = fine ? lo.data_ptr() : nullptr;
+  a.lse = train ? lse.data_ptr<float>() : nullptr;
   const int nw = waves_for((int64_t)a.Nq * a.G, a.B);
-  // Few rows over long segments: the keys are split until about four
-  // workgroups per CU run, each of two tiles at least.
-  const int64_t tiles =
-      std::max<int64_t>(a.Nq / (32 / a.G * nw), std::min(a.B, a.Nq)) * a.KV;
-  const int64_t keys = a.Nk / std::max(a.B, 1);
-  if (tiles < 512)
-    a.splits = (int)std::max<int64_t>(
-        1, std::min<int64_t>({(1024 + tiles - 1) / std::max<int64_t>(tiles, 1),
-                              keys / 128, kMaxSplits}));
+  const int TQ = 32 / a.G * nw, KT = fwd_keys(a.D, nw, f);
   at::Tensor po, pml;
-  if (a.splits > 1) {
+  if (split_axis(a, a.Nq / TQ, a.Nk, KT)) {
     po = at::empty({a.splits, a.Nq, a.H, a.D}, f32);
     pml = at::empty({a.splits, a.Nq, a.H, 2}, f32);
     a.part_o = po.data_ptr<float>();
     a.part_ml = pml.data_ptr<float>();
   }
-  const bool f = q.scalar_type() == at::kFloat;
-  f ? fwd_f32(a, axes, nw, stream()) : fwd_bf16(a, axes, nw, stream());
-  if (a.splits > 1) {
-    const int64_t rows = (int64_t)a.Nq * a.H;
-    const dim3 grid((unsigned)((rows + 3) / 4));
-    if (f)
-      join_kernel<float><<<grid, 256, 0, stream()>>>(a);
-    else
-      join_kernel<__bf16><<<grid, 256, 0, stream()>>>(a);
-    DGMC_CHECK_LAUNCH();
-  }
-  return {out, lse};
+  f      ? fwd_f32(a, axes, nw, stream())
+  : fine ? fwd_bf16_fine(a, axes, nw, stream())
+         : fwd_bf16(a, axes, nw, stream());
+  if (a.splits > 1) join<FWD>(a, f, TQ, KT);
+  return {out, lo, lse};
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>
 segment_attention_bwd(const at::Tensor& dout, const at::Tensor& q,
                       const at::Tensor& k, const at::Tensor& v,
-                      const at::Tensor& out, const at::Tensor& lse,
-                      const at::Tensor& ptr_q, const at::Tensor& ptr_k,
+                      const at::Tensor& out, const at::Tensor& lo,
+                      const at::Tensor& lse, const at::Tensor& ptr_q, const at::Tensor& ptr_k,
                       double scale, double cap,
                       const c10::optional<at::Tensor>& bias,
                       const c10::optional<at::Tensor>& pos_q,
@@ -267,32 +372,53 @@ segment_attention_bwd(const at::Tensor& dout, const at::Tensor& q,
     return {dq, dk, dv, dbias};
   }
   at::Tensor delta = at::empty({a.Nq, a.H}, f32);
+  TORCH_CHECK(q.scalar_type() == at::kFloat ||
+                  (lo.sizes() == q.sizes() && lo.is_contiguous() &&
+                   lo.scalar_type() == q.scalar_type() &&
+                   lo.device() == q.device()),
+              "segment_attention: lo must have q's shape");
   a.o = out.data_ptr();
+  a.out_lo = lo.data_ptr();
   a.dout = dout.data_ptr();
   a.g_sn = dout.stride(0); a.g_sh = dout.stride(1);
   a.vec_g = rows16(dout); a.vec_o = rows16(out);
   a.lse = lse.data_ptr<float>();
   a.delta = delta.data_ptr<float>();
   a.dq = dq.data_ptr();
-  a.dk = a.Nk ? dk.data_ptr() : nullptr;
-  a.dv = a.Nk ? dv.data_ptr() : nullptr;
+  a.dk = dk.data_ptr();
+  a.dv = dv.data_ptr();
+  const bool f = q.scalar_type() == at::kFloat;
   const int nwq = waves_for((int64_t)a.Nq * a.G, a.B);
   const int nwk = waves_for(a.Nk, a.B);
+  const int TQ = 32 / a.G * nwq;
+  at::Tensor pq, pk;
+  if (split_axis(a, a.Nq / TQ, a.Nk, 32)) {
+    pq = at::empty({a.splits, a.Nq, a.H, a.D}, f32);
+    a.part_o = pq.data_ptr<float>();
+  }
   // Workgroups of the dq kernel with a table: each keeps its LDS columns
   // over all of its tiles.
   int nblk = 0;
   at::Tensor part;
   if (axes) {
-    const int nslot = a.Nq / (32 / a.G * nwq) + a.B + 1;
-    nblk = std::max(1, std::min(nslot, 2048 / (a.KV * nwq)));
+    const int items = (a.Nq / TQ + a.B + 1) * a.splits;
+    nblk = std::max(1, std::min(items, 2048 / (a.KV * nwq)));
     part = at::empty({nblk, a.KV, a.G, a.slots}, f32);
     a.part_bias = part.data_ptr<float>();
   }
-  q.scalar_type() == at::kFloat
-      ? bwd_f32(a, axes, nwq, nwk, nblk, stream())
-      : bwd_bf16(a, axes, nwq, nwk, nblk, stream());
+  f ? dq_f32(a, axes, nwq, nblk, stream())
+    : dq_bf16(a, axes, nwq, nblk, stream());
+  if (a.splits > 1) join<DQ>(a, f, TQ, 32);
+  if (a.Nk > 0) {
+    if (split_axis(a, a.Nk / (32 * nwk), a.Nq, 32 / a.G)) {
+      pk = at::empty({2, a.splits, a.Nk, a.KV, a.D}, f32);
+      a.part_o = pk.data_ptr<float>();
+    }
+    f ? dkv_f32(a, axes, nwk, stream()) : dkv_bf16(a, axes, nwk, stream());
+    if (a.splits > 1) join<DKV>(a, f, 32 * nwk, 32 / a.G);
+  }
   if (axes) {
-    bias_sum_kernel<<<a.H, 256, 0, stream()>>>(
+    bias_sum_kernel<<<a.H, kSlots * kSumWays, 0, stream()>>>(
         a.part_bias, dbias.data_ptr<float>(), nblk, a.KV, a.G, a.slots, a.nb,
         a.half, axes);
     DGMC_CHECK_LAUNCH();

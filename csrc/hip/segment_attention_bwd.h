@@ -42,13 +42,66 @@ __device__ __forceinline__ void cap_scores(const Args& a, f32x16& z,
   }
 }
 
+// hist[sl[r]] += v[r] in a lane's own LDS column, in order.  A plain read,
+// add, write: ds_add_f32 took 120 cycles and more a wave (ragged case: 552
+// us, without the table 139 us).  Four at a time: equal slots among the four
+// take the earlier ones' values along and the last write counts.  RUNS: all
+// 16 in one slot (nodes in order, far apart) are added first.
+template <bool RUNS>
+__device__ __forceinline__ void add_slots(DGMC_LDS float* hist,
+                                          const int (&sl)[16], f32x16 v) {
+  if constexpr (RUNS) {
+    int lo = sl[0], hi = sl[0];
+    float s = v[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) {
+      lo = min(lo, sl[r]);
+      hi = max(hi, sl[r]);
+      s += v[r];
+    }
+    if (__all(lo == hi)) {
+      hist[lo * 64] += s;
+      return;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 16; k += 4) {
+    const int a = sl[k], b = sl[k + 1], c = sl[k + 2], d = sl[k + 3];
+    const float ha = hist[a * 64], hb = hist[b * 64], hc = hist[c * 64],
+                hd = hist[d * 64];
+    const float va = v[k], vb = v[k + 1] + (a == b ? va : 0.f);
+    const float vc = v[k + 2] + (b == c ? vb : a == c ? va : 0.f);
+    const float vd =
+        v[k + 3] + (c == d ? vc : b == d ? vb : a == d ? va : 0.f);
+    hist[a * 64] = ha + va;
+    hist[b * 64] = hb + vb;
+    hist[c * 64] = hc + vc;
+    hist[d * 64] = hd + vd;
+  }
+}
+
+// A wave's accumulators -> its lanes' output rows.
+template <int DP, typename T>
+__device__ __forceinline__ void put_acc(T* row, const f32x16 (&acc)[DP / 32],
+                                        int D, float scale) {
+  const int h = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      T o[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = (T)(acc[k][4 * r4 + r] * scale);
+      put4(row, 32 * k + 8 * r4 + 4 * h, D, o);
+    }
+}
+
 template <typename T, int DP, int NW, int POS>
-__global__ __launch_bounds__(NW * 64, 1) void dq_kernel(const Args a,
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(const Args a,
                                                         int nslot) {
   constexpr int KT = 32;
   constexpr int CH = DP * (int)sizeof(T) / 16;
   constexpr int NT = NW * 64;
-  constexpr int LD = (KT * CH + NT - 1) / NT;
   constexpr int TB = KT * CH * 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   DGMC_LDS char* lds = (DGMC_LDS char*)smem;
@@ -70,10 +123,10 @@ __global__ __launch_bounds__(NW * 64, 1) void dq_kernel(const Args a,
     load_table(a, kvh, tab, POS);
     for (int s = 0; s < a.slots; ++s) myhist[s * 64] = 0.f;
   }
-  const T* kbase = (const T*)a.k + (int64_t)kvh * a.k_sh;
-  const T* vbase = (const T*)a.v + (int64_t)kvh * a.v_sh;
+  const int64_t ksb = a.k_sn * (int)sizeof(T), vsb = a.v_sn * (int)sizeof(T);
 
-  for (int slot = blk; slot < nslot; slot += nblk) {
+  for (int it = blk; it < nslot * a.splits; it += nblk) {
+    const int slot = it / a.splits, split = it % a.splits;
     const int seg = find_segment(a.ptr_q, a.B, a.Nq, TQ, slot);
     int q_lo, q_hi, k_lo = 0, k_hi = 0;
     seg_range(a.ptr_q, seg, a.B, a.Nq, q_lo, q_hi);
@@ -84,58 +137,65 @@ __global__ __launch_bounds__(NW * 64, 1) void dq_kernel(const Args a,
     const int64_t qi = (int64_t)q_lo + wave * QW + c / a.G;
     const bool live = c < QW * a.G && qi < q_hi;
     const int64_t row = qi * a.H + head;
-    const T* qrow = (const T*)a.q + qi * a.q_sn + (int64_t)head * a.q_sh;
-    const T* grow = (const T*)a.dout + qi * a.g_sn + (int64_t)head * a.g_sh;
-    const T* orow = (const T*)a.o + row * a.D;
-    u32x4 qf[CH / 2], gf[CH / 2];
+    const int ntile = (k_hi - k_lo + KT - 1) / KT;
+    const int per = split_tiles(a, ntile);
+    const int t0 = split * per, t1 = min(t0 + per, ntile);
+    if (split > 0 && t0 >= t1) continue;
+    const int qo = wave * QW + c / a.G;
+    u32x4 qf[CH / 2], gf[CH / 2], of[CH / 2];
+    load_frags<T>(qf,
+                  (const T*)a.q + (int64_t)q_lo * a.q_sn +
+                      (int64_t)kvh * a.G * a.q_sh,
+                  (qo * a.q_sn + g * a.q_sh) * (int64_t)sizeof(T), live, a.D,
+                  a.vec_q);
+    load_frags<T>(gf,
+                  (const T*)a.dout + (int64_t)q_lo * a.g_sn +
+                      (int64_t)kvh * a.G * a.g_sh,
+                  (qo * a.g_sn + g * a.g_sh) * (int64_t)sizeof(T), live, a.D,
+                  a.vec_g);
+    const int64_t ob = ((int64_t)q_lo * a.H + kvh * a.G) * a.D;
+    const int64_t oo = ((int64_t)qo * a.H + g) * a.D * (int64_t)sizeof(T);
+    load_frags<T>(of, (const T*)a.o + ob, oo, live, a.D, a.vec_o);
+    const float lse = live ? a.lse[row] : INFINITY;
     float dl = 0.f;
 #pragma unroll
-    for (int s = 0; s < CH / 2; ++s) {
-      qf[s] = load_chunk<T>(qrow, 2 * s + h, a.D, live, a.vec_q);
-      gf[s] = load_chunk<T>(grow, 2 * s + h, a.D, live, a.vec_g);
-      dl += Mma<T>::chunk_dot(
-          gf[s], load_chunk<T>(orow, 2 * s + h, a.D, live, a.vec_o));
+    for (int s = 0; s < CH / 2; ++s) dl += Mma<T>::chunk_dot(gf[s], of[s]);
+    if constexpr (sizeof(T) == 2) {
+      load_frags<T>(of, (const T*)a.out_lo + ob, oo, live, a.D, a.vec_o);
+#pragma unroll
+      for (int s = 0; s < CH / 2; ++s) dl += Mma<T>::chunk_dot(gf[s], of[s]);
     }
     dl = sum_half(dl);
-    const float lse = live ? a.lse[row] : INFINITY;
-    if (live && h == 0) a.delta[row] = dl;
+    if (live && h == 0 && split == 0) a.delta[row] = dl;
     float px = 0.f, py = 0.f;
     if (POS > 0 && live) {
       px = load_pos(a.pos_q, qi, POS, 0);
       if (POS == 2) py = load_pos(a.pos_q, qi, POS, 1);
     }
 
-    const int ntile = (k_hi - k_lo + KT - 1) / KT;
-    u32x4 kr[LD], vr[LD];
+    const T* kbase =
+        (const T*)a.k + (int64_t)k_lo * a.k_sn + (int64_t)kvh * a.k_sh;
+    const T* vbase =
+        (const T*)a.v + (int64_t)k_lo * a.v_sn + (int64_t)kvh * a.v_sh;
     float pr[2] = {0.f, 0.f};
-    auto fetch = [&](int t) {
-      const int k0 = k_lo + t * KT;
-#pragma unroll
-      for (int i = 0; i < LD; ++i) {
-        const int e = tid + i * NT, rw = e / CH, ch = e % CH;
-        const int64_t j = (int64_t)k0 + rw;
-        const bool ok = rw < KT && j < k_hi;
-        kr[i] = load_chunk<T>(kbase + j * a.k_sn, ch, a.D, ok, a.vec_k);
-        vr[i] = load_chunk<T>(vbase + j * a.v_sn, ch, a.D, ok, a.vec_v);
-      }
+    auto fetch = [&](int t, int buf) {
+      using S = Stager<T, KT, CH, NT>;
+      const int left = k_hi - k_lo - t * KT;
+      DGMC_LDS char* kt = lds + buf * 2 * TB;
+      const auto ok = [&](int r) { return r < left; };
+      S::fill(kbase + (int64_t)t * KT * a.k_sn, a.D, a.vec_k, kt, ok,
+              [&](int r) { return r * ksb; });
+      S::fill(vbase + (int64_t)t * KT * a.v_sn, a.D, a.vec_v, kt + TB, ok,
+              [&](int r) { return r * vsb; });
       if constexpr (POS > 0) {
-        if (tid < KT && k0 + tid < k_hi) {
-          pr[0] = load_pos(a.pos_k, (int64_t)k0 + tid, POS, 0);
-          if (POS == 2) pr[1] = load_pos(a.pos_k, (int64_t)k0 + tid, POS, 1);
+        if (tid < KT && tid < left) {
+          const int64_t j = (int64_t)k_lo + t * KT + tid;
+          pr[0] = load_pos(a.pos_k, j, POS, 0);
+          if (POS == 2) pr[1] = load_pos(a.pos_k, j, POS, 1);
         }
       }
     };
-    auto stage = [&](int buf) {
-      DGMC_LDS char* kt = lds + buf * 2 * TB;
-#pragma unroll
-      for (int i = 0; i < LD; ++i) {
-        const int e = tid + i * NT, rw = e / CH, ch = e % CH;
-        if (LD * NT == KT * CH || rw < KT) {
-          const int off = (rw * CH + (ch ^ swz<CH>(rw))) * 16;
-          *(DGMC_LDS u32x4*)(kt + off) = kr[i];
-          *(DGMC_LDS u32x4*)(kt + TB + off) = vr[i];
-        }
-      }
+    auto put_pos = [&](int buf) {
       if constexpr (POS > 0) {
         if (tid < KT) {
           kpos[(buf * 2 + 0) * KT + tid] = pr[0];
@@ -150,13 +210,13 @@ __global__ __launch_bounds__(NW * 64, 1) void dq_kernel(const Args a,
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[k][r] = 0.f;
 
-    if (ntile > 0) fetch(0);
-    __syncthreads();       // the previous slot's last tile has been read
-    for (int t = 0; t < ntile; ++t) {
-      const int buf = t & 1;
-      stage(buf);
-      if (t + 1 < ntile) fetch(t + 1);
-      __syncthreads();
+    stage_barrier();       // the previous slot's last tile has been read
+    if (t0 < t1) fetch(t0, 0);
+    for (int t = t0; t < t1; ++t) {
+      const int buf = (t - t0) & 1;
+      put_pos(buf);
+      stage_barrier();
+      if (t + 1 < t1) fetch(t + 1, buf ^ 1);
       const DGMC_LDS char* kt = lds + buf * 2 * TB;
       f32x16 z, dp, th;
 #pragma unroll
@@ -196,10 +256,7 @@ __global__ __launch_bounds__(NW * 64, 1) void dq_kernel(const Args a,
       for (int r = 0; r < 16; ++r)
         z[r] = exp2_(z[r] - lse) * (dp[r] - dl);
       if constexpr (POS > 0) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          __hip_atomic_fetch_add(myhist + sl[r] * 64, z[r], __ATOMIC_RELAXED,
-                                 __HIP_MEMORY_SCOPE_WORKGROUP);
+        add_slots<POS == 1>(myhist, sl, z);
       }
       if (a.cap > 0.f) {
 #pragma unroll
@@ -207,15 +264,12 @@ __global__ __launch_bounds__(NW * 64, 1) void dq_kernel(const Args a,
       }
       Mma<T>::template accum<DP>(acc, kt, 0, z);
     }
-    if (live && a.dq != nullptr) {
-      T* drow = (T*)a.dq + row * a.D;
-#pragma unroll
-      for (int k = 0; k < DP / 32; ++k)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int d = 32 * k + 8 * (r >> 2) + 4 * h + (r & 3);
-          if (d < a.D) drow[d] = (T)(acc[k][r] * a.scale);
-        }
+    if (live) {
+      if (per < ntile)          // joined by join_kernel
+        put_acc<DP>(a.part_o + ((int64_t)split * a.Nq * a.H + row) * a.D, acc,
+                    a.D, 1.f);
+      else
+        put_acc<DP>((T*)a.dq + row * a.D, acc, a.D, a.scale);
     }
   }
   if constexpr (POS > 0) {
@@ -238,11 +292,12 @@ __global__ __launch_bounds__(NW * 64, 1) void dq_kernel(const Args a,
 }
 
 template <typename T, int DP, int NW, int POS>
-__global__ __launch_bounds__(NW * 64, 1) void dkv_kernel(const Args a) {
+__global__
+    __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void dkv_kernel(
+        const Args a) {
   constexpr int QT = 32;                         // packed rows per tile
   constexpr int CH = DP * (int)sizeof(T) / 16;
   constexpr int NT = NW * 64;
-  constexpr int LD = (QT * CH + NT - 1) / NT;
   constexpr int TB = QT * CH * 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   DGMC_LDS char* lds = (DGMC_LDS char*)smem;
@@ -263,14 +318,21 @@ __global__ __launch_bounds__(NW * 64, 1) void dkv_kernel(const Args a) {
 
   const int64_t kj = (int64_t)k_lo + wave * 32 + c;
   const bool live = kj < k_hi;
-  const T* krow = (const T*)a.k + kj * a.k_sn + (int64_t)kvh * a.k_sh;
-  const T* vrow = (const T*)a.v + kj * a.v_sn + (int64_t)kvh * a.v_sh;
+  // Query tiles [t0, t1) of this split.
+  const int ntile = (q_hi - q_lo + QW - 1) / QW;
+  const int per = split_tiles(a, ntile), split = blockIdx.y;
+  const int t0 = split * per, t1 = min(t0 + per, ntile);
+  if (split > 0 && t0 >= t1) return;
+  const int ko = wave * 32 + c;
   u32x4 kf[CH / 2], vf[CH / 2];
-#pragma unroll
-  for (int s = 0; s < CH / 2; ++s) {
-    kf[s] = load_chunk<T>(krow, 2 * s + h, a.D, live, a.vec_k);
-    vf[s] = load_chunk<T>(vrow, 2 * s + h, a.D, live, a.vec_v);
-  }
+  load_frags<T>(kf,
+                (const T*)a.k + (int64_t)k_lo * a.k_sn +
+                    (int64_t)kvh * a.k_sh,
+                ko * a.k_sn * (int64_t)sizeof(T), live, a.D, a.vec_k);
+  load_frags<T>(vf,
+                (const T*)a.v + (int64_t)k_lo * a.v_sn +
+                    (int64_t)kvh * a.v_sh,
+                ko * a.v_sn * (int64_t)sizeof(T), live, a.D, a.vec_v);
   float px = 0.f, py = 0.f;
   const Bucket bk(a);
   const int W = 2 * a.half + 2;
@@ -286,21 +348,22 @@ __global__ __launch_bounds__(NW * 64, 1) void dkv_kernel(const Args a) {
       gb[r] = ((8 * (r >> 2) + 4 * h + (r & 3)) % a.G) * kSlots;
   }
 
-  const int ntile = (q_hi - q_lo + QW - 1) / QW;
-  u32x4 qr[LD], gr[LD];
+  const int64_t qsb = a.q_sn * (int)sizeof(T), qhb = a.q_sh * (int)sizeof(T);
+  const int64_t gsb = a.g_sn * (int)sizeof(T), ghb = a.g_sh * (int)sizeof(T);
+  const T* qbase =
+      (const T*)a.q + (int64_t)q_lo * a.q_sn + (int64_t)kvh * a.G * a.q_sh;
+  const T* gbase =
+      (const T*)a.dout + (int64_t)q_lo * a.g_sn + (int64_t)kvh * a.G * a.g_sh;
   float rv[4] = {INFINITY, 0.f, 0.f, 0.f};
-  auto fetch = [&](int t) {
-#pragma unroll
-    for (int i = 0; i < LD; ++i) {
-      const int e = tid + i * NT, rw = e / CH, ch = e % CH;
-      const int64_t qi = (int64_t)q_lo + t * QW + rw / a.G;
-      const int head = kvh * a.G + rw % a.G;
-      const bool ok = rw < RW && qi < q_hi;
-      qr[i] = load_chunk<T>((const T*)a.q + qi * a.q_sn + head * a.q_sh, ch,
-                            a.D, ok, a.vec_q);
-      gr[i] = load_chunk<T>((const T*)a.dout + qi * a.g_sn + head * a.g_sh,
-                            ch, a.D, ok, a.vec_g);
-    }
+  auto fetch = [&](int t, int buf) {
+    using S = Stager<T, QT, CH, NT>;
+    const int left = q_hi - q_lo - t * QW;
+    DGMC_LDS char* qt = lds + buf * 2 * TB;
+    const auto ok = [&](int r) { return r < RW && r / a.G < left; };
+    S::fill(qbase + (int64_t)t * QW * a.q_sn, a.D, a.vec_q, qt, ok,
+            [&](int r) { return r / a.G * qsb + r % a.G * qhb; });
+    S::fill(gbase + (int64_t)t * QW * a.g_sn, a.D, a.vec_g, qt + TB, ok,
+            [&](int r) { return r / a.G * gsb + r % a.G * ghb; });
     if (tid < QT) {
       const int64_t qi = (int64_t)q_lo + t * QW + tid / a.G;
       const bool ok = tid < RW && qi < q_hi;
@@ -313,17 +376,7 @@ __global__ __launch_bounds__(NW * 64, 1) void dkv_kernel(const Args a) {
       }
     }
   };
-  auto stage = [&](int buf) {
-    DGMC_LDS char* qt = lds + buf * 2 * TB;
-#pragma unroll
-    for (int i = 0; i < LD; ++i) {
-      const int e = tid + i * NT, rw = e / CH, ch = e % CH;
-      if (LD * NT == QT * CH || rw < QT) {
-        const int off = (rw * CH + (ch ^ swz<CH>(rw))) * 16;
-        *(DGMC_LDS u32x4*)(qt + off) = qr[i];
-        *(DGMC_LDS u32x4*)(qt + TB + off) = gr[i];
-      }
-    }
+  auto put_rows = [&](int buf) {
     if (tid < QT) {
 #pragma unroll
       for (int k = 0; k < 2 + POS; ++k)
@@ -337,12 +390,12 @@ __global__ __launch_bounds__(NW * 64, 1) void dkv_kernel(const Args a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) ak[k][r] = av[k][r] = 0.f;
 
-  if (ntile > 0) fetch(0);
-  for (int t = 0; t < ntile; ++t) {
-    const int buf = t & 1;
-    stage(buf);
-    if (t + 1 < ntile) fetch(t + 1);
-    __syncthreads();
+  if (t0 < t1) fetch(t0, 0);
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    put_rows(buf);
+    stage_barrier();
+    if (t + 1 < t1) fetch(t + 1, buf ^ 1);
     const DGMC_LDS char* qt = lds + buf * 2 * TB;
     const DGMC_LDS float* rw = rowv + buf * 4 * QT;
     f32x16 z, dp, th;
@@ -385,18 +438,16 @@ __global__ __launch_bounds__(NW * 64, 1) void dkv_kernel(const Args a) {
     Mma<T>::template accum<DP>(ak, qt, 0, dp);
   }
   if (!live) return;
-  T* dk = (T*)a.dk + (kj * a.KV + kvh) * a.D;
-  T* dv = (T*)a.dv + (kj * a.KV + kvh) * a.D;
-#pragma unroll
-  for (int k = 0; k < DP / 32; ++k)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int d = 32 * k + 8 * (r >> 2) + 4 * h + (r & 3);
-      if (d < a.D) {
-        dk[d] = (T)(ak[k][r] * a.scale);
-        dv[d] = (T)av[k][r];
-      }
-    }
+  const int64_t row = kj * a.KV + kvh;
+  if (per < ntile) {            // joined by join_kernel
+    const int64_t rows = (int64_t)a.Nk * a.KV;
+    float* p = a.part_o + (split * rows + row) * a.D;
+    put_acc<DP>(p, ak, a.D, 1.f);
+    put_acc<DP>(p + a.splits * rows * a.D, av, a.D, 1.f);
+  } else {
+    put_acc<DP>((T*)a.dk + row * a.D, ak, a.D, a.scale);
+    put_acc<DP>((T*)a.dv + row * a.D, av, a.D, 1.f);
+  }
 }
 
 template <typename T, int DP, int NW, int POS>
@@ -407,8 +458,8 @@ void launch_dq(const Args& a, int nblk, hipStream_t st) {
                                (size_t)NW * a.slots * 256 : 0);
   auto kern = dq_kernel<T, DP, NW, POS>;
   allow_lds(reinterpret_cast<const void*>(kern), sm);
-  kern<<<dim3((POS ? nblk : nslot) * a.KV), dim3(NW * 64), sm, st>>>(a,
-                                                                    nslot);
+  kern<<<dim3((POS ? nblk : nslot * a.splits) * a.KV), dim3(NW * 64), sm,
+         st>>>(a, nslot);
   DGMC_CHECK_LAUNCH();
 }
 
@@ -418,8 +469,8 @@ void launch_dkv(const Args& a, hipStream_t st) {
                     (POS ? a.G * kSlots * 4 : 0);
   auto kern = dkv_kernel<T, DP, NW, POS>;
   allow_lds(reinterpret_cast<const void*>(kern), sm);
-  kern<<<dim3((a.Nk / (32 * NW) + a.B + 1) * a.KV), dim3(NW * 64), sm, st>>>(
-      a);
+  kern<<<dim3((a.Nk / (32 * NW) + a.B + 1) * a.KV, a.splits), dim3(NW * 64),
+         sm, st>>>(a);
   DGMC_CHECK_LAUNCH();
 }
 
@@ -435,23 +486,28 @@ void dkv_axes(const Args& a, int axes, hipStream_t st) {
   : axes == 1 ? launch_dkv<T, DP, NW, 1>(a, st)
               : launch_dkv<T, DP, NW, 2>(a, st);
 }
-template <typename T, int DP>
-void bwd_dim(const Args& a, int axes, int nwq, int nwk, int nblk,
-             hipStream_t st) {
-  nwq == 1 ? dq_axes<T, DP, 1>(a, axes, nblk, st)
-           : dq_axes<T, DP, 4>(a, axes, nblk, st);
-  if (a.dk == nullptr) return;
-  nwk == 1 ? dkv_axes<T, DP, 1>(a, axes, st)
-           : dkv_axes<T, DP, 4>(a, axes, st);
+template <typename T>
+void run_dq(const Args& a, int axes, int nw, int nblk, hipStream_t st) {
+  if (a.D <= 32)
+    nw == 1 ? dq_axes<T, 32, 1>(a, axes, nblk, st)
+            : dq_axes<T, 32, 4>(a, axes, nblk, st);
+  else if (a.D <= 64)
+    nw == 1 ? dq_axes<T, 64, 1>(a, axes, nblk, st)
+            : dq_axes<T, 64, 4>(a, axes, nblk, st);
+  else
+    nw == 1 ? dq_axes<T, 128, 1>(a, axes, nblk, st)
+            : dq_axes<T, 128, 4>(a, axes, nblk, st);
 }
 
-// The dq kernel first: it writes the rows' delta.
 template <typename T>
-void run_bwd(const Args& a, int axes, int nwq, int nwk, int nblk,
-             hipStream_t st) {
-  a.D <= 32   ? bwd_dim<T, 32>(a, axes, nwq, nwk, nblk, st)
-  : a.D <= 64 ? bwd_dim<T, 64>(a, axes, nwq, nwk, nblk, st)
-              : bwd_dim<T, 128>(a, axes, nwq, nwk, nblk, st);
+void run_dkv(const Args& a, int axes, int nw, hipStream_t st) {
+  if (a.D <= 32)
+    nw == 1 ? dkv_axes<T, 32, 1>(a, axes, st) : dkv_axes<T, 32, 4>(a, axes, st);
+  else if (a.D <= 64)
+    nw == 1 ? dkv_axes<T, 64, 1>(a, axes, st) : dkv_axes<T, 64, 4>(a, axes, st);
+  else
+    nw == 1 ? dkv_axes<T, 128, 1>(a, axes, st)
+            : dkv_axes<T, 128, 4>(a, axes, st);
 }
 
 }  // namespace segattn

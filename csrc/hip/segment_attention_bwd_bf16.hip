@@ -3,9 +3,11 @@
 
 namespace dgmc {
 namespace segattn {
-void bwd_bf16(const Args& a, int axes, int nwq, int nwk, int nblk,
-              hipStream_t st) {
-  run_bwd<__bf16>(a, axes, nwq, nwk, nblk, st);
+void dq_bf16(const Args& a, int axes, int nw, int nblk, hipStream_t st) {
+  run_dq<__bf16>(a, axes, nw, nblk, st);
+}
+void dkv_bf16(const Args& a, int axes, int nw, hipStream_t st) {
+  run_dkv<__bf16>(a, axes, nw, st);
 }
 }  // namespace segattn
 }  // namespace dgmc

@@ -3,9 +3,11 @@
 
 namespace dgmc {
 namespace segattn {
-void bwd_f32(const Args& a, int axes, int nwq, int nwk, int nblk,
-              hipStream_t st) {
-  run_bwd<float>(a, axes, nwq, nwk, nblk, st);
+void dq_f32(const Args& a, int axes, int nw, int nblk, hipStream_t st) {
+  run_dq<float>(a, axes, nw, nblk, st);
+}
+void dkv_f32(const Args& a, int axes, int nw, hipStream_t st) {
+  run_dkv<float>(a, axes, nw, st);
 }
 }  // namespace segattn
 }  // namespace dgmc

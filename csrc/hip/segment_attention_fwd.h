@@ -9,7 +9,11 @@
 // the output accumulators is skipped otherwise; P <= 2^8 changes no
 // relative rounding), the sum is kept per lane and joined once at the end.
 // P is rounded to bf16 for the bf16 product (fp32: not at all); maximum,
-// sum and outputs are fp32.
+// sum and outputs are fp32.  FINE (bf16, training): P enters as two bf16
+// terms and the rounding rest of the output is kept beside it, because the
+// backward's delta = <do, o> multiplies whole rows of P - its error does not
+// average out over the keys (the table's gradient would lose 2 of bf16's 8
+// bits).
 #pragma once
 
 #include "segment_attention.h"
@@ -17,13 +21,11 @@
 namespace dgmc {
 namespace segattn {
 
-template <typename T, int DP, int NW, int KT, int POS>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(
+template <typename T, int DP, int NW, int KT, int POS, bool FINE>
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) void fwd_kernel(
     const Args a) {
   constexpr int CH = DP * (int)sizeof(T) / 16;   // 16-byte chunks per row
   constexpr int NT = NW * 64;
-  constexpr int LD = KT * CH / NT;               // chunks a thread stages
-  static_assert(LD * NT == KT * CH, "staging");
   constexpr int TB = KT * CH * 16;               // bytes of one tile
   extern __shared__ __attribute__((aligned(16))) char smem[];
   DGMC_LDS char* lds = (DGMC_LDS char*)smem;
@@ -47,11 +49,13 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(
   const int64_t qi = (int64_t)q_lo + wave * QW + c / a.G;
   const bool live = c < QW * a.G && qi < q_hi;
   const int head = kvh * a.G + g;
-  const T* qrow = (const T*)a.q + qi * a.q_sn + (int64_t)head * a.q_sh;
   u32x4 qf[CH / 2];
-#pragma unroll
-  for (int s = 0; s < CH / 2; ++s)
-    qf[s] = load_chunk<T>(qrow, 2 * s + h, a.D, live, a.vec_q);
+  load_frags<T>(qf,
+                (const T*)a.q + (int64_t)q_lo * a.q_sn +
+                    (int64_t)kvh * a.G * a.q_sh,
+                ((wave * QW + c / a.G) * a.q_sn + g * a.q_sh) *
+                    (int64_t)sizeof(T),
+                live, a.D, a.vec_q);
   float px = 0.f, py = 0.f;
   const Bucket bk(a);
   if constexpr (POS > 0) {
@@ -66,39 +70,35 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(
 
   // Key tiles [t0, t1) of this split.
   const int ntile = (k_hi - k_lo + KT - 1) / KT;
-  const int per = (ntile + a.splits - 1) / a.splits;
-  const int t0 = min(split * per, ntile), t1 = min(t0 + per, ntile);
+  const int per = split_tiles(a, ntile);
+  const int t0 = split * per, t1 = min(t0 + per, ntile);
+  if (split > 0 && t0 >= t1) return;
 
-  const T* kbase = (const T*)a.k + (int64_t)kvh * a.k_sh;
-  const T* vbase = (const T*)a.v + (int64_t)kvh * a.v_sh;
-  u32x4 kr[LD], vr[LD];
+  const T* kbase =
+      (const T*)a.k + (int64_t)k_lo * a.k_sn + (int64_t)kvh * a.k_sh;
+  const T* vbase =
+      (const T*)a.v + (int64_t)k_lo * a.v_sn + (int64_t)kvh * a.v_sh;
+  const int64_t ksb = a.k_sn * (int)sizeof(T), vsb = a.v_sn * (int)sizeof(T);
   float pr[2] = {0.f, 0.f};
-  auto fetch = [&](int t) {
-    const int k0 = k_lo + t * KT;
-#pragma unroll
-    for (int i = 0; i < LD; ++i) {
-      const int e = tid + i * NT, row = e / CH, ch = e % CH;
-      const int64_t j = (int64_t)k0 + row;
-      const bool ok = j < k_hi;
-      kr[i] = load_chunk<T>(kbase + j * a.k_sn, ch, a.D, ok, a.vec_k);
-      vr[i] = load_chunk<T>(vbase + j * a.v_sn, ch, a.D, ok, a.vec_v);
-    }
+  // Start tile t's loads into buffer `buf`; its positions wait in registers.
+  auto fetch = [&](int t, int buf) {
+    using S = Stager<T, KT, CH, NT>;
+    const int left = k_hi - k_lo - t * KT;
+    DGMC_LDS char* kt = lds + buf * 2 * TB;
+    const auto ok = [&](int r) { return r < left; };
+    S::fill(kbase + (int64_t)t * KT * a.k_sn, a.D, a.vec_k, kt, ok,
+            [&](int r) { return r * ksb; });
+    S::fill(vbase + (int64_t)t * KT * a.v_sn, a.D, a.vec_v, kt + TB, ok,
+            [&](int r) { return r * vsb; });
     if constexpr (POS > 0) {
-      if (tid < KT && k0 + tid < k_hi) {
-        pr[0] = load_pos(a.pos_k, (int64_t)k0 + tid, POS, 0);
-        if (POS == 2) pr[1] = load_pos(a.pos_k, (int64_t)k0 + tid, POS, 1);
+      if (tid < KT && tid < left) {
+        const int64_t j = (int64_t)k_lo + t * KT + tid;
+        pr[0] = load_pos(a.pos_k, j, POS, 0);
+        if (POS == 2) pr[1] = load_pos(a.pos_k, j, POS, 1);
       }
     }
   };
-  auto stage = [&](int buf) {
-    DGMC_LDS char* kt = lds + buf * 2 * TB;
-#pragma unroll
-    for (int i = 0; i < LD; ++i) {
-      const int e = tid + i * NT, row = e / CH, ch = e % CH;
-      const int off = (row * CH + (ch ^ swz<CH>(row))) * 16;
-      *(DGMC_LDS u32x4*)(kt + off) = kr[i];
-      *(DGMC_LDS u32x4*)(kt + TB + off) = vr[i];
-    }
+  auto put_pos = [&](int buf) {
     if constexpr (POS > 0) {
       if (tid < KT) {
         kpos[(buf * 2 + 0) * KT + tid] = pr[0];
@@ -115,13 +115,16 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(
   float m = -INFINITY, l = 0.f;
   const float s1 = a.cap > 0.f ? a.scale / a.cap : a.scale * kLog2e;
   const float s2 = a.cap * kLog2e;
+  // Plain scores stay unscaled: 2^(s1 z - m) is one fma and one exp2.
+  const bool plain = POS == 0 && a.cap <= 0.f && s1 > 0.f;
+  const float ex = plain ? s1 : 1.f;
 
-  if (t0 < t1) fetch(t0);
+  if (t0 < t1) fetch(t0, 0);
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
-    stage(buf);
-    if (t + 1 < t1) fetch(t + 1);
-    __syncthreads();
+    put_pos(buf);
+    stage_barrier();
+    if (t + 1 < t1) fetch(t + 1, buf ^ 1);
     const DGMC_LDS char* kt = lds + buf * 2 * TB;
     f32x16 z[KT / 32];
 #pragma unroll
@@ -139,7 +142,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           z[u][r] = s2 * tanh_<sizeof(T) == 4>(z[u][r] * s1);
-    } else {
+    } else if (!plain) {
 #pragma unroll
       for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
@@ -179,7 +182,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(
     for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mt = fmaxf(mt, z[u][r]);
-    mt = max_half(mt);
+    mt = max_half(mt) * ex;
     if (__any(mt > m + 8.f)) {
       const float mn = fmaxf(m, mt);
       const float al = mn == m ? 1.f : exp2_(m - mn);
@@ -194,18 +197,19 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(
 #pragma unroll
     for (int u = 0; u < KT / 32; ++u) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) z[u][r] = exp2_(z[u][r] - ms);
+      for (int r = 0; r < 16; ++r) z[u][r] = exp2_(fmaf(z[u][r], ex, -ms));
       float s = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s += z[u][r];
       l += s;
-      Mma<T>::template accum<DP>(acc, kt + TB, 32 * u, z[u]);
+      Mma<T>::template accum<DP, FINE>(acc, kt + TB, 32 * u,
+                                              z[u]);
     }
   }
   l = sum_half(l);
   if (!live) return;
   const int64_t row = qi * a.H + head;
-  if (a.splits > 1) {
+  if (per < ntile) {            // joined by join_kernel
     const int64_t prow = (int64_t)split * a.Nq * a.H + row;
     if (h == 0) {
       a.part_ml[prow * 2] = m;
@@ -233,44 +237,43 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(
       T o[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[r] = (T)(acc[k][4 * r4 + r] * inv);
-      if (a.D % 4 == 0) {
-        if (d < a.D) __builtin_memcpy(__builtin_assume_aligned(
-                         orow + d, 4 * sizeof(T)), o, 4 * sizeof(T));
-      } else {
+      put4(orow, d, a.D, o);
+      if constexpr (FINE) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (d + r < a.D) orow[d + r] = o[r];
+          o[r] = (T)(acc[k][4 * r4 + r] * inv - (float)o[r]);
+        put4((T*)a.out_lo + row * a.D, d, a.D, o);
       }
     }
 }
 
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, bool FINE>
 void launch_fwd(const Args& a, int axes, hipStream_t st) {
-  // Tiles of 64 keys while both buffers of K and V fit 64 KB of LDS.
-  constexpr int KT = (NW > 1 && DP * (int)sizeof(T) <= 256) ? 64 : 32;
+  constexpr int KT =                // (fwd_keys)
+      (NW > 1 && DP * (int)sizeof(T) <= 256) ? 64 : 32;
   const int TQ = 32 / a.G * NW;
   const dim3 grid((a.Nq / TQ + a.B + 1) * a.KV, a.splits), blk(NW * 64);
   const size_t sm = 4 * KT * DP * sizeof(T) +
                     (axes ? 16 * KT + a.G * kSlots * 4 : 0);
-  auto kern = axes == 0   ? fwd_kernel<T, DP, NW, KT, 0>
-              : axes == 1 ? fwd_kernel<T, DP, NW, KT, 1>
-                          : fwd_kernel<T, DP, NW, KT, 2>;
+  auto kern = axes == 0   ? fwd_kernel<T, DP, NW, KT, 0, FINE>
+              : axes == 1 ? fwd_kernel<T, DP, NW, KT, 1, FINE>
+                          : fwd_kernel<T, DP, NW, KT, 2, FINE>;
   allow_lds(reinterpret_cast<const void*>(kern), sm);
   kern<<<grid, blk, sm, st>>>(a);
   DGMC_CHECK_LAUNCH();
 }
 
-template <typename T>
+template <typename T, bool FINE>
 void run_fwd(const Args& a, int axes, int nw, hipStream_t st) {
   if (a.D <= 32)
-    nw == 1 ? launch_fwd<T, 32, 1>(a, axes, st)
-            : launch_fwd<T, 32, 4>(a, axes, st);
+    nw == 1 ? launch_fwd<T, 32, 1, FINE>(a, axes, st)
+            : launch_fwd<T, 32, 4, FINE>(a, axes, st);
   else if (a.D <= 64)
-    nw == 1 ? launch_fwd<T, 64, 1>(a, axes, st)
-            : launch_fwd<T, 64, 4>(a, axes, st);
+    nw == 1 ? launch_fwd<T, 64, 1, FINE>(a, axes, st)
+            : launch_fwd<T, 64, 4, FINE>(a, axes, st);
   else
-    nw == 1 ? launch_fwd<T, 128, 1>(a, axes, st)
-            : launch_fwd<T, 128, 4>(a, axes, st);
+    nw == 1 ? launch_fwd<T, 128, 1, FINE>(a, axes, st)
+            : launch_fwd<T, 128, 4, FINE>(a, axes, st);
 }
 
 }  // namespace segattn

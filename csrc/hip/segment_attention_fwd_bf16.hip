@@ -4,7 +4,7 @@
 namespace dgmc {
 namespace segattn {
 void fwd_bf16(const Args& a, int axes, int nw, hipStream_t st) {
-  run_fwd<__bf16>(a, axes, nw, st);
+  run_fwd<__bf16, false>(a, axes, nw, st);
 }
 }  // namespace segattn
 }  // namespace dgmc

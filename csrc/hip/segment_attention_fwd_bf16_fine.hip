@@ -1,0 +1,10 @@
+// bf16 instances of the segment attention forward, training form.
+#include "segment_attention_fwd.h"
+
+namespace dgmc {
+namespace segattn {
+void fwd_bf16_fine(const Args& a, int axes, int nw, hipStream_t st) {
+  run_fwd<__bf16, true>(a, axes, nw, st);
+}
+}  // namespace segattn
+}  // namespace dgmc

@@ -4,7 +4,7 @@
 namespace dgmc {
 namespace segattn {
 void fwd_f32(const Args& a, int axes, int nw, hipStream_t st) {
-  run_fwd<float>(a, axes, nw, st);
+  run_fwd<float, false>(a, axes, nw, st);
 }
 }  // namespace segattn
 }  // namespace dgmc

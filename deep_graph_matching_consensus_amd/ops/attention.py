@@ -48,25 +48,25 @@ class _SegmentAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k, scale, cap,
                 layout):
         grad = any(ctx.needs_input_grad[:4])
-        out, lse = _backend.ops().segment_attention_fwd(
+        out, lo, lse = _backend.ops().segment_attention_fwd(
             q, k, v, ptr_q, ptr_k, scale, cap, bias, pos_q, pos_k, *layout,
             grad)
         if grad:
             ctx.save_for_backward(q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k,
-                                  out, lse)
+                                  out, lo, lse)
             ctx.args = (scale, cap, layout)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k, out, lse = \
+        q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k, out, lo, lse = \
             ctx.saved_tensors
         scale, cap, layout = ctx.args
         if grad.stride(-1) != 1 and grad.size(-1) != 1:
             grad = grad.contiguous()
         dq, dk, dv, db = _backend.ops().segment_attention_bwd(
-            grad, q, k, v, out, lse, ptr_q, ptr_k, scale, cap, bias, pos_q,
+            grad, q, k, v, out, lo, lse, ptr_q, ptr_k, scale, cap, bias, pos_q,
             pos_k, *layout)
         return (dq, dk, dv, None if bias is None else db) + (None, ) * 7
 

@@ -409,7 +409,11 @@ def test_large_scores_do_not_overflow():
         gap = z.topk(2, dim=1)[0]
         clear = (gap[:, 0] - gap[:, 1]) / 8 > 40
         assert clear.any()
-        assert torch.equal(out['out'][clear, 0], best[clear])
+        # p v / l with one p: rounded p (bf16: 2^-8), the product, 1 / l,
+        # its product and the output (bf16: 2^-8) - p itself cancels
+        far = (out['out'][clear, 0].double() - best[clear].double()).abs()
+        tol = 2 * _u(dtype) + 4 * F
+        assert (far <= tol * best[clear].double().abs()).all()
 
 
 @pytest.mark.gpu
