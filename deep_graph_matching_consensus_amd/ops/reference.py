@@ -188,3 +188,49 @@ def segment_attention(q, k, v, ptr_q, ptr_k, scale, cap=0.0, bias=None,
     if rows < q.size(0) or not outs:
         outs.append(qa[rows:].masked_fill(never, 0))
     return torch.cat(outs, dim=0).to(q.dtype)
+
+
+# --------------------------------------------------------------------------
+# Layer norm, match log-probabilities
+# --------------------------------------------------------------------------
+def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
+    s = x if residual is None else x + residual
+    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+    d = s.to(acc) - s.to(acc).mean(dim=-1, keepdim=True)
+    y = d / torch.sqrt((d * d).mean(dim=-1, keepdim=True) + eps)
+    if weight is not None:
+        y = y * weight.to(acc)
+    if bias is not None:
+        y = y + bias.to(acc)
+    y = y.to(x.dtype)
+    return y if residual is None else (y, s)
+
+
+def match_log_probs(scores, target, n_cols=None, top=0):
+    """``(log_prob, entropy, top_log_prob, top_index)`` of the row softmax
+    over the valid columns (see ``ops/logprob.py``)."""
+    acc = torch.float64 if scores.dtype == torch.float64 else torch.float32
+    V = scores.size(1)
+    z = scores.to(acc)
+    col = torch.arange(V, device=z.device)
+    ninf = torch.full((), -float('inf'), dtype=acc, device=z.device)
+    if n_cols is not None:
+        z = torch.where(col < n_cols.view(-1, 1), z, ninf)
+    top_z = z.detach().amax(dim=-1, keepdim=True)
+    empty = top_z == -float('inf')
+    m = top_z.masked_fill(empty, 0)
+    # (masked entries leave the graph: their gradient is 0)
+    live = z != -float('inf')
+    d = torch.where(live, z, m) - m
+    e = torch.exp(d) * live
+    total = e.sum(dim=-1, keepdim=True).masked_fill(empty, 1)
+    lp = d - torch.log(total)
+    ent = -(e / total * lp).sum(dim=-1)
+    given = (target >= 0) & (target < V)
+    y = torch.where(given, target, torch.zeros_like(target)).view(-1, 1)
+    logp = torch.where(live.gather(1, y), lp.gather(1, y), ninf).view(-1)
+    logp = torch.where(given, logp, torch.zeros_like(logp))
+    idx = z.detach().sort(dim=-1, descending=True, stable=True)[1][:, :top]
+    dead = ~live.gather(1, idx)
+    top_lp = lp.detach().gather(1, idx).masked_fill(dead, -float('inf'))
+    return logp, ent, top_lp, idx.masked_fill(dead, -1)
