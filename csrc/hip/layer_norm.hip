@@ -14,6 +14,7 @@
 // rows a workgroup walks, joined over its row groups through LDS and added
 // over the workgroups in order by a second kernel: no atomics, the same bits
 // every run.
+#include "attentional.h"
 #include "common.h"
 
 namespace dgmc {
@@ -28,8 +29,11 @@ constexpr int kLnMaxCols = 8192;
 // Sum over the TPR lanes that share a row (every lane gets it).
 template <int TPR>
 __device__ __forceinline__ float ln_sum(float v, float* red) {
-#pragma unroll
-  for (int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) v += __shfl_xor(v, o);
+  v = quad_sum(v);                       // lane exchanges of up to 16 lanes
+  v += dpp_mov<0x141>(v);                // are VALU modifiers, no LDS trip
+  if constexpr (TPR >= 16) v += dpp_mov<0x140>(v);
+  if constexpr (TPR >= 32) v += __shfl_xor(v, 16);
+  if constexpr (TPR >= 64) v += __shfl_xor(v, 32);
   if constexpr (TPR > 64) {
     const int wave = threadIdx.x >> 6;
     __syncthreads();
@@ -73,58 +77,68 @@ struct LnArgs {
   float eps;
 };
 
+// A workgroup walks rows blockIdx.x RPB + k gridDim.x RPB; weight and bias
+// stay in registers.
 template <typename T, int TPR, int NV, int N>
 __global__ __launch_bounds__(kLnThreads) void ln_fwd_kernel(const LnArgs a) {
   __shared__ float red[4];
   constexpr int RPB = kLnThreads / TPR;
-  const int t = threadIdx.x % TPR;
-  const int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-  const bool live = r < a.rows;
-  const int C = live ? a.C : 0;
-  float x[NV][N];
-  ln_load<T, TPR, NV, N>((const T*)a.x + r * a.C, t, C, x);
-  if (a.res != nullptr) {
-    float q[NV][N];
-    ln_load<T, TPR, NV, N>((const T*)a.res + r * a.C, t, C, q);
+  const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
+  float w[NV][N], b[NV][N];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int c = min(ln_col<TPR, N>(t, i, e), a.C - 1);
+      w[i][e] = a.w ? a.w[c] : 1.f;
+      b[i][e] = a.b ? a.b[c] : 0.f;
+    }
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows;
+       r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t r = r0 + grp;
+    const bool live = r < a.rows;
+    const int C = live ? a.C : 0;
+    float x[NV][N];
+    ln_load<T, TPR, NV, N>((const T*)a.x + r * a.C, t, C, x);
+    if (a.res != nullptr) {
+      float q[NV][N];
+      ln_load<T, TPR, NV, N>((const T*)a.res + r * a.C, t, C, q);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          x[i][e] = Cvt<T>::to_f(Cvt<T>::from_f(x[i][e] + q[i][e]));
+        const int c = ln_col<TPR, N>(t, i, 0);
+        if (c < C) store_vec<T, N>((T*)a.s + r * a.C + c, x[i]);
+      }
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e) sum += x[i][e];
+    const float mean = ln_sum<TPR>(sum, red) / a.C;
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float d = x[i][e] - mean;
+        sum += ln_col<TPR, N>(t, i, e) < C ? d * d : 0.f;
+      }
+    const float rstd = 1.f / sqrtf(ln_sum<TPR>(sum, red) / a.C + a.eps);
+    if (live && t == 0 && a.stat) a.stat[r] = make_float2(mean, rstd);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      const int c = ln_col<TPR, N>(t, i, 0);
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        x[i][e] = Cvt<T>::to_f(Cvt<T>::from_f(x[i][e] + q[i][e]));
-      const int c = ln_col<TPR, N>(t, i, 0);
-      if (c < C) store_vec<T, N>((T*)a.s + r * a.C + c, x[i]);
+        x[i][e] = fmaf((x[i][e] - mean) * rstd, w[i][e], b[i][e]);
+      if (c < C) store_vec<T, N>((T*)a.y + r * a.C + c, x[i]);
     }
-  }
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int e = 0; e < N; ++e) sum += x[i][e];
-  const float mean = ln_sum<TPR>(sum, red) / a.C;
-  sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float d = x[i][e] - mean;
-      sum += ln_col<TPR, N>(t, i, e) < C ? d * d : 0.f;
-    }
-  const float rstd = 1.f / sqrtf(ln_sum<TPR>(sum, red) / a.C + a.eps);
-  if (live && t == 0 && a.stat) a.stat[r] = make_float2(mean, rstd);
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = ln_col<TPR, N>(t, i, 0);
-    if (c >= C) continue;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float h = (x[i][e] - mean) * rstd;
-      x[i][e] = a.w ? fmaf(h, a.w[c + e], a.b ? a.b[c + e] : 0.f) : h;
-    }
-    store_vec<T, N>((T*)a.y + r * a.C + c, x[i]);
   }
 }
 
-// One workgroup walks rows blockIdx.x RPB + k gridDim.x RPB.
 template <typename T, int TPR, int NV, int N>
 __global__ __launch_bounds__(kLnThreads) void ln_bwd_kernel(const LnArgs a) {
   __shared__ float red[4];
@@ -214,23 +228,26 @@ __global__ __launch_bounds__(kLnThreads) void ln_bwd_kernel(const LnArgs a) {
   }
 }
 
-// out[c] = sum over the blocks' parts in order: 32 columns a workgroup, each
-// by 8 threads that take every 8th part.
-__global__ __launch_bounds__(256) void ln_fold_kernel(
+// out[c] = sum over the blocks' parts in a fixed order: 32 columns a
+// workgroup, each by 32 threads that take every 32nd part.
+constexpr int kLnWays = 32;
+
+__global__ __launch_bounds__(32 * kLnWays) void ln_fold_kernel(
     const float* __restrict__ part, float* __restrict__ dw,
     float* __restrict__ db, int blocks, int C) {
-  __shared__ float red[8][32];
+  __shared__ float red[kLnWays][32];
   const int c = blockIdx.x * 32 + (threadIdx.x & 31), p = threadIdx.x >> 5;
   float s = 0.f;
   if (c < 2 * C) {
 #pragma unroll 8
-    for (int b = p; b < blocks; b += 8) s += part[(int64_t)b * 2 * C + c];
+    for (int b = p; b < blocks; b += kLnWays)
+      s += part[(int64_t)b * 2 * C + c];
   }
   red[p][threadIdx.x & 31] = s;
   __syncthreads();
   if (p != 0 || c >= 2 * C) return;
 #pragma unroll
-  for (int q = 1; q < 8; ++q) s += red[q][threadIdx.x];
+  for (int q = 1; q < kLnWays; ++q) s += red[q][threadIdx.x];
   if (c < C) {
     if (dw) dw[c] = s;
   } else if (db) {
@@ -291,7 +308,7 @@ void ln_check(const at::Tensor& t, const at::Tensor& x, const char* name) {
               "layer_norm: ", name, " must be contiguous and like x");
 }
 
-void ln_check_w(const c10::optional<at::Tensor>& w, const at::Tensor& x) {
+void ln_check_w(const OptTensor& w, const at::Tensor& x) {
   TORCH_CHECK(!w.has_value() ||
                   (w->device() == x.device() &&
                    w->scalar_type() == at::kFloat && w->is_contiguous() &&
@@ -301,12 +318,10 @@ void ln_check_w(const c10::optional<at::Tensor>& w, const at::Tensor& x) {
 
 }  // namespace
 
-// x: contiguous [rows, C].  Returns (y, s, stat): s is empty without a
-// residual, stat [rows, 2] (mean, rstd) empty unless `train`.
 std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd(
-    const at::Tensor& x, const c10::optional<at::Tensor>& residual,
-    const c10::optional<at::Tensor>& weight,
-    const c10::optional<at::Tensor>& bias, double eps, bool train) {
+    const at::Tensor& x, const OptTensor& residual,
+    const OptTensor& weight,
+    const OptTensor& bias, double eps, bool train) {
   TORCH_CHECK(x.dim() == 2 && x.size(1) >= 1 && x.size(1) <= kLnMaxCols,
               "layer_norm: x must be [rows, 1 to ", kLnMaxCols, "]");
   ln_check(x, x, "x");
@@ -337,8 +352,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd(
   DGMC_DISPATCH_FLOAT(x.scalar_type(), T, [&] {
     ln_width<T>(vec, a.C, [&](auto tpr, auto nv, auto n) {
       constexpr int rpb = kLnThreads / tpr();
-      const int64_t blocks = (a.rows + rpb - 1) / rpb;
-      TORCH_CHECK(blocks < (1 << 24), "layer_norm: too many rows");
+      // 2048 workgroups (eight a CU, all resident) at most.
+      const int64_t blocks =
+          std::min<int64_t>((a.rows + rpb - 1) / rpb, 2048);
       ln_fwd_kernel<T, tpr(), nv(), n()>
           <<<dim3((unsigned)blocks), kLnThreads, 0, stream()>>>(a);
     });
@@ -347,11 +363,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd(
   return {y, s, stat};
 }
 
-// Returns (dx, dw, db): dw and db fp32, empty unless `with_weight`.
 std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_bwd(
-    const at::Tensor& dy, const c10::optional<at::Tensor>& ds,
+    const at::Tensor& dy, const OptTensor& ds,
     const at::Tensor& s, const at::Tensor& stat,
-    const c10::optional<at::Tensor>& weight, bool with_weight) {
+    const OptTensor& weight, bool with_weight) {
   TORCH_CHECK(s.dim() == 2 && s.size(1) >= 1 && s.size(1) <= kLnMaxCols,
               "layer_norm: s must be [rows, 1 to ", kLnMaxCols, "]");
   ln_check(s, s, "s");
@@ -401,7 +416,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_bwd(
     DGMC_CHECK_LAUNCH();
   });
   if (with_weight) {
-    ln_fold_kernel<<<(2 * C + 31) / 32, 256, 0, stream()>>>(
+    ln_fold_kernel<<<(2 * C + 31) / 32, 32 * kLnWays, 0, stream()>>>(
         a.part, dw.data_ptr<float>(), db.data_ptr<float>(), blocks, C);
     DGMC_CHECK_LAUNCH();
   }

@@ -21,6 +21,7 @@
 //
 // Rows past one workgroup's registers are cut into parts; a second kernel
 // joins the parts' maxima, sums and selections.
+#include "attentional.h"
 #include "common.h"
 
 namespace dgmc {
@@ -182,10 +183,11 @@ __device__ __forceinline__ void lp_block_sum(float& l, float& t,
 }
 
 template <typename T, int NT, int NV>
-__global__ __launch_bounds__(NT) void lp_row_kernel(const LpArgs a) {
+__global__ __launch_bounds__(NT, 4) void lp_row_kernel(const LpArgs a) {
   constexpr int N = Vec16<T>::N;
   constexpr int GS = NT / 64;                  // lanes of one of 64 groups
-  __shared__ float gmax[64], thr_s, red[NT / 64][2];
+  __shared__ float gmax[64], red[NT / 64][2];
+  __shared__ int ranks[NT / 64][64];
   __shared__ float cand_v[kLpCand];
   __shared__ int cand_j[kLpCand], count;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -222,10 +224,21 @@ __global__ __launch_bounds__(NT) void lp_row_kernel(const LpArgs a) {
       __builtin_memcpy(&raw[i], e, 16);
     }
   }
+  // Masked columns and empty slots become -inf once, here.
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = b0 + (i * NT + tid) * N;
+    if (c < c0 || c + N > c1) {
+      T e[N];
+      __builtin_memcpy(e, &raw[i], 16);
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (c + k < c0 || c + k >= c1) e[k] = Cvt<T>::from_f(-INFINITY);
+      __builtin_memcpy(&raw[i], e, 16);
+    }
+  }
   auto value = [&](int i, int k) {
-    const int c = b0 + (i * NT + tid) * N + k;
-    const T* e = reinterpret_cast<const T*>(&raw[i]);
-    return c >= c0 && c < c1 ? Cvt<T>::to_f(e[k]) : -INFINITY;
+    return Cvt<T>::to_f(reinterpret_cast<const T*>(&raw[i])[k]);
   };
 
   float m = -INFINITY;
@@ -233,6 +246,16 @@ __global__ __launch_bounds__(NT) void lp_row_kernel(const LpArgs a) {
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int k = 0; k < N; ++k) m = fmaxf(m, value(i, k));
+  const float lane_max = m;
+  // (opaque between the passes: the vectors are unpacked anew, not kept as
+  // twice the registers)
+  auto again = [&] {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      asm volatile("" : "+v"(raw[i].x), "+v"(raw[i].y), "+v"(raw[i].z),
+                   "+v"(raw[i].w));
+  };
+  again();
 #pragma unroll
   for (int o = 1; o < GS; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
   if (tid % GS == 0) gmax[tid / GS] = m;
@@ -240,21 +263,25 @@ __global__ __launch_bounds__(NT) void lp_row_kernel(const LpArgs a) {
   const float gm = gmax[lane];
   m = wave_max(gm);
   const float ms = m == -INFINITY ? 0.f : m;
-  if (a.k > 0 && tid < 64) {
-    // The k-th largest of the 64 maxima (equal ones by group number).
+  // Each wave ranks the 64 maxima against its share of them (equal ones by
+  // group number).
+  if (a.k > 0) {
     int rank = 0;
-    for (int o = 0; o < 64; ++o) {
-      const float w = lane_of(gm, o);
+#pragma unroll
+    for (int q = 0; q < 64 / (NT / 64); ++q) {
+      const int o = (tid >> 6) * (64 / (NT / 64)) + q;
+      const float w = gmax[o];
       rank += w > gm || (w == gm && o < lane);
     }
-    if (rank == a.k - 1) thr_s = gm;
+    ranks[tid >> 6][lane] = rank;
   }
   float l = 0.f, t = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int k = 0; k < N; ++k) lp_add(value(i, k) - ms, l, t);
-  lp_block_sum<NT>(l, t, red);                 // (a barrier: thr_s is there)
+  again();
+  lp_block_sum<NT>(l, t, red);                 // (a barrier: ranks are there)
   if (tid == 0) {
     if (a.parts > 1)
       a.part[r * a.parts + p] = make_float4(m, l, t, 0.f);
@@ -263,7 +290,12 @@ __global__ __launch_bounds__(NT) void lp_row_kernel(const LpArgs a) {
   }
   if (a.k == 0) return;
 
-  const float ll = logf(l), thr = thr_s;
+  int rank = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) rank += ranks[w][lane];
+  // The k-th largest of the 64 maxima.
+  const float ll = logf(l),
+              thr = lane_of(gm, __ffsll(__ballot(rank == a.k - 1)) - 1);
   auto put = [&](int q, float v, int j) {
     if (a.parts > 1) {
       a.part_v[(r * a.parts + p) * a.k + q] = v;
@@ -272,6 +304,8 @@ __global__ __launch_bounds__(NT) void lp_row_kernel(const LpArgs a) {
       lp_put(a, r, q, v, j, ms, ll);
     }
   };
+  // (about k lanes of the workgroup hold a candidate)
+  if (lane_max >= thr && lane_max > -INFINITY)
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -287,6 +321,18 @@ __global__ __launch_bounds__(NT) void lp_row_kernel(const LpArgs a) {
     }
   __syncthreads();
   const int n = count;
+  if (n <= 64) {
+    // One wave, a candidate a lane, the others' values by readlane.
+    if (tid >= 64) return;
+    const bool own = lane < n;
+    const float v = own ? cand_v[lane] : -INFINITY;
+    const int j = own ? cand_j[lane] : -1;
+    int q = 0;
+    for (int o = 0; o < n; ++o)
+      q += lp_before(lane_of(v, o), __builtin_amdgcn_readlane(j, o), v, j);
+    if (own ? q < a.k : lane < a.k) put(own ? q : lane, v, j);
+    return;
+  }
   if (n <= kLpCand) {
     for (int c = tid; c < max(n, a.k); c += NT) {
       if (c >= n) {
@@ -295,10 +341,11 @@ __global__ __launch_bounds__(NT) void lp_row_kernel(const LpArgs a) {
       }
       const float v = cand_v[c];
       const int j = cand_j[c];
-      int rank = 0;
+      int q = 0;
+#pragma unroll 4
       for (int o = 0; o < n; ++o)
-        rank += lp_before(cand_v[o], cand_j[o], v, j);
-      if (rank < a.k) put(rank, v, j);
+        q += lp_before(cand_v[o], cand_j[o], v, j);
+      if (q < a.k) put(q, v, j);
     }
     return;
   }
@@ -469,7 +516,7 @@ __global__ __launch_bounds__(256) void lp_bwd_kernel(const LpArgs a) {
 }
 
 void lp_check(const at::Tensor& z, const at::Tensor& y,
-              const c10::optional<at::Tensor>& n) {
+              const OptTensor& n) {
   TORCH_CHECK(z.is_cuda() && z.dim() == 2 && z.size(1) >= 1 &&
                   z.size(1) < (1 << 30) &&
                   (z.size(1) == 1 || z.stride(1) == 1),
@@ -490,7 +537,7 @@ void lp_rows(LpArgs& a, const at::TensorOptions& f32, hipStream_t st) {
   // (a vector less than the registers hold: room for the misaligned start)
   a.width = (NT * NV - 1) * Vec16<T>::N;
   a.parts = (a.V + a.width - 1) / a.width;
-  TORCH_CHECK(a.rows * a.parts < (1 << 22) * (int64_t)(1024 / NT),
+  TORCH_CHECK(a.rows * a.parts < (1 << 23) * (int64_t)(512 / NT),
               "match_log_probs: too many rows for one call");
   at::Tensor part, pv, pi;
   if (a.parts > 1) {
@@ -521,11 +568,9 @@ void lp_small(const LpArgs& a, hipStream_t st) {
 
 }  // namespace
 
-// Returns (logp [R], entropy [R], top_lp [R, k], top_idx [R, k], stat):
-// stat [R, 2] is empty unless `train`.
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>
 match_logprob_fwd(const at::Tensor& z, const at::Tensor& y,
-                  const c10::optional<at::Tensor>& n, int64_t k, bool train) {
+                  const OptTensor& n, int64_t k, bool train) {
   lp_check(z, y, n);
   TORCH_CHECK(k >= 0 && k <= kLpMaxTop && k <= z.size(1),
               "match_log_probs: top must be 0 to ", kLpMaxTop,
@@ -555,27 +600,26 @@ match_logprob_fwd(const at::Tensor& z, const at::Tensor& y,
   const hipStream_t st = stream();
   DGMC_DISPATCH_FLOAT(z.scalar_type(), T, [&] {
     constexpr int N = Vec16<T>::N;
-    const int vecs = (a.V + N - 1) / N + 1;
+    constexpr int S = N / 4;        // 8, 16, 32 .. 64 values a lane
+    const int vals = a.V + 2 * N;   // (with room for a misaligned start)
     if (a.V <= 16) lp_small<T, 16, 1>(a, st);
     else if (a.V <= 32) lp_small<T, 16, 2>(a, st);
     else if (a.V <= 64) lp_small<T, 16, 4>(a, st);
     else if (a.V <= kLpSmall) lp_small<T, 64, 4>(a, st);
-    else if (vecs <= 256) lp_rows<T, 256, 1>(a, f32, st);
-    else if (vecs <= 512) lp_rows<T, 256, 2>(a, f32, st);
-    else if (vecs <= 1024) lp_rows<T, 256, 4>(a, f32, st);
-    else if (vecs <= 2048) lp_rows<T, 256, 8>(a, f32, st);
-    else if (vecs <= 3 * 1024) lp_rows<T, 1024, 3>(a, f32, st);
-    else if (vecs <= 5 * 1024) lp_rows<T, 1024, 5>(a, f32, st);
-    else lp_rows<T, 1024, 8>(a, f32, st);
+    else if (vals <= 256 * 8) lp_rows<T, 256, 2 / S>(a, f32, st);
+    else if (vals <= 256 * 16) lp_rows<T, 256, 4 / S>(a, f32, st);
+    else if (vals <= 256 * 32) lp_rows<T, 256, 8 / S>(a, f32, st);
+    else if (vals <= 512 * 24) lp_rows<T, 512, 6 / S>(a, f32, st);
+    else if (vals <= 512 * 40) lp_rows<T, 512, 10 / S>(a, f32, st);
+    else lp_rows<T, 512, 16 / S>(a, f32, st);
   });
   return {logp, ent, top_lp, top_idx, stat};
 }
 
-// dz [R, V], contiguous, in z's type.
-at::Tensor match_logprob_bwd(const c10::optional<at::Tensor>& gl,
-                             const c10::optional<at::Tensor>& gh,
+at::Tensor match_logprob_bwd(const OptTensor& gl,
+                             const OptTensor& gh,
                              const at::Tensor& z, const at::Tensor& y,
-                             const c10::optional<at::Tensor>& n,
+                             const OptTensor& n,
                              const at::Tensor& logp, const at::Tensor& ent,
                              const at::Tensor& stat) {
   lp_check(z, y, n);

@@ -5,42 +5,6 @@
 #include <torch/library.h>
 
 namespace dgmc {
-std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd(
-    const at::Tensor& x, const c10::optional<at::Tensor>& residual,
-    const c10::optional<at::Tensor>& weight,
-    const c10::optional<at::Tensor>& bias, double eps, bool train);
-std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_bwd(
-    const at::Tensor& dy, const c10::optional<at::Tensor>& ds,
-    const at::Tensor& s, const at::Tensor& stat,
-    const c10::optional<at::Tensor>& weight, bool with_weight);
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>
-match_logprob_fwd(const at::Tensor& z, const at::Tensor& y,
-                  const c10::optional<at::Tensor>& n, int64_t k, bool train);
-at::Tensor match_logprob_bwd(const c10::optional<at::Tensor>& gl,
-                             const c10::optional<at::Tensor>& gh,
-                             const at::Tensor& z, const at::Tensor& y,
-                             const c10::optional<at::Tensor>& n,
-                             const at::Tensor& logp, const at::Tensor& ent,
-                             const at::Tensor& stat);
-namespace segattn {
-std::tuple<at::Tensor, at::Tensor, at::Tensor> segment_attention_fwd(
-    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-    const at::Tensor& ptr_q, const at::Tensor& ptr_k, double scale,
-    double cap, const c10::optional<at::Tensor>& bias,
-    const c10::optional<at::Tensor>& pos_q,
-    const c10::optional<at::Tensor>& pos_k, int64_t half, int64_t mbits,
-    double dmax, bool train);
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>
-segment_attention_bwd(const at::Tensor& dout, const at::Tensor& q,
-                      const at::Tensor& k, const at::Tensor& v,
-                      const at::Tensor& out, const at::Tensor& lo,
-                      const at::Tensor& lse, const at::Tensor& ptr_q, const at::Tensor& ptr_k,
-                      double scale, double cap,
-                      const c10::optional<at::Tensor>& bias,
-                      const c10::optional<at::Tensor>& pos_q,
-                      const c10::optional<at::Tensor>& pos_k, int64_t half,
-                      int64_t mbits, double dmax);
-}  // namespace segattn
 void relconv_fwd(const at::Tensor& ptr, const at::Tensor& col,
                  const at::Tensor& split, const at::Tensor& hub,
                  const at::Tensor& xa, const c10::optional<at::Tensor>& xb,
@@ -649,28 +613,6 @@ TORCH_LIBRARY(dgmc_amd, m) {
       "sinkhorn_transport_bwd(Tensor? grad_P, Tensor grad_joint, Tensor r_s, "
       "Tensor S_hat, Tensor ptr_s, Tensor ptr_t, Tensor a_hist, Tensor "
       "b_hist, int iters, float tau, Tensor? add) -> Tensor");
-  m.def(
-      "layer_norm_fwd(Tensor x, Tensor? residual, Tensor? weight, Tensor? "
-      "bias, float eps, bool train) -> (Tensor, Tensor, Tensor)");
-  m.def(
-      "layer_norm_bwd(Tensor dy, Tensor? ds, Tensor s, Tensor stat, Tensor? "
-      "weight, bool with_weight) -> (Tensor, Tensor, Tensor)");
-  m.def(
-      "match_logprob_fwd(Tensor z, Tensor y, Tensor? n, int k, bool train) -> "
-      "(Tensor, Tensor, Tensor, Tensor, Tensor)");
-  m.def(
-      "match_logprob_bwd(Tensor? gl, Tensor? gh, Tensor z, Tensor y, Tensor? "
-      "n, Tensor logp, Tensor ent, Tensor stat) -> Tensor");
-  m.def(
-      "segment_attention_fwd(Tensor q, Tensor k, Tensor v, Tensor ptr_q, "
-      "Tensor ptr_k, float scale, float cap, Tensor? bias, Tensor? pos_q, "
-      "Tensor? pos_k, int half, int mbits, float dmax, bool train) -> "
-      "(Tensor, Tensor, Tensor)");
-  m.def(
-      "segment_attention_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, "
-      "Tensor out, Tensor lo, Tensor lse, Tensor ptr_q, Tensor ptr_k, float scale, "
-      "float cap, Tensor? bias, Tensor? pos_q, Tensor? pos_k, int half, int "
-      "mbits, float dmax) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(dgmc_amd, CompositeExplicitAutograd, m) {
@@ -765,10 +707,4 @@ TORCH_LIBRARY_IMPL(dgmc_amd, CUDA, m) {
   m.impl("sinkhorn_bwd", &dgmc::sinkhorn_bwd);
   m.impl("sinkhorn_transport", &dgmc::sinkhorn_transport);
   m.impl("sinkhorn_transport_bwd", &dgmc::sinkhorn_transport_bwd);
-  m.impl("layer_norm_fwd", &dgmc::layer_norm_fwd);
-  m.impl("layer_norm_bwd", &dgmc::layer_norm_bwd);
-  m.impl("match_logprob_fwd", &dgmc::match_logprob_fwd);
-  m.impl("match_logprob_bwd", &dgmc::match_logprob_bwd);
-  m.impl("segment_attention_fwd", &dgmc::segattn::segment_attention_fwd);
-  m.impl("segment_attention_bwd", &dgmc::segattn::segment_attention_bwd);
 }

@@ -1,6 +1,7 @@
 // Segment attention: entry points, the join of split keys and the sum of the
 // bias table's gradient.  The kernels are in segment_attention_{fwd,bwd}.h,
 // instantiated per type in segment_attention_{fwd,bwd}_{bf16,f32}.hip.
+#include "attentional.h"
 #include "segment_attention.h"
 
 namespace dgmc {
@@ -206,10 +207,11 @@ static int rows16(const at::Tensor& t) {
 static Args make_args(const at::Tensor& q, const at::Tensor& k,
                       const at::Tensor& v, const at::Tensor& ptr_q,
                       const at::Tensor& ptr_k, double scale, double cap,
-                      const c10::optional<at::Tensor>& bias,
-                      const c10::optional<at::Tensor>& pos_q,
-                      const c10::optional<at::Tensor>& pos_k, int64_t half,
-                      int64_t mbits, double dmax, int& axes) {
+                      const OptTensor& bias, const OptTensor& pos_q,
+                      const OptTensor& pos_k, const BucketLayout& layout,
+                      int& axes) {
+  const int64_t half = layout.half, mbits = layout.mbits;
+  const double dmax = layout.dmax;
   check_heads(q, "q", q);
   check_heads(k, "k", q);
   check_heads(v, "v", q);
@@ -300,16 +302,14 @@ static bool split_axis(Args& a, int64_t tiles, int64_t n, int tile) {
   return a.splits > 1;
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> segment_attention_fwd(
+std::tuple<at::Tensor, at::Tensor, at::Tensor> forward(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& ptr_q, const at::Tensor& ptr_k, double scale,
-    double cap, const c10::optional<at::Tensor>& bias,
-    const c10::optional<at::Tensor>& pos_q,
-    const c10::optional<at::Tensor>& pos_k, int64_t half, int64_t mbits,
-    double dmax, bool train) {
+    double cap, const OptTensor& bias, const OptTensor& pos_q,
+    const OptTensor& pos_k, const BucketLayout& layout, bool train) {
   int axes;
   Args a = make_args(q, k, v, ptr_q, ptr_k, scale, cap, bias, pos_q, pos_k,
-                     half, mbits, dmax, axes);
+                     layout, axes);
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   const auto f32 = q.options().dtype(at::kFloat);
   at::Tensor out = at::empty({a.Nq, a.H, a.D}, q.options());
@@ -337,19 +337,15 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> segment_attention_fwd(
   return {out, lo, lse};
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>
-segment_attention_bwd(const at::Tensor& dout, const at::Tensor& q,
-                      const at::Tensor& k, const at::Tensor& v,
-                      const at::Tensor& out, const at::Tensor& lo,
-                      const at::Tensor& lse, const at::Tensor& ptr_q, const at::Tensor& ptr_k,
-                      double scale, double cap,
-                      const c10::optional<at::Tensor>& bias,
-                      const c10::optional<at::Tensor>& pos_q,
-                      const c10::optional<at::Tensor>& pos_k, int64_t half,
-                      int64_t mbits, double dmax) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
+    const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k,
+    const at::Tensor& v, const at::Tensor& out, const at::Tensor& lo,
+    const at::Tensor& lse, const at::Tensor& ptr_q, const at::Tensor& ptr_k,
+    double scale, double cap, const OptTensor& bias, const OptTensor& pos_q,
+    const OptTensor& pos_k, const BucketLayout& layout) {
   int axes;
   Args a = make_args(q, k, v, ptr_q, ptr_k, scale, cap, bias, pos_q, pos_k,
-                     half, mbits, dmax, axes);
+                     layout, axes);
   check_heads(dout, "dout", q);
   TORCH_CHECK(dout.sizes() == q.sizes() && out.sizes() == q.sizes() &&
                   out.scalar_type() == q.scalar_type() &&

@@ -15,7 +15,6 @@ every sum has a fixed order.  CPU tensors use the oracle in
 :mod:`.reference`.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _backend
 from . import reference as ref
@@ -41,34 +40,6 @@ def bucket_starts(half, octave_steps=1):
 def bias_width(half, axes=1):
     """Columns of a bias table: ``2 half + 1`` signed buckets per axis."""
     return (2 * half + 1) ** axes
-
-
-class _SegmentAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k, scale, cap,
-                layout):
-        grad = any(ctx.needs_input_grad[:4])
-        out, lo, lse = _backend.ops().segment_attention_fwd(
-            q, k, v, ptr_q, ptr_k, scale, cap, bias, pos_q, pos_k, *layout,
-            grad)
-        if grad:
-            ctx.save_for_backward(q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k,
-                                  out, lo, lse)
-            ctx.args = (scale, cap, layout)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k, out, lo, lse = \
-            ctx.saved_tensors
-        scale, cap, layout = ctx.args
-        if grad.stride(-1) != 1 and grad.size(-1) != 1:
-            grad = grad.contiguous()
-        dq, dk, dv, db = _backend.ops().segment_attention_bwd(
-            grad, q, k, v, out, lo, lse, ptr_q, ptr_k, scale, cap, bias, pos_q,
-            pos_k, *layout)
-        return (dq, dk, dv, None if bias is None else db) + (None, ) * 7
 
 
 def _check(q, k, v, ptr_q, ptr_k, cap):
@@ -206,6 +177,6 @@ def segment_attention(q, k, v, ptr_q, ptr_k=None, scale=None, cap=0.0,
                for t in (q, k, v))
     if bias is not None:
         bias = bias.float().contiguous()
-    return _SegmentAttention.apply(q, k, v, bias, ptr_q.contiguous(),
-                                   ptr_k.contiguous(), pos_q, pos_k, scale,
-                                   float(cap), layout)
+    return _backend.ops().segment_attention.default(
+        q, k, v, bias, ptr_q.contiguous(), ptr_k.contiguous(), pos_q, pos_k,
+        scale, float(cap), *layout)

@@ -8,7 +8,6 @@ The scores are never normalised in memory.  CPU tensors use the oracle in
 import collections
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _backend
 from . import reference as ref
@@ -17,30 +16,6 @@ MAX_TOP = 32
 
 MatchLogProbs = collections.namedtuple(
     'MatchLogProbs', ['log_prob', 'entropy', 'top_log_prob', 'top_index'])
-
-
-class _MatchLogProbs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, scores, target, n_cols, top):
-        grad = ctx.needs_input_grad[0]
-        logp, ent, top_lp, top_idx, stat = _backend.ops().match_logprob_fwd(
-            scores, target, n_cols, top, grad)
-        ctx.mark_non_differentiable(top_lp, top_idx)
-        if grad:
-            ctx.save_for_backward(scores, target, n_cols, logp, ent, stat)
-            ctx.set_materialize_grads(False)
-        return logp, ent, top_lp, top_idx
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gl, gh, _lp, _idx):
-        if gl is None and gh is None:
-            return None, None, None, None
-        scores, target, n_cols, logp, ent, stat = ctx.saved_tensors
-        gl, gh = (None if g is None else g.float().contiguous()
-                  for g in (gl, gh))
-        return _backend.ops().match_logprob_bwd(
-            gl, gh, scores, target, n_cols, logp, ent, stat), None, None, None
 
 
 def match_log_probs(scores, target, n_cols=None, top=0):
@@ -89,6 +64,6 @@ def match_log_probs(scores, target, n_cols=None, top=0):
                          '{}'.format(scores.dtype))
     if scores.stride(1) != 1 and scores.size(1) > 1:
         scores = scores.contiguous()
-    return MatchLogProbs(*_MatchLogProbs.apply(
+    return MatchLogProbs(*_backend.ops().match_logprob.default(
         scores, target.contiguous(),
         None if n_cols is None else n_cols.contiguous(), int(top)))

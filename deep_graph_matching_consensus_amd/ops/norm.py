@@ -5,41 +5,11 @@ with an optional residual added on the way.  CPU tensors use the oracle in
 :mod:`.reference`.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _backend
 from . import reference as ref
 
 MAX_COLUMNS = 8192
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, weight, bias, eps):
-        grad = any(ctx.needs_input_grad[:4])
-        y, s, stat = _backend.ops().layer_norm_fwd(x, residual, weight, bias,
-                                                   eps, grad)
-        if residual is None:
-            s = x
-        if grad:
-            ctx.save_for_backward(s, weight, stat)
-            ctx.set_materialize_grads(False)
-        ctx.has_bias = bias is not None
-        return (y, s) if residual is not None else y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, ds=None):
-        s, weight, stat = ctx.saved_tensors
-        if dy is None:
-            return ds, ds, None, None, None
-        need_w = weight is not None and any(ctx.needs_input_grad[2:4])
-        dx, dw, db = _backend.ops().layer_norm_bwd(
-            dy.contiguous(), None if ds is None else ds.contiguous(), s,
-            stat, weight, need_w)
-        return (dx, dx if ctx.needs_input_grad[1] else None,
-                dw if need_w else None,
-                db if need_w and ctx.has_bias else None, None)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
@@ -84,7 +54,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
     res = None if residual is None else residual.reshape(-1, C).contiguous()
     weight, bias = (None if t is None else t.float().contiguous()
                     for t in (weight, bias))
-    out = _LayerNorm.apply(flat, res, weight, bias, float(eps))
-    if residual is None:
-        return out.view(x.shape)
-    return out[0].view(x.shape), out[1].view(x.shape)
+    out = _backend.ops().layer_norm.default(flat, res, weight, bias,
+                                            float(eps))
+    out = [t.view(x.shape) for t in out]
+    return out[0] if residual is None else tuple(out)

@@ -234,3 +234,12 @@ def test_repeats_and_captured_replays_are_identical():
         torch.cuda.synchronize()
         for a, b in zip(outs, eager):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    x = torch.randn(3, 16, device='cuda', requires_grad=True)
+    g, = torch.autograd.grad(layer_norm(x).square().sum(), x,
+                             create_graph=True)
+    with pytest.raises(RuntimeError, match='differentiated again'):
+        g.sum().backward()

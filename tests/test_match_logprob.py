@@ -290,3 +290,13 @@ def test_repeats_and_captured_replays_are_identical(V):
         torch.cuda.synchronize()
         for a, b in zip(outs, eager):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    z = torch.randn(3, 16, device='cuda', requires_grad=True)
+    y = torch.zeros(3, dtype=torch.long, device='cuda')
+    g, = torch.autograd.grad(match_log_probs(z, y).entropy.sum(), z,
+                             create_graph=True)
+    with pytest.raises(RuntimeError, match='differentiated again'):
+        g.sum().backward()

@@ -522,3 +522,13 @@ def test_offsets_past_32_bits():
     ptr = torch.tensor([0, n], dtype=torch.int32, device='cuda')
     assert torch.equal(segment_attention(x, k, k, ptr),
                        segment_attention(x, x, x, ptr))
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    q = torch.randn(5, 1, 16, device='cuda', requires_grad=True)
+    ptr = torch.tensor([0, 5], dtype=torch.int32, device='cuda')
+    g, = torch.autograd.grad(segment_attention(q, q, q, ptr).sum(), q,
+                             create_graph=True)
+    with pytest.raises(RuntimeError, match='differentiated again'):
+        g.sum().backward()
