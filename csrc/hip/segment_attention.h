@@ -12,13 +12,19 @@
 // / G)), so every K / V tile staged in LDS serves all of them, a single new
 // query fills G rows, and dK / dV sum over the group inside one workgroup.
 //
-// Work list without a plan.  Segment b's tiles occupy the slots from
-// f(b) = ptr[b] / TQ + b on (TQ queries per tile): f grows by at least
-// ceil(n_b / TQ) per segment, so floor(N / TQ) + B + 1 slots always suffice
-// and the grid depends on N and B only - no host copy of ptr, no sort, and
-// a captured graph may change ptr between replays.  A wave finds its
-// segment by a 64-way search (two dependent loads for B <= 4096).  Slots
-// without a tile end at once.
+// Tiles are consecutive packed rows, whatever segments they belong to: a
+// tile visits the keys from its first row's segment to its last row's, and
+// where it spans several segments each lane masks by its own row's key range
+// (a wave skips key tiles outside all of its rows).  Small graphs so share a
+// tile (9-node graphs: 3 to 4 a wave) and the grid depends on N only - no
+// plan, no host copy of ptr, and a captured graph may change ptr between
+// replays.  A masked pair's weight is 0, but 0 times a NaN or inf of another
+// segment is NaN in a product that sums over the tile: a tile of several
+// segments that ends with a non-finite result is done again segment by
+// segment, each on its own rows alone, so segments never touch each other.
+// Rows find their segments on the device: a 64-way wave search for
+// the tile's first row (two dependent loads for B <= 4096), then the next 64
+// boundaries, one a lane, searched in registers.
 //
 // Matrix products.  32 x 32 accumulators: lane l holds column l & 31 and
 // rows 8 (r / 4) + 4 (l >> 5) + r % 4.  Scores are formed TRANSPOSED to the
@@ -79,33 +85,91 @@ __device__ __forceinline__ int split_tiles(const Args& a, int n) {
   return max(a.chunk, (n + a.splits - 1) / a.splits);
 }
 
-// Segment `b` rows (clamped to [0, N]; the first segment starts at row 0,
-// "segment" B is the tail behind the last one).
+// First row of segment `b` (clamped to [0, N]; the first segment starts at
+// row 0, "segment" B is the tail behind the last one).
 __device__ __forceinline__ int seg_begin(const int* ptr, int b, int N) {
   return b == 0 ? 0 : min(max(ptr[b], 0), N);
 }
-__device__ __forceinline__ void seg_range(const int* ptr, int b, int B, int N,
-                                          int& lo, int& hi) {
-  lo = seg_begin(ptr, b, N);
-  hi = b >= B ? N : min(max(ptr[b + 1], lo), N);
-}
 
-// Largest b in [0, B] with f(b) <= slot (wave-uniform result).
-__device__ __forceinline__ int find_segment(const int* ptr, int B, int N,
-                                            int per, int slot) {
+// Segment of a (wave-uniform) row: the last b in [0, B] that begins at or
+// before it.
+__device__ __forceinline__ int segment_of(const int* ptr, int B, int N,
+                                          int row) {
   const int lane = threadIdx.x & 63;
   int lo = 0, n = B + 1;
   while (n > 1) {
     const int step = (n + 63) >> 6;
-    const int idx = lo + lane * step;
     bool ok = lane * step < n;
-    if (ok) ok = seg_begin(ptr, idx, N) / per + idx <= slot;
-    const int c = max(__popcll(__ballot(ok)), 1);
-    const int adv = (c - 1) * step;
+    if (ok) ok = seg_begin(ptr, lo + lane * step, N) <= row;
+    const int adv = (max(__popcll(__ballot(ok)), 1) - 1) * step;
     lo += adv;
     n = min(step, n - adv);
   }
   return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// Segment of every lane's own `row`, at or behind a row of segment b0.
+__device__ __forceinline__ int lane_segment(const int* ptr, int B, int N,
+                                            int b0, int row) {
+  const int lane = threadIdx.x & 63;
+  int seg = b0;
+  for (int base = b0 + 1;; base += 64) {
+    const int e = base + lane <= B ? seg_begin(ptr, base + lane, N)
+                                   : 0x7fffffff;
+    int n = 0;                    // boundaries at or before the row
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1)
+      if (__shfl(e, n + s - 1) <= row) n += s;
+    if (n == 63 && __shfl(e, 63) <= row) n = 64;
+    seg += n;
+    if (!__any(n == 64)) return seg;
+  }
+}
+
+// Rows [lo, hi) of segment `seg` on the other side (none of the tail's).
+__device__ __forceinline__ void seg_range(const int* ptr, int seg, int B,
+                                          int N, int& lo, int& hi) {
+  const int b = min(seg, B);
+  lo = b == 0 && B == 0 ? N : seg_begin(ptr, b, N);
+  hi = b < B ? min(max(ptr[b + 1], lo), N) : lo;
+}
+
+// Segments [b0, b1] of a tile of own rows [r0, r1), and the other side's
+// rows [lo, hi) that it visits.
+__device__ __forceinline__ void tile_range(const int* own, const int* other,
+                                           int B, int N, int No, int r0,
+                                           int r1, int& b0, int& b1, int& lo,
+                                           int& hi) {
+  b0 = segment_of(own, B, N, r0);
+  b1 = segment_of(own, B, N, r1 - 1);
+  int x;
+  seg_range(other, b0, B, No, lo, x);
+  seg_range(other, b1, B, No, x, hi);
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = max(__builtin_amdgcn_readfirstlane(hi), lo);
+}
+
+// Whether an accumulator of this lane is not finite.
+template <int M>
+__device__ __forceinline__ bool not_finite(const f32x16 (&acc)[M]) {
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < M; ++k)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s = fmaf(acc[k][r], 0.f, s);
+  return s != 0.f;
+}
+
+// Workgroup-wide any().
+template <int NW>
+__device__ __forceinline__ bool any_lane(bool v) {
+  if constexpr (NW == 1) return __any(v);
+  else return __syncthreads_or(v);
+}
+
+// Lane value of a wave-uniform lane number.
+__device__ __forceinline__ int lane_int(int v, int lane) {
+  return __builtin_amdgcn_readlane(v, lane);
 }
 
 // 16-byte chunk swizzle of an LDS tile row with CH chunks: both 16-byte
@@ -347,6 +411,22 @@ __device__ __forceinline__ void put4(T* row, int d, int D, const T* v) {
     for (int r = 0; r < 4; ++r)
       if (d + r < D) row[d + r] = v[r];
   }
+}
+
+// A wave's accumulators -> its lanes' output rows.
+template <int DP, typename T>
+__device__ __forceinline__ void put_acc(T* row, const f32x16 (&acc)[DP / 32],
+                                        int D, float scale) {
+  const int h = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      T o[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = (T)(acc[k][4 * r4 + r] * scale);
+      put4(row, 32 * k + 8 * r4 + 4 * h, D, o);
+    }
 }
 
 // Chunk (row, ch) of a swizzled LDS tile.

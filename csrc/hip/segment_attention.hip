@@ -29,24 +29,21 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int per_tile,
                                                    int key_tile) {
   __shared__ float red[256][9];
   __shared__ float wsum[16];
-  const int kvh = blockIdx.x % a.KV, slot = blockIdx.x / a.KV;
+  __shared__ float2 ml[16][kMaxSplits];
+  const int kvh = blockIdx.x % a.KV;
   const int* own = MODE == DKV ? a.ptr_k : a.ptr_q;
   const int* other = MODE == DKV ? a.ptr_q : a.ptr_k;
   const int N = MODE == DKV ? a.Nk : a.Nq, No = MODE == DKV ? a.Nq : a.Nk;
-  const int seg = find_segment(own, a.B, N, per_tile, slot);
-  if (seg >= a.B) return;
-  int lo, hi, o_lo, o_hi;
-  seg_range(own, seg, a.B, N, lo, hi);
-  lo += (slot - (seg_begin(own, seg, N) / per_tile + seg)) * per_tile;
-  if (lo >= hi) return;
-  seg_range(other, seg, a.B, No, o_lo, o_hi);
+  const int lo = blockIdx.x / a.KV * per_tile, hi = min(lo + per_tile, N);
+  int b0, b1, o_lo, o_hi;
+  tile_range(own, other, a.B, N, No, lo, hi, b0, b1, o_lo, o_hi);
   const int ntile = (o_hi - o_lo + key_tile - 1) / key_tile;
   const int per = split_tiles(a, ntile);
   if (per >= ntile) return;
   const int ns = (ntile + per - 1) / per;
 
   const int G = MODE == DKV ? 1 : a.G, heads = G * a.KV;
-  const int rows = min(per_tile, hi - lo) * G;
+  const int rows = (hi - lo) * G;
   const int64_t all = (int64_t)N * heads;
   const int grp = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
   // `ways` (a power of two) groups share a row; 16 / ways rows a round.
@@ -63,19 +60,30 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int per_tile,
     float M = -INFINITY, L = 0.f, o[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) o[k] = 0.f;
+    if (MODE == FWD) {
+      // The round's maxima and sums, all loads at once.
+      __syncthreads();
+      for (int e = threadIdx.x; e < rpr * ns; e += 256) {
+        const int q = e / ns, s = e - q * ns;
+        if (r0 + q < rows) {
+          const int64_t w = (int64_t)(lo + (r0 + q) / G) * heads + kvh * G +
+                            (r0 + q) % G;
+          ml[q][s] = *(const float2*)(a.part_ml + (s * all + w) * 2);
+        }
+      }
+      __syncthreads();
+    }
     if (live) {
       if (MODE == FWD) {
-#pragma unroll 4
-        for (int s = 0; s < ns; ++s)
-          M = fmaxf(M, a.part_ml[(s * all + row) * 2]);
+        for (int s = 0; s < ns; ++s) M = fmaxf(M, ml[rr][s].x);
         if (M == -INFINITY) M = 0.f;
       }
 #pragma unroll 4
       for (int s = way; s < ns; s += ways) {
         float w = 1.f;
         if (MODE == FWD) {
-          w = exp2_(a.part_ml[(s * all + row) * 2] - M);
-          L += w * a.part_ml[(s * all + row) * 2 + 1];
+          w = exp2_(ml[rr][s].x - M);
+          L += w * ml[rr][s].y;
         }
         const float* p = part + (s * all + row) * a.D;
         if (a.D % 4 == 0 && d0 + 8 <= a.D) {
@@ -133,7 +141,7 @@ static void join(const Args& a, bool f32, int per_tile, int key_tile) {
   const int N = MODE == DKV ? a.Nk : a.Nq;
   // (workgroups along z share a tile's rows, 16 a round)
   const int G = MODE == DKV ? 1 : a.G;
-  const dim3 grid((N / per_tile + a.B + 1) * a.KV, MODE == DKV ? 2 : 1,
+  const dim3 grid((N + per_tile - 1) / per_tile * a.KV, MODE == DKV ? 2 : 1,
                   (per_tile * G + 15) / 16);
   if (f32)
     join_kernel<float, MODE><<<grid, 256, 0, stream()>>>(a, per_tile,
@@ -241,10 +249,8 @@ static Args make_args(const at::Tensor& q, const at::Tensor& k,
   // 32-bit row numbers and launch sizes (threads of a launch < 2^32).
   const int64_t lim = (int64_t)1 << 31;
   TORCH_CHECK(q.size(0) < lim - 4096 && k.size(0) < lim - 4096 &&
-                  (q.size(0) * a.G + 64 * (int64_t)a.B + 64) * a.KV <
-                      ((int64_t)1 << 30) &&
-                  (k.size(0) + 64 * (int64_t)a.B + 64) * a.KV <
-                      ((int64_t)1 << 30),
+                  q.size(0) * a.H < ((int64_t)1 << 30) &&
+                  k.size(0) * a.KV < ((int64_t)1 << 30),
               "segment_attention: too many rows for one call");
   a.Nq = (int)q.size(0); a.Nk = (int)k.size(0);
   a.ptr_q = ptr_q.data_ptr<int>(); a.ptr_k = ptr_k.data_ptr<int>();
@@ -397,7 +403,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
   int nblk = 0;
   at::Tensor part;
   if (axes) {
-    const int items = (a.Nq / TQ + a.B + 1) * a.splits;
+    const int items = (a.Nq + TQ - 1) / TQ * a.splits;
     nblk = std::max(1, std::min(items, 2048 / (a.KV * nwq)));
     part = at::empty({nblk, a.KV, a.G, a.slots}, f32);
     a.part_bias = part.data_ptr<float>();

@@ -80,25 +80,9 @@ __device__ __forceinline__ void add_slots(DGMC_LDS float* hist,
   }
 }
 
-// A wave's accumulators -> its lanes' output rows.
-template <int DP, typename T>
-__device__ __forceinline__ void put_acc(T* row, const f32x16 (&acc)[DP / 32],
-                                        int D, float scale) {
-  const int h = (threadIdx.x >> 5) & 1;
-#pragma unroll
-  for (int k = 0; k < DP / 32; ++k)
-#pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      T o[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) o[r] = (T)(acc[k][4 * r4 + r] * scale);
-      put4(row, 32 * k + 8 * r4 + 4 * h, D, o);
-    }
-}
-
 template <typename T, int DP, int NW, int POS>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(const Args a,
-                                                        int nslot) {
+                                                        int ntiles) {
   constexpr int KT = 32;
   constexpr int CH = DP * (int)sizeof(T) / 16;
   constexpr int NT = NW * 64;
@@ -125,22 +109,21 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(con
   }
   const int64_t ksb = a.k_sn * (int)sizeof(T), vsb = a.v_sn * (int)sizeof(T);
 
-  for (int it = blk; it < nslot * a.splits; it += nblk) {
-    const int slot = it / a.splits, split = it % a.splits;
-    const int seg = find_segment(a.ptr_q, a.B, a.Nq, TQ, slot);
-    int q_lo, q_hi, k_lo = 0, k_hi = 0;
-    seg_range(a.ptr_q, seg, a.B, a.Nq, q_lo, q_hi);
-    q_lo += (slot - (seg_begin(a.ptr_q, seg, a.Nq) / TQ + seg)) * TQ;
-    if (q_lo >= q_hi) continue;
-    if (seg < a.B) seg_range(a.ptr_k, seg, a.B, a.Nk, k_lo, k_hi);
+  for (int it = blk; it < ntiles * a.splits; it += nblk) {
+    const int split = it % a.splits;
+    const int q_lo = it / a.splits * TQ, q_hi = min(q_lo + TQ, a.Nq);
+    int b0, b1, k_lo, k_hi;
+    tile_range(a.ptr_q, a.ptr_k, a.B, a.Nq, a.Nk, q_lo, q_hi, b0, b1, k_lo,
+               k_hi);
+    const int ntile = (k_hi - k_lo + KT - 1) / KT;
+    const int per = split_tiles(a, ntile);
+    if (split > 0 && split * per >= ntile) continue;
+    k_lo += split * per * KT;
+    k_hi = min(k_lo + per * KT, k_hi);
 
     const int64_t qi = (int64_t)q_lo + wave * QW + c / a.G;
     const bool live = c < QW * a.G && qi < q_hi;
     const int64_t row = qi * a.H + head;
-    const int ntile = (k_hi - k_lo + KT - 1) / KT;
-    const int per = split_tiles(a, ntile);
-    const int t0 = split * per, t1 = min(t0 + per, ntile);
-    if (split > 0 && t0 >= t1) continue;
     const int qo = wave * QW + c / a.G;
     u32x4 qf[CH / 2], gf[CH / 2], of[CH / 2];
     load_frags<T>(qf,
@@ -173,23 +156,35 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(con
       if (POS == 2) py = load_pos(a.pos_q, qi, POS, 1);
     }
 
-    const T* kbase =
-        (const T*)a.k + (int64_t)k_lo * a.k_sn + (int64_t)kvh * a.k_sh;
-    const T* vbase =
-        (const T*)a.v + (int64_t)k_lo * a.v_sn + (int64_t)kvh * a.v_sh;
+    // The row's own keys; the wave's first and last row bound them all.
+    const int w0 = q_lo + wave * QW, wrows = min(QW, q_hi - w0);
+    int r_lo = 0, r_hi = 0, f_lo = 0, f_hi = 0, l_lo = 0, l_hi = 0;
+    int seg = -1;
+    if (wrows > 0) {
+      seg = lane_segment(a.ptr_q, a.B, a.Nq,
+                         segment_of(a.ptr_q, a.B, a.Nq, w0),
+                         min((int)qi, q_hi - 1));
+      seg_range(a.ptr_k, seg, a.B, a.Nk, r_lo, r_hi);
+      const int last = (wrows - 1) * a.G;
+      f_lo = lane_int(r_lo, 0), f_hi = lane_int(r_hi, 0);
+      l_lo = lane_int(r_lo, last), l_hi = lane_int(r_hi, last);
+    }
+
+    const T* kbase = (const T*)a.k + (int64_t)kvh * a.k_sh;
+    const T* vbase = (const T*)a.v + (int64_t)kvh * a.v_sh;
     float pr[2] = {0.f, 0.f};
-    auto fetch = [&](int t, int buf) {
+    auto fetch = [&](int k0, int e, int buf) {
       using S = Stager<T, KT, CH, NT>;
-      const int left = k_hi - k_lo - t * KT;
+      const int left = e - k0;
       DGMC_LDS char* kt = lds + buf * 2 * TB;
       const auto ok = [&](int r) { return r < left; };
-      S::fill(kbase + (int64_t)t * KT * a.k_sn, a.D, a.vec_k, kt, ok,
+      S::fill(kbase + (int64_t)k0 * a.k_sn, a.D, a.vec_k, kt, ok,
               [&](int r) { return r * ksb; });
-      S::fill(vbase + (int64_t)t * KT * a.v_sn, a.D, a.vec_v, kt + TB, ok,
+      S::fill(vbase + (int64_t)k0 * a.v_sn, a.D, a.vec_v, kt + TB, ok,
               [&](int r) { return r * vsb; });
       if constexpr (POS > 0) {
         if (tid < KT && tid < left) {
-          const int64_t j = (int64_t)k_lo + t * KT + tid;
+          const int64_t j = (int64_t)k0 + tid;
           pr[0] = load_pos(a.pos_k, j, POS, 0);
           if (POS == 2) pr[1] = load_pos(a.pos_k, j, POS, 1);
         }
@@ -204,19 +199,28 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(con
       }
     };
 
+    // Passes as in the forward; the table's gradient is whole after the first
+    // (no sum over a tile enters a dz).
+    for (int pass = b0 - 1;; ++pass) {
+    int p_lo = k_lo, p_hi = k_hi;
+    if (pass >= b0) {
+      seg_range(a.ptr_k, pass, a.B, a.Nk, p_lo, p_hi);
+      p_lo = max(p_lo, k_lo);
+      p_hi = min(p_hi, k_hi);
+    }
     f32x16 acc[DP / 32];
 #pragma unroll
     for (int k = 0; k < DP / 32; ++k)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[k][r] = 0.f;
 
-    stage_barrier();       // the previous slot's last tile has been read
-    if (t0 < t1) fetch(t0, 0);
-    for (int t = t0; t < t1; ++t) {
-      const int buf = (t - t0) & 1;
+    stage_barrier();       // the last tile staged before has been read
+    if (p_lo < p_hi) fetch(p_lo, p_hi, 0);
+    for (int k0 = p_lo, buf = 0; k0 < p_hi; k0 += KT, buf ^= 1) {
       put_pos(buf);
       stage_barrier();
-      if (t + 1 < t1) fetch(t + 1, buf ^ 1);
+      if (k0 + KT < p_hi) fetch(k0 + KT, p_hi, buf ^ 1);
+      if (k0 >= l_hi || k0 + KT <= f_lo) continue;  // none of this wave's
       const DGMC_LDS char* kt = lds + buf * 2 * TB;
       f32x16 z, dp, th;
 #pragma unroll
@@ -246,17 +250,19 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(con
           }
         }
       }
-      const int left = k_hi - (k_lo + t * KT);
-      if (left < KT) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (8 * (r >> 2) + 4 * h + (r & 3) >= left) z[r] = -INFINITY;
-      }
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         z[r] = exp2_(z[r] - lse) * (dp[r] - dl);
+      if (k0 < l_lo || k0 + KT > f_hi) {
+        // (selected, not multiplied away: a masked key may hold NaN)
+        const unsigned n = r_hi - r_lo;
+        const int j0 = k0 + 4 * h - r_lo;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if ((unsigned)(j0 + 8 * (r >> 2) + (r & 3)) >= n) z[r] = 0.f;
+      }
       if constexpr (POS > 0) {
-        add_slots<POS == 1>(myhist, sl, z);
+        if (pass < b0) add_slots<POS == 1>(myhist, sl, z);
       }
       if (a.cap > 0.f) {
 #pragma unroll
@@ -264,12 +270,16 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(con
       }
       Mma<T>::template accum<DP>(acc, kt, 0, z);
     }
-    if (live) {
+    const bool redo =
+        pass < b0 && b1 > b0 && any_lane<NW>(live && not_finite(acc));
+    if (!redo && live && (pass < b0 || seg == pass)) {
       if (per < ntile)          // joined by join_kernel
         put_acc<DP>(a.part_o + ((int64_t)split * a.Nq * a.H + row) * a.D, acc,
                     a.D, 1.f);
       else
         put_acc<DP>((T*)a.dq + row * a.D, acc, a.D, a.scale);
+    }
+    if (pass < b0 ? !redo : pass == b1) break;
     }
   }
   if constexpr (POS > 0) {
@@ -306,23 +316,34 @@ __global__
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int h = lane >> 5, c = lane & 31;
-  const int kvh = blockIdx.x % a.KV, slot = blockIdx.x / a.KV;
+  const int kvh = blockIdx.x % a.KV;
   const int QW = 32 / a.G, RW = QW * a.G;
-  const int seg = find_segment(a.ptr_k, a.B, a.Nk, 32 * NW, slot);
-  int k_lo, k_hi, q_lo = 0, q_hi = 0;
-  seg_range(a.ptr_k, seg, a.B, a.Nk, k_lo, k_hi);
-  k_lo += (slot - (seg_begin(a.ptr_k, seg, a.Nk) / (32 * NW) + seg)) * 32 *
-          NW;
-  if (k_lo >= k_hi) return;
-  if (seg < a.B) seg_range(a.ptr_q, seg, a.B, a.Nq, q_lo, q_hi);
+  const int k_lo = blockIdx.x / a.KV * 32 * NW;
+  const int k_hi = min(k_lo + 32 * NW, a.Nk);
+  int b0, b1, q_lo, q_hi;
+  tile_range(a.ptr_k, a.ptr_q, a.B, a.Nk, a.Nq, k_lo, k_hi, b0, b1, q_lo,
+             q_hi);
 
   const int64_t kj = (int64_t)k_lo + wave * 32 + c;
   const bool live = kj < k_hi;
-  // Query tiles [t0, t1) of this split.
+  // The queries of this split.
   const int ntile = (q_hi - q_lo + QW - 1) / QW;
   const int per = split_tiles(a, ntile), split = blockIdx.y;
-  const int t0 = split * per, t1 = min(t0 + per, ntile);
-  if (split > 0 && t0 >= t1) return;
+  if (split > 0 && split * per >= ntile) return;
+  q_lo += split * per * QW;
+  q_hi = min(q_lo + per * QW, q_hi);
+  // The key's own queries; the wave's first and last key bound them all.
+  const int w0 = k_lo + wave * 32, wrows = min(32, k_hi - w0);
+  int r_lo = 0, r_hi = 0, f_lo = 0, f_hi = 0, l_lo = 0, l_hi = 0;
+  int seg = -1;
+  if (wrows > 0) {
+    seg = lane_segment(a.ptr_k, a.B, a.Nk,
+                       segment_of(a.ptr_k, a.B, a.Nk, w0),
+                       min((int)kj, k_hi - 1));
+    seg_range(a.ptr_q, seg, a.B, a.Nq, r_lo, r_hi);
+    f_lo = lane_int(r_lo, 0), f_hi = lane_int(r_hi, 0);
+    l_lo = lane_int(r_lo, wrows - 1), l_hi = lane_int(r_hi, wrows - 1);
+  }
   const int ko = wave * 32 + c;
   u32x4 kf[CH / 2], vf[CH / 2];
   load_frags<T>(kf,
@@ -350,23 +371,21 @@ __global__
 
   const int64_t qsb = a.q_sn * (int)sizeof(T), qhb = a.q_sh * (int)sizeof(T);
   const int64_t gsb = a.g_sn * (int)sizeof(T), ghb = a.g_sh * (int)sizeof(T);
-  const T* qbase =
-      (const T*)a.q + (int64_t)q_lo * a.q_sn + (int64_t)kvh * a.G * a.q_sh;
-  const T* gbase =
-      (const T*)a.dout + (int64_t)q_lo * a.g_sn + (int64_t)kvh * a.G * a.g_sh;
+  const T* qbase = (const T*)a.q + (int64_t)kvh * a.G * a.q_sh;
+  const T* gbase = (const T*)a.dout + (int64_t)kvh * a.G * a.g_sh;
   float rv[4] = {INFINITY, 0.f, 0.f, 0.f};
-  auto fetch = [&](int t, int buf) {
+  auto fetch = [&](int q0, int e, int buf) {
     using S = Stager<T, QT, CH, NT>;
-    const int left = q_hi - q_lo - t * QW;
+    const int left = e - q0;
     DGMC_LDS char* qt = lds + buf * 2 * TB;
     const auto ok = [&](int r) { return r < RW && r / a.G < left; };
-    S::fill(qbase + (int64_t)t * QW * a.q_sn, a.D, a.vec_q, qt, ok,
+    S::fill(qbase + (int64_t)q0 * a.q_sn, a.D, a.vec_q, qt, ok,
             [&](int r) { return r / a.G * qsb + r % a.G * qhb; });
-    S::fill(gbase + (int64_t)t * QW * a.g_sn, a.D, a.vec_g, qt + TB, ok,
+    S::fill(gbase + (int64_t)q0 * a.g_sn, a.D, a.vec_g, qt + TB, ok,
             [&](int r) { return r / a.G * gsb + r % a.G * ghb; });
     if (tid < QT) {
-      const int64_t qi = (int64_t)q_lo + t * QW + tid / a.G;
-      const bool ok = tid < RW && qi < q_hi;
+      const int64_t qi = (int64_t)q0 + tid / a.G;
+      const bool ok = tid < RW && qi < e;
       const int64_t row = qi * a.H + kvh * a.G + tid % a.G;
       rv[0] = ok ? a.lse[row] : INFINITY;      // p = 0 in a row not there
       rv[1] = ok ? a.delta[row] : 0.f;
@@ -384,18 +403,27 @@ __global__
     }
   };
 
+  // Passes as in the forward.
+  for (int pass = b0 - 1;; ++pass) {
+  int p_lo = q_lo, p_hi = q_hi;
+  if (pass >= b0) {
+    seg_range(a.ptr_q, pass, a.B, a.Nq, p_lo, p_hi);
+    p_lo = max(p_lo, q_lo);
+    p_hi = min(p_hi, q_hi);
+    stage_barrier();
+  }
   f32x16 ak[DP / 32], av[DP / 32];
 #pragma unroll
   for (int k = 0; k < DP / 32; ++k)
 #pragma unroll
     for (int r = 0; r < 16; ++r) ak[k][r] = av[k][r] = 0.f;
 
-  if (t0 < t1) fetch(t0, 0);
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
+  if (p_lo < p_hi) fetch(p_lo, p_hi, 0);
+  for (int q0 = p_lo, buf = 0; q0 < p_hi; q0 += QW, buf ^= 1) {
     put_rows(buf);
     stage_barrier();
-    if (t + 1 < t1) fetch(t + 1, buf ^ 1);
+    if (q0 + QW < p_hi) fetch(q0 + QW, p_hi, buf ^ 1);
+    if (q0 >= l_hi || q0 + QW <= f_lo) continue;  // none of this wave's
     const DGMC_LDS char* qt = lds + buf * 2 * TB;
     const DGMC_LDS float* rw = rowv + buf * 4 * QT;
     f32x16 z, dp, th;
@@ -430,6 +458,15 @@ __global__
         dp[i] = z[i] * (dp[i] - de[r]);
       }
     }
+    if (q0 < l_lo || q0 + QW > f_hi) {
+      // Packed rows of other segments (selected, not multiplied away: they
+      // may hold NaN; rows from RW on have p = 0).
+      const unsigned n = (r_hi - r_lo) * a.G;
+      const int j0 = (q0 - r_lo) * a.G + 4 * h;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if ((unsigned)(j0 + 8 * (r >> 2) + (r & 3)) >= n) z[r] = dp[r] = 0.f;
+    }
     if (a.cap > 0.f) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] *= fmaf(-th[r], th[r], 1.f);
@@ -437,29 +474,34 @@ __global__
     Mma<T>::template accum<DP>(av, qt + TB, 0, z);
     Mma<T>::template accum<DP>(ak, qt, 0, dp);
   }
-  if (!live) return;
-  const int64_t row = kj * a.KV + kvh;
-  if (per < ntile) {            // joined by join_kernel
-    const int64_t rows = (int64_t)a.Nk * a.KV;
-    float* p = a.part_o + (split * rows + row) * a.D;
-    put_acc<DP>(p, ak, a.D, 1.f);
-    put_acc<DP>(p + a.splits * rows * a.D, av, a.D, 1.f);
-  } else {
-    put_acc<DP>((T*)a.dk + row * a.D, ak, a.D, a.scale);
-    put_acc<DP>((T*)a.dv + row * a.D, av, a.D, 1.f);
+  const bool redo = pass < b0 && b1 > b0 &&
+                    any_lane<NW>(live && (not_finite(ak) || not_finite(av)));
+  if (!redo && live && (pass < b0 || seg == pass)) {
+    const int64_t row = kj * a.KV + kvh;
+    if (per < ntile) {          // joined by join_kernel
+      const int64_t rows = (int64_t)a.Nk * a.KV;
+      float* p = a.part_o + (split * rows + row) * a.D;
+      put_acc<DP>(p, ak, a.D, 1.f);
+      put_acc<DP>(p + a.splits * rows * a.D, av, a.D, 1.f);
+    } else {
+      put_acc<DP>((T*)a.dk + row * a.D, ak, a.D, a.scale);
+      put_acc<DP>((T*)a.dv + row * a.D, av, a.D, 1.f);
+    }
+  }
+  if (pass < b0 ? !redo : pass == b1) return;
   }
 }
 
 template <typename T, int DP, int NW, int POS>
 void launch_dq(const Args& a, int nblk, hipStream_t st) {
-  const int TQ = 32 / a.G * NW, nslot = a.Nq / TQ + a.B + 1;
+  const int TQ = 32 / a.G * NW, ntiles = (a.Nq + TQ - 1) / TQ;
   const size_t sm = 4 * 32 * DP * sizeof(T) +
                     (POS ? 16 * 32 + a.G * kSlots * 4 +
                                (size_t)NW * a.slots * 256 : 0);
   auto kern = dq_kernel<T, DP, NW, POS>;
   allow_lds(reinterpret_cast<const void*>(kern), sm);
-  kern<<<dim3((POS ? nblk : nslot * a.splits) * a.KV), dim3(NW * 64), sm,
-         st>>>(a, nslot);
+  kern<<<dim3((POS ? nblk : ntiles * a.splits) * a.KV), dim3(NW * 64), sm,
+         st>>>(a, ntiles);
   DGMC_CHECK_LAUNCH();
 }
 
@@ -469,8 +511,8 @@ void launch_dkv(const Args& a, hipStream_t st) {
                     (POS ? a.G * kSlots * 4 : 0);
   auto kern = dkv_kernel<T, DP, NW, POS>;
   allow_lds(reinterpret_cast<const void*>(kern), sm);
-  kern<<<dim3((a.Nk / (32 * NW) + a.B + 1) * a.KV, a.splits), dim3(NW * 64),
-         sm, st>>>(a);
+  kern<<<dim3((a.Nk + 32 * NW - 1) / (32 * NW) * a.KV, a.splits),
+         dim3(NW * 64), sm, st>>>(a);
   DGMC_CHECK_LAUNCH();
 }
 

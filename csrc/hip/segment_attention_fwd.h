@@ -34,15 +34,18 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) v
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int h = lane >> 5, c = lane & 31;
-  const int kvh = blockIdx.x % a.KV, slot = blockIdx.x / a.KV;
-  const int split = blockIdx.y;
+  const int kvh = blockIdx.x % a.KV, split = blockIdx.y;
   const int QW = 32 / a.G, TQ = QW * NW;
-  const int seg = find_segment(a.ptr_q, a.B, a.Nq, TQ, slot);
-  int q_lo, q_hi, k_lo = 0, k_hi = 0;
-  seg_range(a.ptr_q, seg, a.B, a.Nq, q_lo, q_hi);
-  q_lo += (slot - (seg_begin(a.ptr_q, seg, a.Nq) / TQ + seg)) * TQ;
-  if (q_lo >= q_hi) return;
-  if (seg < a.B) seg_range(a.ptr_k, seg, a.B, a.Nk, k_lo, k_hi);
+  const int q_lo = blockIdx.x / a.KV * TQ, q_hi = min(q_lo + TQ, a.Nq);
+  int b0, b1, k_lo, k_hi;
+  tile_range(a.ptr_q, a.ptr_k, a.B, a.Nq, a.Nk, q_lo, q_hi, b0, b1, k_lo,
+             k_hi);
+  // The keys of this split.
+  const int ntile = (k_hi - k_lo + KT - 1) / KT;
+  const int per = split_tiles(a, ntile);
+  if (split > 0 && split * per >= ntile) return;
+  k_lo += split * per * KT;
+  k_hi = min(k_lo + per * KT, k_hi);
 
   // This lane's packed row.
   const int g = c % a.G;
@@ -68,31 +71,39 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) v
   const DGMC_LDS float* mytab = tab + g * kSlots;
   const int W = 2 * a.half + 2;
 
-  // Key tiles [t0, t1) of this split.
-  const int ntile = (k_hi - k_lo + KT - 1) / KT;
-  const int per = split_tiles(a, ntile);
-  const int t0 = split * per, t1 = min(t0 + per, ntile);
-  if (split > 0 && t0 >= t1) return;
+  // The row's own keys; the wave's first and last row bound them all.
+  const int w0 = q_lo + wave * QW;
+  const int wrows = min(QW, q_hi - w0);
+  int r_lo = 0, r_hi = 0, f_lo = 0, f_hi = 0, l_lo = 0, l_hi = 0;
+  int seg = -1;
+  if (wrows > 0) {
+    seg = lane_segment(a.ptr_q, a.B, a.Nq,
+                       segment_of(a.ptr_q, a.B, a.Nq, w0),
+                       min((int)qi, q_hi - 1));
+    seg_range(a.ptr_k, seg, a.B, a.Nk, r_lo, r_hi);
+    const int last = (wrows - 1) * a.G;
+    f_lo = lane_int(r_lo, 0), f_hi = lane_int(r_hi, 0);
+    l_lo = lane_int(r_lo, last), l_hi = lane_int(r_hi, last);
+  }
 
-  const T* kbase =
-      (const T*)a.k + (int64_t)k_lo * a.k_sn + (int64_t)kvh * a.k_sh;
-  const T* vbase =
-      (const T*)a.v + (int64_t)k_lo * a.v_sn + (int64_t)kvh * a.v_sh;
+  const T* kbase = (const T*)a.k + (int64_t)kvh * a.k_sh;
+  const T* vbase = (const T*)a.v + (int64_t)kvh * a.v_sh;
   const int64_t ksb = a.k_sn * (int)sizeof(T), vsb = a.v_sn * (int)sizeof(T);
   float pr[2] = {0.f, 0.f};
-  // Start tile t's loads into buffer `buf`; its positions wait in registers.
-  auto fetch = [&](int t, int buf) {
+  // Start the loads of keys [k0, e) into buffer `buf`; their positions wait
+  // in registers.
+  auto fetch = [&](int k0, int e, int buf) {
     using S = Stager<T, KT, CH, NT>;
-    const int left = k_hi - k_lo - t * KT;
+    const int left = e - k0;
     DGMC_LDS char* kt = lds + buf * 2 * TB;
     const auto ok = [&](int r) { return r < left; };
-    S::fill(kbase + (int64_t)t * KT * a.k_sn, a.D, a.vec_k, kt, ok,
+    S::fill(kbase + (int64_t)k0 * a.k_sn, a.D, a.vec_k, kt, ok,
             [&](int r) { return r * ksb; });
-    S::fill(vbase + (int64_t)t * KT * a.v_sn, a.D, a.vec_v, kt + TB, ok,
+    S::fill(vbase + (int64_t)k0 * a.v_sn, a.D, a.vec_v, kt + TB, ok,
             [&](int r) { return r * vsb; });
     if constexpr (POS > 0) {
       if (tid < KT && tid < left) {
-        const int64_t j = (int64_t)k_lo + t * KT + tid;
+        const int64_t j = (int64_t)k0 + tid;
         pr[0] = load_pos(a.pos_k, j, POS, 0);
         if (POS == 2) pr[1] = load_pos(a.pos_k, j, POS, 1);
       }
@@ -107,24 +118,34 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) v
     }
   };
 
-  f32x16 acc[DP / 32];
-#pragma unroll
-  for (int k = 0; k < DP / 32; ++k)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[k][r] = 0.f;
-  float m = -INFINITY, l = 0.f;
   const float s1 = a.cap > 0.f ? a.scale / a.cap : a.scale * kLog2e;
   const float s2 = a.cap * kLog2e;
   // Plain scores stay unscaled: 2^(s1 z - m) is one fma and one exp2.
   const bool plain = POS == 0 && a.cap <= 0.f && s1 > 0.f;
   const float ex = plain ? s1 : 1.f;
 
-  if (t0 < t1) fetch(t0, 0);
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
+  // Pass b0 - 1: all rows over all keys of the tile; passes b0 .. b1 (only
+  // after a non-finite result): segment by segment.
+  for (int pass = b0 - 1;; ++pass) {
+  int p_lo = k_lo, p_hi = k_hi;
+  if (pass >= b0) {
+    seg_range(a.ptr_k, pass, a.B, a.Nk, p_lo, p_hi);
+    p_lo = max(p_lo, k_lo);
+    p_hi = min(p_hi, k_hi);
+    stage_barrier();
+  }
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[k][r] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  if (p_lo < p_hi) fetch(p_lo, p_hi, 0);
+  for (int k0 = p_lo, buf = 0; k0 < p_hi; k0 += KT, buf ^= 1) {
     put_pos(buf);
     stage_barrier();
-    if (t + 1 < t1) fetch(t + 1, buf ^ 1);
+    if (k0 + KT < p_hi) fetch(k0 + KT, p_hi, buf ^ 1);
+    if (k0 >= l_hi || k0 + KT <= f_lo) continue;    // none of this wave's
     const DGMC_LDS char* kt = lds + buf * 2 * TB;
     f32x16 z[KT / 32];
 #pragma unroll
@@ -168,13 +189,14 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) v
         }
       }
     }
-    const int left = k_hi - (k_lo + t * KT);
-    if (left < KT) {
+    if (k0 < l_lo || k0 + KT > f_hi) {
+      const unsigned n = r_hi - r_lo;
+      const int j0 = k0 + 4 * h - r_lo;
 #pragma unroll
       for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (32 * u + 8 * (r >> 2) + 4 * h + (r & 3) >= left)
+          if ((unsigned)(j0 + 32 * u + 8 * (r >> 2) + (r & 3)) >= n)
             z[u][r] = -INFINITY;
     }
     float mt = z[0][0];
@@ -207,44 +229,42 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) v
     }
   }
   l = sum_half(l);
-  if (!live) return;
+  const bool redo =
+      pass < b0 && b1 > b0 && any_lane<NW>(live && not_finite(acc));
   const int64_t row = qi * a.H + head;
-  if (per < ntile) {            // joined by join_kernel
-    const int64_t prow = (int64_t)split * a.Nq * a.H + row;
-    if (h == 0) {
-      a.part_ml[prow * 2] = m;
-      a.part_ml[prow * 2 + 1] = l;
-    }
-    float* po = a.part_o + prow * a.D;
-#pragma unroll
-    for (int k = 0; k < DP / 32; ++k)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int d = 32 * k + 8 * (r >> 2) + 4 * h + (r & 3);
-        if (d < a.D) po[d] = acc[k][r];
+  if (!redo && live && (pass < b0 || seg == pass)) {
+    if (per < ntile) {          // joined by join_kernel
+      const int64_t prow = (int64_t)split * a.Nq * a.H + row;
+      if (h == 0) {
+        a.part_ml[prow * 2] = m;
+        a.part_ml[prow * 2 + 1] = l;
       }
-    return;
+      put_acc<DP>(a.part_o + prow * a.D, acc, a.D, 1.f);
+    } else {
+      // l is 0 only without a key of finite score: such a row is 0.
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      if (h == 0 && a.lse) a.lse[row] = l == 0.f ? INFINITY : m + log2f(l);
+      T* orow = (T*)a.out + row * a.D;
+#pragma unroll
+      for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int d = 32 * k + 8 * r4 + 4 * h;
+          T o[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[r] = (T)(acc[k][4 * r4 + r] * inv);
+          put4(orow, d, a.D, o);
+          if constexpr (FINE) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              o[r] = (T)(acc[k][4 * r4 + r] * inv - (float)o[r]);
+            put4((T*)a.out_lo + row * a.D, d, a.D, o);
+          }
+        }
+    }
   }
-  // l is 0 only without a key of finite score: such a row is 0.
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (h == 0 && a.lse) a.lse[row] = l == 0.f ? INFINITY : m + log2f(l);
-  T* orow = (T*)a.out + row * a.D;
-#pragma unroll
-  for (int k = 0; k < DP / 32; ++k)
-#pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      const int d = 32 * k + 8 * r4 + 4 * h;
-      T o[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) o[r] = (T)(acc[k][4 * r4 + r] * inv);
-      put4(orow, d, a.D, o);
-      if constexpr (FINE) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          o[r] = (T)(acc[k][4 * r4 + r] * inv - (float)o[r]);
-        put4((T*)a.out_lo + row * a.D, d, a.D, o);
-      }
-    }
+  if (pass < b0 ? !redo : pass == b1) return;
+  }
 }
 
 template <typename T, int DP, int NW, bool FINE>
@@ -252,7 +272,7 @@ void launch_fwd(const Args& a, int axes, hipStream_t st) {
   constexpr int KT =                // (fwd_keys)
       (NW > 1 && DP * (int)sizeof(T) <= 256) ? 64 : 32;
   const int TQ = 32 / a.G * NW;
-  const dim3 grid((a.Nq / TQ + a.B + 1) * a.KV, a.splits), blk(NW * 64);
+  const dim3 grid((a.Nq + TQ - 1) / TQ * a.KV, a.splits), blk(NW * 64);
   const size_t sm = 4 * KT * DP * sizeof(T) +
                     (axes ? 16 * KT + a.G * kSlots * 4 : 0);
   auto kern = axes == 0   ? fwd_kernel<T, DP, NW, KT, 0, FINE>

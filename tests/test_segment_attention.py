@@ -532,3 +532,46 @@ def test_second_derivatives_are_refused():
                              create_graph=True)
     with pytest.raises(RuntimeError, match='differentiated again'):
         g.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('axes,cap', [(0, 0.0), (1, 2.0)])
+@pytest.mark.parametrize('what', ['q', 'k', 'v', 'do'])
+def test_non_finite_segments_stay_alone(dtype, axes, cap, what):
+    """NaN and inf in some segments' rows never reach the segments that
+    share tiles with them (rows and keys of a tile are consecutive rows,
+    whatever their segments)."""
+    lens = [5, 7, 0, 40, 3, 60, 1, 1, 150]
+    st = _case(lens, [9, 4, 3, 30, 0, 80, 2, 1, 90], 2, 1, 32, dtype,
+               axes=axes, half=2, tail=4)
+    val, tol = _plain(st, cap=cap, half=2)
+    pq, pk = st['ptr_q'].tolist(), st['ptr_k'].tolist()
+    own = pq if what in ('q', 'do') else pk
+    st[what][own[1] + 1] = float('nan')
+    st[what][own[5]:own[5] + 40] = math.inf
+    got = _run(st, 'cuda', cap=cap)
+    for n, t in got.items():
+        if n == 'dbias':        # the bad rows' own contribution
+            continue
+        ptr = pq if n in ('out', 'dq') else pk
+        for b in range(len(lens)):
+            rows = slice(ptr[b], ptr[b + 1])
+            if b in (1, 5):
+                continue
+            err = (t[rows].double() - val[n][rows]).abs()
+            assert (err <= tol[n][rows] + 1e-30).all(), (n, b)
+    bad = {'q': ('out', 'dq', 'dk'), 'k': ('out', 'dq', 'dk'),
+           'v': ('out', 'dq', 'dk'), 'do': ('dq', 'dk', 'dv')}[what]
+    for n in bad:
+        ptr = pq if n in ('out', 'dq') else pk
+        assert not torch.isfinite(got[n][ptr[1]:ptr[2]]).all(), n
+
+
+@pytest.mark.gpu
+def test_many_empty_segments_between_rows():
+    """More boundaries than lanes between two rows of a tile."""
+    lens = [3] + [0] * 200 + [2] + [0] * 70 + [5, 0, 0, 1] + [0] * 64 + [4]
+    st = _case(lens, None, 2, 2, 32, torch.float32)
+    val, tol = _plain(st)
+    _close(_run(st, 'cuda'), val, tol)
