@@ -52,6 +52,7 @@ namespace segattn {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
@@ -73,7 +74,7 @@ struct Args {
   const float* bias;                  // [H, nb]
   const int *pos_q, *pos_k;           // [N, axes]
   int64_t q_sn, q_sh, k_sn, k_sh, v_sn, v_sh, o_sn, o_sh, g_sn, g_sh;
-  int B, Nq, Nk, H, KV, G, D, nb, half, mbits, slots;
+  int B, Nq, Nk, H, KV, G, gmul, D, nb, half, mbits, slots;
   float scale, cap, dmax, dmul;
   int vec_q, vec_k, vec_v, vec_o, vec_g;   // 16-byte rows
   int splits, chunk;                  // most splits, least tiles of one
@@ -134,20 +135,63 @@ __device__ __forceinline__ void seg_range(const int* ptr, int seg, int B,
   hi = b < B ? min(max(ptr[b + 1], lo), N) : lo;
 }
 
-// Segments [b0, b1] of a tile of own rows [r0, r1), and the other side's
-// rows [lo, hi) that it visits.
-__device__ __forceinline__ void tile_range(const int* own, const int* other,
-                                           int B, int N, int No, int r0,
-                                           int r1, int& b0, int& b1, int& lo,
-                                           int& hi) {
-  b0 = segment_of(own, B, N, r0);
-  b1 = segment_of(own, B, N, r1 - 1);
-  int x;
-  seg_range(other, b0, B, No, lo, x);
-  seg_range(other, b1, B, No, x, hi);
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  hi = max(__builtin_amdgcn_readfirstlane(hi), lo);
-}
+// What a wave knows of its tile's own rows [t_lo, t_hi) and the other side's:
+// the segments [b0, b1] and other rows [lo, hi) of the whole tile, the lane's
+// own segment and range [r_lo, r_hi), and the ranges of the wave's first and
+// last row (ranges ascend with the rows, so these bound all of them).
+struct Rows {
+  int b0, b1, lo, hi;
+  int seg, r_lo, r_hi, f_lo, f_hi, l_lo, l_hi;
+
+  // `row`: the lane's row (clamped into the tile); `last`: the lane of the
+  // wave's last row, -1 for a wave without rows.
+  template <int NW>
+  __device__ __forceinline__ static Rows find(const int* own, const int* other,
+                                              int B, int N, int No, int t_lo,
+                                              int t_hi, int row, int last) {
+    Rows w;
+    w.b0 = segment_of(own, B, N, t_lo);
+    w.seg = lane_segment(own, B, N, w.b0, min(row, t_hi - 1));
+    const int l = max(last, 0);
+    w.b1 = NW == 1 ? __builtin_amdgcn_readlane(w.seg, l)
+                   : __builtin_amdgcn_readfirstlane(
+                         lane_segment(own, B, N, w.b0, t_hi - 1));
+    int x = 0, y = 0, z = 0;
+    if (NW > 1) {
+      seg_range(other, w.b0, B, No, x, z);
+      seg_range(other, w.b1, B, No, z, y);
+    }
+    seg_range(other, w.seg, B, No, w.r_lo, w.r_hi);
+    w.f_lo = __builtin_amdgcn_readlane(w.r_lo, 0);
+    w.f_hi = __builtin_amdgcn_readlane(w.r_hi, 0);
+    w.l_lo = __builtin_amdgcn_readlane(w.r_lo, l);
+    w.l_hi = __builtin_amdgcn_readlane(w.r_hi, l);
+    w.lo = NW == 1 ? w.f_lo : __builtin_amdgcn_readfirstlane(x);
+    w.hi = max(NW == 1 ? w.l_hi : __builtin_amdgcn_readfirstlane(y), w.lo);
+    if (last < 0) w.seg = -1, w.f_lo = w.l_hi = 0;   // (skips every tile)
+    return w;
+  }
+  // No row of the wave reaches other rows [x, x + n).
+  __device__ __forceinline__ bool skip(int x, int n) const {
+    return x >= l_hi || x + n <= f_lo;
+  }
+  // Every row of the wave takes all of them.
+  __device__ __forceinline__ bool whole(int x, int n) const {
+    return x >= l_lo && x + n <= f_hi;
+  }
+  // Pass `pass` of a tile cut to [s_lo, s_hi): all of it (pass < b0) or the
+  // segment's own part.
+  __device__ __forceinline__ void pass_range(const int* other, int B, int No,
+                                             int pass, int s_lo, int s_hi,
+                                             int& p_lo, int& p_hi) const {
+    p_lo = s_lo;
+    p_hi = s_hi;
+    if (pass < b0) return;
+    seg_range(other, pass, B, No, p_lo, p_hi);
+    p_lo = max(p_lo, s_lo);
+    p_hi = min(p_hi, s_hi);
+  }
+};
 
 // Whether an accumulator of this lane is not finite.
 template <int M>
@@ -167,27 +211,60 @@ __device__ __forceinline__ bool any_lane(bool v) {
   else return __syncthreads_or(v);
 }
 
-// Lane value of a wave-uniform lane number.
-__device__ __forceinline__ int lane_int(int v, int lane) {
-  return __builtin_amdgcn_readlane(v, lane);
+// A value the compiler cannot see through: what is computed from it inside a
+// loop stays there and holds no register across it.
+__device__ __forceinline__ int opaque(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+// A lane's LDS address in this buffer: one register and an xor a read where
+// rows are long (registers are short there), all of them kept otherwise.
+template <int CH>
+__device__ __forceinline__ int lane_base(int v) {
+  return CH > 8 ? opaque(v) : v;
 }
 
 // 16-byte chunk swizzle of an LDS tile row with CH chunks: both 16-byte
 // column reads over 16 rows and transposing reads of 4 rows spread over all
-// banks.
+// banks.  Linear over xor of row numbers without common bits, so a lane's
+// address is its own base xor a constant, plus a constant.
 template <int CH>
-__device__ __forceinline__ int swz(int row) {
+__host__ __device__ constexpr int swz(int row) {
   if constexpr (CH >= 16) return ((row & 3) << 2) | ((row >> 2) & 3);
   else if constexpr (CH == 8)
     return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
   else return (row >> 2) & 3;
 }
 
-__device__ __forceinline__ float max_half(float v) {   // over lanes l, l ^ 32
-  return fmaxf(v, __shfl_xor(v, 32));
+template <int CH>
+__host__ __device__ constexpr int swz_xor(int row, int chunk) {
+  return (swz<CH>(row) ^ chunk) * 16;
+}
+
+// x / G and x % G for x < 32 (gmul = ceil(1024 / G): the excess stays under
+// 1 / 32, below the next multiple).
+__device__ __forceinline__ int div_group(const Args& a, int x) {
+  return (x * a.gmul) >> 10;
+}
+
+// v of lanes l and l ^ 32 (one VALU swap of the halves; the two results as
+// scalars before the casts: a bit cast of a vector's element took element 0).
+__device__ __forceinline__ void halves(float v, float& a, float& b) {
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const unsigned x = r[0], y = r[1];
+  a = __builtin_bit_cast(float, x);
+  b = __builtin_bit_cast(float, y);
+}
+__device__ __forceinline__ float max_half(float v) {
+  float a, b;
+  halves(v, a, b);
+  return fmaxf(a, b);
 }
 __device__ __forceinline__ float sum_half(float v) {
-  return v + __shfl_xor(v, 32);
+  float a, b;
+  halves(v, a, b);
+  return a + b;
 }
 __device__ __forceinline__ float exp2_(float x) {
   return __builtin_amdgcn_exp2f(x);
@@ -226,27 +303,23 @@ struct Stager {
   static constexpr int N = (ROWS * CH + NT - 1) / NT;
   static constexpr bool kFull = N * NT == ROWS * CH;
 
-  // Slot i of thread `tid`: its row and (global) chunk.
-  __device__ __forceinline__ static int row(int tid, int i) {
-    return (tid + i * NT) / CH;
-  }
-  __device__ __forceinline__ static int chunk(int tid, int i) {
-    return ((tid + i * NT) % CH) ^ swz<CH>(row(tid, i));
-  }
   // `ok(row)`: the row is there, at `off(row)` bytes from `base` (below 2^31
   // where vec is set).
   template <typename Ok, typename Off>
   __device__ __forceinline__ static void fill(const T* base, int D, int vec,
                                               DGMC_LDS char* tile, Ok ok,
                                               Off off) {
-    const int wave = threadIdx.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (vec) {
+      // (a wave's many slots are computed anew every tile, a few are kept)
+      const int tid = N > 2 ? opaque(threadIdx.x) : threadIdx.x;
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<T*>(base), 0, 0x80000000u, 0x00020000);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         if (!kFull && i * NT + wave * 64 >= ROWS * CH) continue;
-        const int ch = chunk(threadIdx.x, i), r = row(threadIdx.x, i);
+        const int r = (tid + i * NT) / CH;
+        const int ch = ((tid + i * NT) % CH) ^ swz<CH>(r);
         const unsigned o =
             ok(r) && ch * E < D ? (unsigned)off(r) + ch * 16 : kNoRow;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
@@ -254,13 +327,12 @@ struct Stager {
             0, 0);
       }
     } else {
-      // (opaque: nothing of this path is kept in registers over the loop)
-      int tid = threadIdx.x;
-      asm volatile("" : "+v"(tid));
+      const int tid = opaque(threadIdx.x);
 #pragma unroll 1
       for (int i = 0; i < N; ++i) {
         if (!kFull && tid + i * NT >= ROWS * CH) continue;
-        const int ch = chunk(tid, i), r = row(tid, i);
+        const int r = (tid + i * NT) / CH;
+        const int ch = ((tid + i * NT) % CH) ^ swz<CH>(r);
         const u32x4 v = load_chunk<T>(
             (const T*)((const char*)base + off(r)), ch, D, ok(r), 0);
         *(DGMC_LDS u32x4*)(tile + (tid + i * NT) * 16) = v;
@@ -303,27 +375,32 @@ __device__ __forceinline__ void stage_barrier() {
 }
 
 // --------------------------------------------------------------------------
-// Matrix core policies
+// Matrix core policies.  `rows` and `cols` are a lane's byte offsets into a
+// staged tile for the two ways it is read: row operand (16-byte chunks of
+// row c) and transposed operand of accum().
 // --------------------------------------------------------------------------
 template <typename T> struct Mma;
 
 template <> struct Mma<__bf16> {
+  template <int CH> __device__ __forceinline__ static int cols() {
+    const int lane = threadIdx.x & 63;
+    const int row = 4 * (lane >> 5) + ((lane >> 2) & 3);
+    const int ch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    return row * CH * 16 + ((ch ^ swz<CH>(row)) * 16) + 8 * (lane & 1);
+  }
   // acc += A B for one pair of 16-byte chunks (K = 16).
   __device__ __forceinline__ static f32x16 dot(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
         __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
         0);
   }
-  // acc[blk] += tile^T p: rows of `tile` (32 from row0) are the K index, in
-  // the accumulator's row order.  FINE: p as the sum of two bf16 terms.
+  // acc[blk] += tile^T p: 32 rows of the tile are the K index, in the
+  // accumulator's row order.  FINE: p as the sum of two bf16 terms.
   template <int DP, bool FINE = false>
   __device__ __forceinline__ static void accum(f32x16 (&acc)[DP / 32],
                                                const DGMC_LDS char* tile,
-                                               int row0, f32x16 p) {
+                                               int cols, f32x16 p) {
     constexpr int CH = DP / 8;
-    const int lane = threadIdx.x & 63;
-    const int h = lane >> 5, ds = (lane >> 4) & 1, q = (lane >> 2) & 3,
-              pp = lane & 3;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       bf16x8 b, lo_b;
@@ -334,18 +411,18 @@ template <> struct Mma<__bf16> {
         for (int i = 0; i < 8; ++i)
           lo_b[i] = (__bf16)(p[8 * c + i] - (float)b[i]);
       }
-      const int r0 = row0 + 16 * c + 4 * h + q, r1 = r0 + 8;
 #pragma unroll
       for (int k = 0; k < DP / 32; ++k) {
-        const int ch = 4 * k + 2 * ds + (pp >> 1);
-        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (DGMC_LDS i16x4*)(tile + (r0 * CH + (ch ^ swz<CH>(r0))) * 16 +
-                              8 * (pp & 1)));
-        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (DGMC_LDS i16x4*)(tile + (r1 * CH + (ch ^ swz<CH>(r1))) * 16 +
-                              8 * (pp & 1)));
-        const i16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5,
-                                                   6, 7);
+        i16x4 v[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = 16 * c + 8 * i;
+          v[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (DGMC_LDS i16x4*)(tile + (cols ^ swz_xor<CH>(row, 4 * k)) +
+                                row * CH * 16));
+        }
+        const i16x8 both = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4,
+                                                   5, 6, 7);
         acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
             __builtin_bit_cast(bf16x8, both), b, acc[k], 0, 0, 0);
         if constexpr (FINE)
@@ -353,6 +430,26 @@ template <> struct Mma<__bf16> {
               __builtin_bit_cast(bf16x8, both), lo_b, acc[k], 0, 0, 0);
       }
     }
+  }
+  // l + the sum of p as the product takes it: rounded, two a v_dot2 (FINE:
+  // the fp32 values).
+  template <bool FINE>
+  __device__ __forceinline__ static float sum(f32x16 p, float l) {
+    float s[2] = {l, 0.f};
+    if constexpr (FINE) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r & 1] += p[r];
+    } else {
+      const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const bf16x2 v = {(__bf16)p[r], (__bf16)p[r + 1]};
+        s[(r >> 1) & 1] = __builtin_amdgcn_fdot2_f32_bf16(v, one,
+                                                          s[(r >> 1) & 1],
+                                                          false);
+      }
+    }
+    return s[0] + s[1];
   }
   __device__ __forceinline__ static float chunk_dot(u32x4 a, u32x4 b) {
     const bf16x8 x = __builtin_bit_cast(bf16x8, a),
@@ -365,6 +462,10 @@ template <> struct Mma<__bf16> {
 };
 
 template <> struct Mma<float> {
+  template <int CH> __device__ __forceinline__ static int cols() {
+    const int lane = threadIdx.x & 63, row = 4 * (lane >> 5), d = lane & 31;
+    return row * CH * 16 + (((d >> 2) ^ swz<CH>(row)) * 16) + 4 * (d & 3);
+  }
   __device__ __forceinline__ static f32x16 dot(u32x4 a, u32x4 b, f32x16 c) {
     const f32x4 x = __builtin_bit_cast(f32x4, a),
                 y = __builtin_bit_cast(f32x4, b);
@@ -376,21 +477,26 @@ template <> struct Mma<float> {
   template <int DP, bool FINE = false>
   __device__ __forceinline__ static void accum(f32x16 (&acc)[DP / 32],
                                                const DGMC_LDS char* tile,
-                                               int row0, f32x16 p) {
+                                               int cols, f32x16 p) {
     constexpr int CH = DP / 4;
-    const int lane = threadIdx.x & 63, h = lane >> 5, d = lane & 31;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int row = row0 + 8 * (r >> 2) + 4 * h + (r & 3);
+      const int row = 8 * (r >> 2) + (r & 3);
 #pragma unroll
       for (int k = 0; k < DP / 32; ++k) {
-        const int ch = 8 * k + (d >> 2);
         const float a = *(const DGMC_LDS float*)(
-            tile + (row * CH + (ch ^ swz<CH>(row))) * 16 + 4 * (d & 3));
+            tile + (cols ^ swz_xor<CH>(row, 8 * k)) + row * CH * 16);
         acc[k] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[k], 0, 0,
                                                       0);
       }
     }
+  }
+  template <bool FINE>
+  __device__ __forceinline__ static float sum(f32x16 p, float l) {
+    float s[4] = {l, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r & 3] += p[r];
+    return (s[0] + s[1]) + (s[2] + s[3]);
   }
   __device__ __forceinline__ static float chunk_dot(u32x4 a, u32x4 b) {
     const f32x4 x = __builtin_bit_cast(f32x4, a),
@@ -398,6 +504,24 @@ template <> struct Mma<float> {
     return (x[0] * y[0] + x[1] * y[1]) + (x[2] * y[2] + x[3] * y[3]);
   }
 };
+
+// Row operand: chunks h, h + 2, .. of row c of a staged block of 32 rows.
+template <int CH>
+__device__ __forceinline__ int row_base() {
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  return c * CH * 16 + ((h ^ swz<CH>(c)) * 16);
+}
+template <typename T, int CH>
+__device__ __forceinline__ f32x16 row_dot(const DGMC_LDS char* tile, int rows,
+                                          const u32x4 (&f)[CH / 2]) {
+  f32x16 acc = Mma<T>::dot(*(const DGMC_LDS u32x4*)(tile + rows), f[0],
+                           f32x16{});
+#pragma unroll
+  for (int s = 1; s < CH / 2; ++s)
+    acc = Mma<T>::dot(*(const DGMC_LDS u32x4*)(tile + (rows ^ (32 * s))),
+                      f[s], acc);
+  return acc;
+}
 
 // Four values of an output row of D at d (d % 4 == 0).
 template <typename T>
@@ -427,14 +551,6 @@ __device__ __forceinline__ void put_acc(T* row, const f32x16 (&acc)[DP / 32],
       for (int r = 0; r < 4; ++r) o[r] = (T)(acc[k][4 * r4 + r] * scale);
       put4(row, 32 * k + 8 * r4 + 4 * h, D, o);
     }
-}
-
-// Chunk (row, ch) of a swizzled LDS tile.
-template <int CH>
-__device__ __forceinline__ u32x4 lds_chunk(const DGMC_LDS char* tile, int row,
-                                           int ch) {
-  return *(const DGMC_LDS u32x4*)(tile + (row * CH + (ch ^ swz<CH>(row))) *
-                                             16);
 }
 
 // --------------------------------------------------------------------------

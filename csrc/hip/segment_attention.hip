@@ -15,7 +15,7 @@ void dq_f32(const Args& a, int axes, int nw, int nblk, hipStream_t st);
 void dkv_bf16(const Args& a, int axes, int nw, hipStream_t st);
 void dkv_f32(const Args& a, int axes, int nw, hipStream_t st);
 
-constexpr int kMaxSplits = 64;
+constexpr int kMaxSplits = 512;
 
 // Join of the split rows (FWD: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M)
 // l_s; DQ, DKV: plain sums), in order of the splits.  A workgroup takes the
@@ -26,18 +26,16 @@ enum { FWD, DQ, DKV };
 
 template <typename T, int MODE>
 __global__ __launch_bounds__(256) void join_kernel(const Args a, int per_tile,
-                                                   int key_tile) {
+                                                   int key_tile, int ways) {
   __shared__ float red[256][9];
   __shared__ float wsum[16];
-  __shared__ float2 ml[16][kMaxSplits];
   const int kvh = blockIdx.x % a.KV;
   const int* own = MODE == DKV ? a.ptr_k : a.ptr_q;
   const int* other = MODE == DKV ? a.ptr_q : a.ptr_k;
   const int N = MODE == DKV ? a.Nk : a.Nq, No = MODE == DKV ? a.Nq : a.Nk;
   const int lo = blockIdx.x / a.KV * per_tile, hi = min(lo + per_tile, N);
-  int b0, b1, o_lo, o_hi;
-  tile_range(own, other, a.B, N, No, lo, hi, b0, b1, o_lo, o_hi);
-  const int ntile = (o_hi - o_lo + key_tile - 1) / key_tile;
+  const Rows w = Rows::find<4>(own, other, a.B, N, No, lo, hi, lo, 0);
+  const int ntile = (w.hi - w.lo + key_tile - 1) / key_tile;
   const int per = split_tiles(a, ntile);
   if (per >= ntile) return;
   const int ns = (ntile + per - 1) / per;
@@ -47,8 +45,6 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int per_tile,
   const int64_t all = (int64_t)N * heads;
   const int grp = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
   // `ways` (a power of two) groups share a row; 16 / ways rows a round.
-  int ways = 1;
-  while (ways < 16 && 2 * ways * rows <= 16 && ways < ns) ways *= 2;
   const int rpr = 16 / ways, rr = grp / ways, way = grp % ways;
   const float* part =
       a.part_o + (MODE == DKV ? blockIdx.y * a.splits * all * a.D : 0);
@@ -60,30 +56,23 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int per_tile,
     float M = -INFINITY, L = 0.f, o[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) o[k] = 0.f;
-    if (MODE == FWD) {
-      // The round's maxima and sums, all loads at once.
-      __syncthreads();
-      for (int e = threadIdx.x; e < rpr * ns; e += 256) {
-        const int q = e / ns, s = e - q * ns;
-        if (r0 + q < rows) {
-          const int64_t w = (int64_t)(lo + (r0 + q) / G) * heads + kvh * G +
-                            (r0 + q) % G;
-          ml[q][s] = *(const float2*)(a.part_ml + (s * all + w) * 2);
-        }
-      }
-      __syncthreads();
-    }
     if (live) {
+      const float* ml = a.part_ml + row * 2;
       if (MODE == FWD) {
-        for (int s = 0; s < ns; ++s) M = fmaxf(M, ml[rr][s].x);
+#pragma unroll 4
+        for (int s = threadIdx.x & 15; s < ns; s += 16)
+          M = fmaxf(M, ml[s * all * 2]);
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
         if (M == -INFINITY) M = 0.f;
       }
 #pragma unroll 4
       for (int s = way; s < ns; s += ways) {
-        float w = 1.f;
+        float wt = 1.f;
         if (MODE == FWD) {
-          w = exp2_(ml[rr][s].x - M);
-          L += w * ml[rr][s].y;
+          const float2 x = *(const float2*)(ml + s * all * 2);
+          wt = exp2_(x.x - M);
+          L += wt * x.y;
         }
         const float* p = part + (s * all + row) * a.D;
         if (a.D % 4 == 0 && d0 + 8 <= a.D) {
@@ -91,13 +80,13 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int per_tile,
                       y = *(const f32x4*)(p + d0 + 4);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            o[k] += w * x[k];
-            o[4 + k] += w * y[k];
+            o[k] += wt * x[k];
+            o[4 + k] += wt * y[k];
           }
         } else {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            if (d0 + k < a.D) o[k] += w * p[d0 + k];
+            if (d0 + k < a.D) o[k] += wt * p[d0 + k];
         }
       }
     }
@@ -107,10 +96,10 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int per_tile,
       if ((threadIdx.x & 15) == 0) wsum[grp] = L;
       __syncthreads();
       if (way == 0) {
-        for (int w = 1; w < ways; ++w) {
+        for (int k2 = 1; k2 < ways; ++k2) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) o[k] += red[threadIdx.x + 16 * w][k];
-          L += wsum[grp + w];
+          for (int k = 0; k < 8; ++k) o[k] += red[threadIdx.x + 16 * k2][k];
+          L += wsum[grp + k2];
         }
       }
       __syncthreads();
@@ -139,16 +128,18 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int per_tile,
 template <int MODE>
 static void join(const Args& a, bool f32, int per_tile, int key_tile) {
   const int N = MODE == DKV ? a.Nk : a.Nq;
-  // (workgroups along z share a tile's rows, 16 a round)
   const int G = MODE == DKV ? 1 : a.G;
+  int ways = 1;                     // at most four splits of a row a group
+  while (ways < 16 && 4 * ways < a.splits) ways *= 2;
+  // (workgroups along z share a tile's rows, 16 / ways a round)
   const dim3 grid((N + per_tile - 1) / per_tile * a.KV, MODE == DKV ? 2 : 1,
-                  (per_tile * G + 15) / 16);
+                  std::min((per_tile * G * ways + 15) / 16, 128));
   if (f32)
     join_kernel<float, MODE><<<grid, 256, 0, stream()>>>(a, per_tile,
-                                                         key_tile);
+                                                         key_tile, ways);
   else
     join_kernel<__bf16, MODE><<<grid, 256, 0, stream()>>>(a, per_tile,
-                                                          key_tile);
+                                                          key_tile, ways);
   DGMC_CHECK_LAUNCH();
 }
 
@@ -245,6 +236,7 @@ static Args make_args(const at::Tensor& q, const at::Tensor& k,
   a.v_sn = v.stride(0); a.v_sh = v.stride(1);
   a.B = (int)ptr_q.size(0) - 1;
   a.H = (int)q.size(1); a.KV = (int)k.size(1); a.G = a.H / a.KV;
+  a.gmul = (1024 + a.G - 1) / a.G;
   a.D = (int)q.size(2);
   // 32-bit row numbers and launch sizes (threads of a launch < 2^32).
   const int64_t lim = (int64_t)1 << 31;

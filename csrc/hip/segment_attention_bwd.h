@@ -23,66 +23,34 @@
 namespace dgmc {
 namespace segattn {
 
-// Scores of one 32 x 32 block in log2 units, from the raw products; `t`
-// receives tanh where the scores are capped.
-template <bool EXACT>
-__device__ __forceinline__ void cap_scores(const Args& a, f32x16& z,
-                                           f32x16& t) {
-  if (a.cap > 0.f) {
-    const float s1 = a.scale / a.cap, s2 = a.cap * kLog2e;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      t[r] = tanh_<EXACT>(z[r] * s1);
-      z[r] = s2 * t[r];
-    }
-  } else {
-    const float s1 = a.scale * kLog2e;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) z[r] *= s1;
-  }
-}
-
-// hist[sl[r]] += v[r] in a lane's own LDS column, in order.  A plain read,
-// add, write: ds_add_f32 took 120 cycles and more a wave (ragged case: 552
-// us, without the table 139 us).  Four at a time: equal slots among the four
-// take the earlier ones' values along and the last write counts.  RUNS: all
-// 16 in one slot (nodes in order, far apart) are added first.
-template <bool RUNS>
+// hist[sl[r]] += v[r] in a lane's own LDS column, four at a time and in
+// order.  A plain read, add, write: ds_add_f32 took 120 cycles and more a
+// wave (ragged case: 552 us, without the table 139 us).  Equal slots among
+// the four take the earlier ones' values along and the last write counts;
+// where all four are one slot in every lane (nodes in order, far apart) they
+// are added first.
 __device__ __forceinline__ void add_slots(DGMC_LDS float* hist,
-                                          const int (&sl)[16], f32x16 v) {
-  if constexpr (RUNS) {
-    int lo = sl[0], hi = sl[0];
-    float s = v[0];
-#pragma unroll
-    for (int r = 1; r < 16; ++r) {
-      lo = min(lo, sl[r]);
-      hi = max(hi, sl[r]);
-      s += v[r];
-    }
-    if (__all(lo == hi)) {
-      hist[lo * 64] += s;
-      return;
-    }
+                                          const int (&sl)[4],
+                                          const float (&v)[4]) {
+  const int a = sl[0], b = sl[1], c = sl[2], d = sl[3];
+  if (__all(a == b && b == c && c == d)) {
+    hist[a * 64] += (v[0] + v[1]) + (v[2] + v[3]);
+    return;
   }
-#pragma unroll
-  for (int k = 0; k < 16; k += 4) {
-    const int a = sl[k], b = sl[k + 1], c = sl[k + 2], d = sl[k + 3];
-    const float ha = hist[a * 64], hb = hist[b * 64], hc = hist[c * 64],
-                hd = hist[d * 64];
-    const float va = v[k], vb = v[k + 1] + (a == b ? va : 0.f);
-    const float vc = v[k + 2] + (b == c ? vb : a == c ? va : 0.f);
-    const float vd =
-        v[k + 3] + (c == d ? vc : b == d ? vb : a == d ? va : 0.f);
-    hist[a * 64] = ha + va;
-    hist[b * 64] = hb + vb;
-    hist[c * 64] = hc + vc;
-    hist[d * 64] = hd + vd;
-  }
+  const float ha = hist[a * 64], hb = hist[b * 64], hc = hist[c * 64],
+              hd = hist[d * 64];
+  const float va = v[0], vb = v[1] + (a == b ? va : 0.f);
+  const float vc = v[2] + (b == c ? vb : a == c ? va : 0.f);
+  const float vd = v[3] + (c == d ? vc : b == d ? vb : a == d ? va : 0.f);
+  hist[a * 64] = ha + va;
+  hist[b * 64] = hb + vb;
+  hist[c * 64] = hc + vc;
+  hist[d * 64] = hd + vd;
 }
 
 template <typename T, int DP, int NW, int POS>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(const Args a,
-                                                        int ntiles) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(
+    const Args a, int ntiles) {
   constexpr int KT = 32;
   constexpr int CH = DP * (int)sizeof(T) / 16;
   constexpr int NT = NW * 64;
@@ -98,8 +66,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(con
   const int kvh = blockIdx.x % a.KV, blk = blockIdx.x / a.KV;
   const int nblk = gridDim.x / a.KV;
   const int QW = 32 / a.G, TQ = QW * NW;
-  const int g = c % a.G, W = 2 * a.half + 2;
-  const int head = kvh * a.G + g;
+  const int cq = div_group(a, c), g = c - cq * a.G, W = 2 * a.half + 2;
+  const int head = kvh * a.G + g, qo = wave * QW + cq;
   const Bucket bk(a);
   const DGMC_LDS float* mytab = tab + g * kSlots;
   DGMC_LDS float* myhist = hist + wave * a.slots * 64 + lane;
@@ -107,25 +75,20 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(con
     load_table(a, kvh, tab, POS);
     for (int s = 0; s < a.slots; ++s) myhist[s * 64] = 0.f;
   }
-  const int64_t ksb = a.k_sn * (int)sizeof(T), vsb = a.v_sn * (int)sizeof(T);
+  const T* kbase = (const T*)a.k + (int64_t)kvh * a.k_sh;
+  const T* vbase = (const T*)a.v + (int64_t)kvh * a.v_sh;
+  const bool capped = a.cap > 0.f;
+  const float s1 = capped ? a.scale / a.cap : a.scale * kLog2e;
+  const float s2 = a.cap * kLog2e;
+  const int rows0 = row_base<CH>(), cols0 = Mma<T>::template cols<CH>();
 
   for (int it = blk; it < ntiles * a.splits; it += nblk) {
     const int split = it % a.splits;
     const int q_lo = it / a.splits * TQ, q_hi = min(q_lo + TQ, a.Nq);
-    int b0, b1, k_lo, k_hi;
-    tile_range(a.ptr_q, a.ptr_k, a.B, a.Nq, a.Nk, q_lo, q_hi, b0, b1, k_lo,
-               k_hi);
-    const int ntile = (k_hi - k_lo + KT - 1) / KT;
-    const int per = split_tiles(a, ntile);
-    if (split > 0 && split * per >= ntile) continue;
-    k_lo += split * per * KT;
-    k_hi = min(k_lo + per * KT, k_hi);
-
-    const int64_t qi = (int64_t)q_lo + wave * QW + c / a.G;
+    const int qi = q_lo + qo;
     const bool live = c < QW * a.G && qi < q_hi;
-    const int64_t row = qi * a.H + head;
-    const int qo = wave * QW + c / a.G;
-    u32x4 qf[CH / 2], gf[CH / 2], of[CH / 2];
+    const int64_t row = (int64_t)qi * a.H + head;
+    u32x4 qf[CH / 2], gf[CH / 2];
     load_frags<T>(qf,
                   (const T*)a.q + (int64_t)q_lo * a.q_sn +
                       (int64_t)kvh * a.G * a.q_sh,
@@ -136,19 +99,34 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(con
                       (int64_t)kvh * a.G * a.g_sh,
                   (qo * a.g_sn + g * a.g_sh) * (int64_t)sizeof(T), live, a.D,
                   a.vec_g);
-    const int64_t ob = ((int64_t)q_lo * a.H + kvh * a.G) * a.D;
-    const int64_t oo = ((int64_t)qo * a.H + g) * a.D * (int64_t)sizeof(T);
-    load_frags<T>(of, (const T*)a.o + ob, oo, live, a.D, a.vec_o);
-    const float lse = live ? a.lse[row] : INFINITY;
+    const int wrows = min(QW, q_hi - q_lo - wave * QW);
+    const Rows w =
+        Rows::find<NW>(a.ptr_q, a.ptr_k, a.B, a.Nq, a.Nk, q_lo, q_hi, qi,
+                       wrows > 0 ? (wrows - 1) * a.G : -1);
+    const int ntile = (w.hi - w.lo + KT - 1) / KT;
+    const int per = split_tiles(a, ntile);
+    if (split > 0 && split * per >= ntile) continue;
+    const int k_lo = w.lo + split * per * KT;
+    const int k_hi = min(k_lo + per * KT, w.hi);
+
+    // delta, in two parts of the output for bf16 (its rounding's rest).
     float dl = 0.f;
-#pragma unroll
-    for (int s = 0; s < CH / 2; ++s) dl += Mma<T>::chunk_dot(gf[s], of[s]);
-    if constexpr (sizeof(T) == 2) {
-      load_frags<T>(of, (const T*)a.out_lo + ob, oo, live, a.D, a.vec_o);
+    {
+      const int64_t ob = ((int64_t)q_lo * a.H + kvh * a.G) * a.D;
+      const int64_t oo = ((int64_t)qo * a.H + g) * a.D * (int64_t)sizeof(T);
+      u32x4 of[CH / 2];
+      load_frags<T>(of, (const T*)a.o + ob, oo, live, a.D, a.vec_o);
 #pragma unroll
       for (int s = 0; s < CH / 2; ++s) dl += Mma<T>::chunk_dot(gf[s], of[s]);
+      if constexpr (sizeof(T) == 2) {
+        load_frags<T>(of, (const T*)a.out_lo + ob, oo, live, a.D, a.vec_o);
+#pragma unroll
+        for (int s = 0; s < CH / 2; ++s)
+          dl += Mma<T>::chunk_dot(gf[s], of[s]);
+      }
     }
     dl = sum_half(dl);
+    const float lse = live ? a.lse[row] : INFINITY;
     if (live && h == 0 && split == 0) a.delta[row] = dl;
     float px = 0.f, py = 0.f;
     if (POS > 0 && live) {
@@ -156,22 +134,6 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(con
       if (POS == 2) py = load_pos(a.pos_q, qi, POS, 1);
     }
 
-    // The row's own keys; the wave's first and last row bound them all.
-    const int w0 = q_lo + wave * QW, wrows = min(QW, q_hi - w0);
-    int r_lo = 0, r_hi = 0, f_lo = 0, f_hi = 0, l_lo = 0, l_hi = 0;
-    int seg = -1;
-    if (wrows > 0) {
-      seg = lane_segment(a.ptr_q, a.B, a.Nq,
-                         segment_of(a.ptr_q, a.B, a.Nq, w0),
-                         min((int)qi, q_hi - 1));
-      seg_range(a.ptr_k, seg, a.B, a.Nk, r_lo, r_hi);
-      const int last = (wrows - 1) * a.G;
-      f_lo = lane_int(r_lo, 0), f_hi = lane_int(r_hi, 0);
-      l_lo = lane_int(r_lo, last), l_hi = lane_int(r_hi, last);
-    }
-
-    const T* kbase = (const T*)a.k + (int64_t)kvh * a.k_sh;
-    const T* vbase = (const T*)a.v + (int64_t)kvh * a.v_sh;
     float pr[2] = {0.f, 0.f};
     auto fetch = [&](int k0, int e, int buf) {
       using S = Stager<T, KT, CH, NT>;
@@ -179,14 +141,13 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(con
       DGMC_LDS char* kt = lds + buf * 2 * TB;
       const auto ok = [&](int r) { return r < left; };
       S::fill(kbase + (int64_t)k0 * a.k_sn, a.D, a.vec_k, kt, ok,
-              [&](int r) { return r * ksb; });
+              [&](int r) { return r * (a.k_sn * (int)sizeof(T)); });
       S::fill(vbase + (int64_t)k0 * a.v_sn, a.D, a.vec_v, kt + TB, ok,
-              [&](int r) { return r * vsb; });
+              [&](int r) { return r * (a.v_sn * (int)sizeof(T)); });
       if constexpr (POS > 0) {
         if (tid < KT && tid < left) {
-          const int64_t j = (int64_t)k0 + tid;
-          pr[0] = load_pos(a.pos_k, j, POS, 0);
-          if (POS == 2) pr[1] = load_pos(a.pos_k, j, POS, 1);
+          pr[0] = load_pos(a.pos_k, (int64_t)k0 + tid, POS, 0);
+          if (POS == 2) pr[1] = load_pos(a.pos_k, (int64_t)k0 + tid, POS, 1);
         }
       }
     };
@@ -201,85 +162,81 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(con
 
     // Passes as in the forward; the table's gradient is whole after the first
     // (no sum over a tile enters a dz).
-    for (int pass = b0 - 1;; ++pass) {
-    int p_lo = k_lo, p_hi = k_hi;
-    if (pass >= b0) {
-      seg_range(a.ptr_k, pass, a.B, a.Nk, p_lo, p_hi);
-      p_lo = max(p_lo, k_lo);
-      p_hi = min(p_hi, k_hi);
-    }
-    f32x16 acc[DP / 32];
+    for (int pass = w.b0 - 1;; ++pass) {
+      int p_lo, p_hi;
+      w.pass_range(a.ptr_k, a.B, a.Nk, pass, k_lo, k_hi, p_lo, p_hi);
+      f32x16 acc[DP / 32];
 #pragma unroll
-    for (int k = 0; k < DP / 32; ++k)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[k][r] = 0.f;
-
-    stage_barrier();       // the last tile staged before has been read
-    if (p_lo < p_hi) fetch(p_lo, p_hi, 0);
-    for (int k0 = p_lo, buf = 0; k0 < p_hi; k0 += KT, buf ^= 1) {
-      put_pos(buf);
-      stage_barrier();
-      if (k0 + KT < p_hi) fetch(k0 + KT, p_hi, buf ^ 1);
-      if (k0 >= l_hi || k0 + KT <= f_lo) continue;  // none of this wave's
-      const DGMC_LDS char* kt = lds + buf * 2 * TB;
-      f32x16 z, dp, th;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) z[r] = dp[r] = th[r] = 0.f;
-#pragma unroll
-      for (int s = 0; s < CH / 2; ++s) {
-        z = Mma<T>::dot(lds_chunk<CH>(kt, c, 2 * s + h), qf[s], z);
-        dp = Mma<T>::dot(lds_chunk<CH>(kt + TB, c, 2 * s + h), gf[s], dp);
-      }
-      cap_scores<sizeof(T) == 4>(a, z, th);
-      int sl[16];
-      if constexpr (POS > 0) {
+      for (int k = 0; k < DP / 32; ++k) acc[k] = f32x16{};
+      stage_barrier();     // the last tile staged before has been read
+      if (p_lo < p_hi) fetch(p_lo, p_hi, 0);
+      for (int k0 = p_lo, buf = 0; k0 < p_hi; k0 += KT, buf ^= 1) {
+        put_pos(buf);
+        stage_barrier();
+        if (k0 + KT < p_hi) fetch(k0 + KT, p_hi, buf ^ 1);
+        if (w.skip(k0, KT)) continue;
+        const int rows = lane_base<CH>(rows0 + buf * 2 * TB);
+        const int cols = lane_base<CH>(cols0 + buf * 2 * TB);
+        f32x16 z = row_dot<T, CH>(lds, rows, qf);
+        const f32x16 dp = row_dot<T, CH>(lds + TB, rows, gf);
+        const bool whole = w.whole(k0, KT);
+        const unsigned n = w.r_hi - w.r_lo;
+        const int j0 = k0 + 4 * h - w.r_lo;
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
-          const int rw = 8 * r4 + 4 * h;
-          const f32x4 kx =
-              *(const DGMC_LDS f32x4*)(kpos + (buf * 2 + 0) * KT + rw);
-          f32x4 ky = kx;
-          if (POS == 2)
-            ky = *(const DGMC_LDS f32x4*)(kpos + (buf * 2 + 1) * KT + rw);
+          float v[4], t[4] = {0.f, 0.f, 0.f, 0.f};
+          int sl[4] = {0, 0, 0, 0};
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            int s = bk.slot(kx[r] - px);
-            if (POS == 2) s = s * W + bk.slot(ky[r] - py);
-            sl[4 * r4 + r] = s;
-            z[4 * r4 + r] += mytab[s];
+          for (int r = 0; r < 4; ++r) v[r] = z[4 * r4 + r] * s1;
+          if (capped) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              t[r] = tanh_<sizeof(T) == 4>(v[r]);
+              v[r] = s2 * t[r];
+            }
           }
+          if constexpr (POS > 0) {
+            const int o = 8 * r4 + 4 * h;
+            const f32x4 kx =
+                *(const DGMC_LDS f32x4*)(kpos + (buf * 2 + 0) * KT + o);
+            f32x4 ky = kx;
+            if (POS == 2)
+              ky = *(const DGMC_LDS f32x4*)(kpos + (buf * 2 + 1) * KT + o);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              sl[r] = bk.slot(kx[r] - px);
+              if (POS == 2) sl[r] = sl[r] * W + bk.slot(ky[r] - py);
+              v[r] += mytab[sl[r]];
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            v[r] = exp2_(v[r] - lse) * (dp[4 * r4 + r] - dl);
+          if (!whole) {
+            // (selected, not multiplied away: a masked key may hold NaN)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if ((unsigned)(j0 + 8 * r4 + r) >= n) v[r] = t[r] = 0.f;
+          }
+          if constexpr (POS > 0) {
+            if (pass < w.b0) add_slots(myhist, sl, v);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            z[4 * r4 + r] = v[r] * fmaf(-t[r], t[r], 1.f);
         }
+        Mma<T>::template accum<DP>(acc, lds, cols, z);
       }
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        z[r] = exp2_(z[r] - lse) * (dp[r] - dl);
-      if (k0 < l_lo || k0 + KT > f_hi) {
-        // (selected, not multiplied away: a masked key may hold NaN)
-        const unsigned n = r_hi - r_lo;
-        const int j0 = k0 + 4 * h - r_lo;
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if ((unsigned)(j0 + 8 * (r >> 2) + (r & 3)) >= n) z[r] = 0.f;
+      const bool redo = pass < w.b0 && w.b1 > w.b0 &&
+                        any_lane<NW>(live && not_finite(acc));
+      if (!redo && live && (pass < w.b0 || w.seg == pass)) {
+        if (per < ntile)        // joined by join_kernel
+          put_acc<DP>(a.part_o + ((int64_t)split * a.Nq * a.H + row) * a.D,
+                      acc, a.D, 1.f);
+        else
+          put_acc<DP>((T*)a.dq + row * a.D, acc, a.D, a.scale);
       }
-      if constexpr (POS > 0) {
-        if (pass < b0) add_slots<POS == 1>(myhist, sl, z);
-      }
-      if (a.cap > 0.f) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) z[r] *= fmaf(-th[r], th[r], 1.f);
-      }
-      Mma<T>::template accum<DP>(acc, kt, 0, z);
-    }
-    const bool redo =
-        pass < b0 && b1 > b0 && any_lane<NW>(live && not_finite(acc));
-    if (!redo && live && (pass < b0 || seg == pass)) {
-      if (per < ntile)          // joined by join_kernel
-        put_acc<DP>(a.part_o + ((int64_t)split * a.Nq * a.H + row) * a.D, acc,
-                    a.D, 1.f);
-      else
-        put_acc<DP>((T*)a.dq + row * a.D, acc, a.D, a.scale);
-    }
-    if (pass < b0 ? !redo : pass == b1) break;
+      if (pass < w.b0 ? !redo : pass == w.b1) break;
     }
   }
   if constexpr (POS > 0) {
@@ -290,21 +247,22 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(con
     for (int e = tid; e < a.G * a.slots; e += NT) {
       const int gg = e / a.slots, s = e % a.slots;
       float sum = 0.f;
-      for (int w = 0; w < NW; ++w)
+      for (int wv = 0; wv < NW; ++wv) {
+#pragma unroll 8
         for (int j = 0; j < 64; ++j) {
-          const int col = (j + s) & 63;
-          if ((col & 31) < RW && (col & 31) % a.G == gg)
-            sum += hist[(w * a.slots + s) * 64 + col];
+          const int col = (j + s) & 63, cc = col & 31;
+          const float x = hist[(wv * a.slots + s) * 64 + col];
+          sum += cc < RW && cc - div_group(a, cc) * a.G == gg ? x : 0.f;
         }
+      }
       a.part_bias[((int64_t)blk * a.KV + kvh) * a.G * a.slots + e] = sum;
     }
   }
 }
 
 template <typename T, int DP, int NW, int POS>
-__global__
-    __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void dkv_kernel(
-        const Args a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(
+    const Args a) {
   constexpr int QT = 32;                         // packed rows per tile
   constexpr int CH = DP * (int)sizeof(T) / 16;
   constexpr int NT = NW * 64;
@@ -316,35 +274,12 @@ __global__
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int h = lane >> 5, c = lane & 31;
-  const int kvh = blockIdx.x % a.KV;
+  const int kvh = blockIdx.x % a.KV, split = blockIdx.y;
   const int QW = 32 / a.G, RW = QW * a.G;
   const int k_lo = blockIdx.x / a.KV * 32 * NW;
   const int k_hi = min(k_lo + 32 * NW, a.Nk);
-  int b0, b1, q_lo, q_hi;
-  tile_range(a.ptr_k, a.ptr_q, a.B, a.Nk, a.Nq, k_lo, k_hi, b0, b1, q_lo,
-             q_hi);
-
-  const int64_t kj = (int64_t)k_lo + wave * 32 + c;
+  const int ko = wave * 32 + c, kj = k_lo + ko;
   const bool live = kj < k_hi;
-  // The queries of this split.
-  const int ntile = (q_hi - q_lo + QW - 1) / QW;
-  const int per = split_tiles(a, ntile), split = blockIdx.y;
-  if (split > 0 && split * per >= ntile) return;
-  q_lo += split * per * QW;
-  q_hi = min(q_lo + per * QW, q_hi);
-  // The key's own queries; the wave's first and last key bound them all.
-  const int w0 = k_lo + wave * 32, wrows = min(32, k_hi - w0);
-  int r_lo = 0, r_hi = 0, f_lo = 0, f_hi = 0, l_lo = 0, l_hi = 0;
-  int seg = -1;
-  if (wrows > 0) {
-    seg = lane_segment(a.ptr_k, a.B, a.Nk,
-                       segment_of(a.ptr_k, a.B, a.Nk, w0),
-                       min((int)kj, k_hi - 1));
-    seg_range(a.ptr_q, seg, a.B, a.Nq, r_lo, r_hi);
-    f_lo = lane_int(r_lo, 0), f_hi = lane_int(r_hi, 0);
-    l_lo = lane_int(r_lo, wrows - 1), l_hi = lane_int(r_hi, wrows - 1);
-  }
-  const int ko = wave * 32 + c;
   u32x4 kf[CH / 2], vf[CH / 2];
   load_frags<T>(kf,
                 (const T*)a.k + (int64_t)k_lo * a.k_sn +
@@ -354,23 +289,27 @@ __global__
                 (const T*)a.v + (int64_t)k_lo * a.v_sn +
                     (int64_t)kvh * a.v_sh,
                 ko * a.v_sn * (int64_t)sizeof(T), live, a.D, a.vec_v);
+  const int wrows = min(32, k_hi - k_lo - wave * 32);
+  const Rows w = Rows::find<NW>(a.ptr_k, a.ptr_q, a.B, a.Nk, a.Nq, k_lo, k_hi,
+                                kj, wrows > 0 ? wrows - 1 : -1);
+  // The queries of this split.
+  const int ntile = (w.hi - w.lo + QW - 1) / QW;
+  const int per = split_tiles(a, ntile);
+  if (split > 0 && split * per >= ntile) return;
+  const int q_lo = w.lo + split * per * QW;
+  const int q_hi = min(q_lo + per * QW, w.hi);
+
   float px = 0.f, py = 0.f;
   const Bucket bk(a);
   const int W = 2 * a.half + 2;
-  int gb[16];                     // the accumulator rows' tables
   if constexpr (POS > 0) {
     load_table(a, kvh, tab, POS);
     if (live) {
       px = load_pos(a.pos_k, kj, POS, 0);
       if (POS == 2) py = load_pos(a.pos_k, kj, POS, 1);
     }
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-      gb[r] = ((8 * (r >> 2) + 4 * h + (r & 3)) % a.G) * kSlots;
   }
 
-  const int64_t qsb = a.q_sn * (int)sizeof(T), qhb = a.q_sh * (int)sizeof(T);
-  const int64_t gsb = a.g_sn * (int)sizeof(T), ghb = a.g_sh * (int)sizeof(T);
   const T* qbase = (const T*)a.q + (int64_t)kvh * a.G * a.q_sh;
   const T* gbase = (const T*)a.dout + (int64_t)kvh * a.G * a.g_sh;
   float rv[4] = {INFINITY, 0.f, 0.f, 0.f};
@@ -378,20 +317,24 @@ __global__
     using S = Stager<T, QT, CH, NT>;
     const int left = e - q0;
     DGMC_LDS char* qt = lds + buf * 2 * TB;
-    const auto ok = [&](int r) { return r < RW && r / a.G < left; };
+    const auto ok = [&](int r) { return r < RW && div_group(a, r) < left; };
+    const auto off = [&](int r, int64_t sn, int64_t sh) {
+      const int i = div_group(a, r);
+      return (i * sn + (r - i * a.G) * sh) * (int64_t)sizeof(T);
+    };
     S::fill(qbase + (int64_t)q0 * a.q_sn, a.D, a.vec_q, qt, ok,
-            [&](int r) { return r / a.G * qsb + r % a.G * qhb; });
+            [&](int r) { return off(r, a.q_sn, a.q_sh); });
     S::fill(gbase + (int64_t)q0 * a.g_sn, a.D, a.vec_g, qt + TB, ok,
-            [&](int r) { return r / a.G * gsb + r % a.G * ghb; });
+            [&](int r) { return off(r, a.g_sn, a.g_sh); });
     if (tid < QT) {
-      const int64_t qi = (int64_t)q0 + tid / a.G;
-      const bool ok = tid < RW && qi < e;
-      const int64_t row = qi * a.H + kvh * a.G + tid % a.G;
-      rv[0] = ok ? a.lse[row] : INFINITY;      // p = 0 in a row not there
-      rv[1] = ok ? a.delta[row] : 0.f;
+      const int i = div_group(a, tid), qi = q0 + i;
+      const bool there = tid < RW && qi < e;
+      const int64_t row = (int64_t)qi * a.H + kvh * a.G + tid - i * a.G;
+      rv[0] = there ? a.lse[row] : INFINITY;   // p = 0 in a row not there
+      rv[1] = there ? a.delta[row] : 0.f;
       if (POS > 0) {
-        rv[2] = ok ? load_pos(a.pos_q, qi, POS, 0) : 0.f;
-        if (POS == 2) rv[3] = ok ? load_pos(a.pos_q, qi, POS, 1) : 0.f;
+        rv[2] = there ? load_pos(a.pos_q, qi, POS, 0) : 0.f;
+        if (POS == 2) rv[3] = there ? load_pos(a.pos_q, qi, POS, 1) : 0.f;
       }
     }
   };
@@ -402,93 +345,99 @@ __global__
         rowv[(buf * 4 + k) * QT + tid] = rv[k];
     }
   };
+  const bool capped = a.cap > 0.f;
+  const float s1 = capped ? a.scale / a.cap : a.scale * kLog2e;
+  const float s2 = a.cap * kLog2e;
+  const int rows0 = row_base<CH>(), cols0 = Mma<T>::template cols<CH>();
 
   // Passes as in the forward.
-  for (int pass = b0 - 1;; ++pass) {
-  int p_lo = q_lo, p_hi = q_hi;
-  if (pass >= b0) {
-    seg_range(a.ptr_q, pass, a.B, a.Nq, p_lo, p_hi);
-    p_lo = max(p_lo, q_lo);
-    p_hi = min(p_hi, q_hi);
-    stage_barrier();
-  }
-  f32x16 ak[DP / 32], av[DP / 32];
+  for (int pass = w.b0 - 1;; ++pass) {
+    int p_lo, p_hi;
+    w.pass_range(a.ptr_q, a.B, a.Nq, pass, q_lo, q_hi, p_lo, p_hi);
+    f32x16 ak[DP / 32], av[DP / 32];
 #pragma unroll
-  for (int k = 0; k < DP / 32; ++k)
+    for (int k = 0; k < DP / 32; ++k) ak[k] = av[k] = f32x16{};
+    if (pass >= w.b0) stage_barrier();
+    if (p_lo < p_hi) fetch(p_lo, p_hi, 0);
+    for (int q0 = p_lo, buf = 0; q0 < p_hi; q0 += QW, buf ^= 1) {
+      put_rows(buf);
+      stage_barrier();
+      if (q0 + QW < p_hi) fetch(q0 + QW, p_hi, buf ^ 1);
+      if (w.skip(q0, QW)) continue;
+      const DGMC_LDS float* rw = rowv + buf * 4 * QT;
+      const int rows = lane_base<CH>(rows0 + buf * 2 * TB);
+      const int cols = lane_base<CH>(cols0 + buf * 2 * TB);
+      f32x16 z = row_dot<T, CH>(lds, rows, kf);
+      f32x16 dp = row_dot<T, CH>(lds + TB, rows, vf);
+      const bool whole = w.whole(q0, QW);
+      const unsigned n = (w.r_hi - w.r_lo) * a.G;
+      const int j0 = (q0 - w.r_lo) * a.G + 4 * h;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) ak[k][r] = av[k][r] = 0.f;
-
-  if (p_lo < p_hi) fetch(p_lo, p_hi, 0);
-  for (int q0 = p_lo, buf = 0; q0 < p_hi; q0 += QW, buf ^= 1) {
-    put_rows(buf);
-    stage_barrier();
-    if (q0 + QW < p_hi) fetch(q0 + QW, p_hi, buf ^ 1);
-    if (q0 >= l_hi || q0 + QW <= f_lo) continue;  // none of this wave's
-    const DGMC_LDS char* qt = lds + buf * 2 * TB;
-    const DGMC_LDS float* rw = rowv + buf * 4 * QT;
-    f32x16 z, dp, th;
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const int o = 8 * r4 + 4 * h;
+        const f32x4 ls = *(const DGMC_LDS f32x4*)(rw + o);
+        const f32x4 de = *(const DGMC_LDS f32x4*)(rw + QT + o);
+        float p[4], t[4] = {0.f, 0.f, 0.f, 0.f}, ds[4];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) z[r] = dp[r] = th[r] = 0.f;
+        for (int r = 0; r < 4; ++r) p[r] = z[4 * r4 + r] * s1;
+        if (capped) {
 #pragma unroll
-    for (int s = 0; s < CH / 2; ++s) {
-      z = Mma<T>::dot(lds_chunk<CH>(qt, c, 2 * s + h), kf[s], z);
-      dp = Mma<T>::dot(lds_chunk<CH>(qt + TB, c, 2 * s + h), vf[s], dp);
-    }
-    cap_scores<sizeof(T) == 4>(a, z, th);
+          for (int r = 0; r < 4; ++r) {
+            t[r] = tanh_<sizeof(T) == 4>(p[r]);
+            p[r] = s2 * t[r];
+          }
+        }
+        if constexpr (POS > 0) {
+          const f32x4 qx = *(const DGMC_LDS f32x4*)(rw + 2 * QT + o);
+          f32x4 qy = qx;
+          if (POS == 2) qy = *(const DGMC_LDS f32x4*)(rw + 3 * QT + o);
 #pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      const int o = 8 * r4 + 4 * h;
-      const f32x4 ls = *(const DGMC_LDS f32x4*)(rw + o);
-      const f32x4 de = *(const DGMC_LDS f32x4*)(rw + QT + o);
-      if constexpr (POS > 0) {
-        const f32x4 qx = *(const DGMC_LDS f32x4*)(rw + 2 * QT + o);
-        f32x4 qy = qx;
-        if (POS == 2) qy = *(const DGMC_LDS f32x4*)(rw + 3 * QT + o);
+          for (int r = 0; r < 4; ++r) {
+            int s = bk.slot(px - qx[r]);
+            if (POS == 2) s = s * W + bk.slot(py - qy[r]);
+            // (the row's head: its table)
+            const int i = o + r;
+            if (a.G > 1) s += (i - div_group(a, i) * a.G) * kSlots;
+            p[r] += tab[s];
+          }
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          int s = bk.slot(px - qx[r]);
-          if (POS == 2) s = s * W + bk.slot(py - qy[r]);
-          z[4 * r4 + r] += tab[gb[4 * r4 + r] + s];
+          p[r] = exp2_(p[r] - ls[r]);
+          ds[r] = p[r] * (dp[4 * r4 + r] - de[r]);
+        }
+        if (!whole) {
+          // Packed rows of other segments (selected, not multiplied away:
+          // they may hold NaN; rows from RW on have p = 0).
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if ((unsigned)(j0 + 8 * r4 + r) >= n) p[r] = ds[r] = t[r] = 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          z[4 * r4 + r] = p[r];
+          dp[4 * r4 + r] = ds[r] * fmaf(-t[r], t[r], 1.f);
         }
       }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 4 * r4 + r;
-        z[i] = exp2_(z[i] - ls[r]);
-        dp[i] = z[i] * (dp[i] - de[r]);
+      Mma<T>::template accum<DP>(av, lds + TB, cols, z);
+      Mma<T>::template accum<DP>(ak, lds, cols, dp);
+    }
+    const bool redo =
+        pass < w.b0 && w.b1 > w.b0 &&
+        any_lane<NW>(live && (not_finite(ak) || not_finite(av)));
+    if (!redo && live && (pass < w.b0 || w.seg == pass)) {
+      const int64_t row = (int64_t)kj * a.KV + kvh;
+      if (per < ntile) {        // joined by join_kernel
+        const int64_t all = (int64_t)a.Nk * a.KV;
+        float* p = a.part_o + (split * all + row) * a.D;
+        put_acc<DP>(p, ak, a.D, 1.f);
+        put_acc<DP>(p + a.splits * all * a.D, av, a.D, 1.f);
+      } else {
+        put_acc<DP>((T*)a.dk + row * a.D, ak, a.D, a.scale);
+        put_acc<DP>((T*)a.dv + row * a.D, av, a.D, 1.f);
       }
     }
-    if (q0 < l_lo || q0 + QW > f_hi) {
-      // Packed rows of other segments (selected, not multiplied away: they
-      // may hold NaN; rows from RW on have p = 0).
-      const unsigned n = (r_hi - r_lo) * a.G;
-      const int j0 = (q0 - r_lo) * a.G + 4 * h;
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if ((unsigned)(j0 + 8 * (r >> 2) + (r & 3)) >= n) z[r] = dp[r] = 0.f;
-    }
-    if (a.cap > 0.f) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) dp[r] *= fmaf(-th[r], th[r], 1.f);
-    }
-    Mma<T>::template accum<DP>(av, qt + TB, 0, z);
-    Mma<T>::template accum<DP>(ak, qt, 0, dp);
-  }
-  const bool redo = pass < b0 && b1 > b0 &&
-                    any_lane<NW>(live && (not_finite(ak) || not_finite(av)));
-  if (!redo && live && (pass < b0 || seg == pass)) {
-    const int64_t row = kj * a.KV + kvh;
-    if (per < ntile) {          // joined by join_kernel
-      const int64_t rows = (int64_t)a.Nk * a.KV;
-      float* p = a.part_o + (split * rows + row) * a.D;
-      put_acc<DP>(p, ak, a.D, 1.f);
-      put_acc<DP>(p + a.splits * rows * a.D, av, a.D, 1.f);
-    } else {
-      put_acc<DP>((T*)a.dk + row * a.D, ak, a.D, a.scale);
-      put_acc<DP>((T*)a.dv + row * a.D, av, a.D, 1.f);
-    }
-  }
-  if (pass < b0 ? !redo : pass == b1) return;
+    if (pass < w.b0 ? !redo : pass == w.b1) return;
   }
 }
 

@@ -22,11 +22,13 @@ namespace dgmc {
 namespace segattn {
 
 template <typename T, int DP, int NW, int KT, int POS, bool FINE>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) void fwd_kernel(
-    const Args a) {
+__global__ __launch_bounds__(
+    NW * 64, sizeof(T) == 2 ? (DP <= 64 ? 4 : 2) : 1) void
+fwd_kernel(const Args a) {
   constexpr int CH = DP * (int)sizeof(T) / 16;   // 16-byte chunks per row
   constexpr int NT = NW * 64;
   constexpr int TB = KT * CH * 16;               // bytes of one tile
+  constexpr int UB = 32 * CH * 16;               // bytes of 32 rows
   extern __shared__ __attribute__((aligned(16))) char smem[];
   DGMC_LDS char* lds = (DGMC_LDS char*)smem;
   DGMC_LDS float* kpos = (DGMC_LDS float*)(lds + 4 * TB);   // [2][2][KT]
@@ -37,28 +39,28 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) v
   const int kvh = blockIdx.x % a.KV, split = blockIdx.y;
   const int QW = 32 / a.G, TQ = QW * NW;
   const int q_lo = blockIdx.x / a.KV * TQ, q_hi = min(q_lo + TQ, a.Nq);
-  int b0, b1, k_lo, k_hi;
-  tile_range(a.ptr_q, a.ptr_k, a.B, a.Nq, a.Nk, q_lo, q_hi, b0, b1, k_lo,
-             k_hi);
-  // The keys of this split.
-  const int ntile = (k_hi - k_lo + KT - 1) / KT;
-  const int per = split_tiles(a, ntile);
-  if (split > 0 && split * per >= ntile) return;
-  k_lo += split * per * KT;
-  k_hi = min(k_lo + per * KT, k_hi);
 
   // This lane's packed row.
-  const int g = c % a.G;
-  const int64_t qi = (int64_t)q_lo + wave * QW + c / a.G;
+  const int cq = div_group(a, c), g = c - cq * a.G;
+  const int qo = wave * QW + cq, qi = q_lo + qo;
   const bool live = c < QW * a.G && qi < q_hi;
   const int head = kvh * a.G + g;
   u32x4 qf[CH / 2];
   load_frags<T>(qf,
                 (const T*)a.q + (int64_t)q_lo * a.q_sn +
                     (int64_t)kvh * a.G * a.q_sh,
-                ((wave * QW + c / a.G) * a.q_sn + g * a.q_sh) *
-                    (int64_t)sizeof(T),
-                live, a.D, a.vec_q);
+                (qo * a.q_sn + g * a.q_sh) * (int64_t)sizeof(T), live, a.D,
+                a.vec_q);
+  const int wrows = min(QW, q_hi - q_lo - wave * QW);
+  const Rows w = Rows::find<NW>(a.ptr_q, a.ptr_k, a.B, a.Nq, a.Nk, q_lo, q_hi,
+                                qi, wrows > 0 ? (wrows - 1) * a.G : -1);
+  // The keys of this split.
+  const int ntile = (w.hi - w.lo + KT - 1) / KT;
+  const int per = split_tiles(a, ntile);
+  if (split > 0 && split * per >= ntile) return;
+  const int k_lo = w.lo + split * per * KT;
+  const int k_hi = min(k_lo + per * KT, w.hi);
+
   float px = 0.f, py = 0.f;
   const Bucket bk(a);
   if constexpr (POS > 0) {
@@ -71,24 +73,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) v
   const DGMC_LDS float* mytab = tab + g * kSlots;
   const int W = 2 * a.half + 2;
 
-  // The row's own keys; the wave's first and last row bound them all.
-  const int w0 = q_lo + wave * QW;
-  const int wrows = min(QW, q_hi - w0);
-  int r_lo = 0, r_hi = 0, f_lo = 0, f_hi = 0, l_lo = 0, l_hi = 0;
-  int seg = -1;
-  if (wrows > 0) {
-    seg = lane_segment(a.ptr_q, a.B, a.Nq,
-                       segment_of(a.ptr_q, a.B, a.Nq, w0),
-                       min((int)qi, q_hi - 1));
-    seg_range(a.ptr_k, seg, a.B, a.Nk, r_lo, r_hi);
-    const int last = (wrows - 1) * a.G;
-    f_lo = lane_int(r_lo, 0), f_hi = lane_int(r_hi, 0);
-    l_lo = lane_int(r_lo, last), l_hi = lane_int(r_hi, last);
-  }
-
   const T* kbase = (const T*)a.k + (int64_t)kvh * a.k_sh;
   const T* vbase = (const T*)a.v + (int64_t)kvh * a.v_sh;
-  const int64_t ksb = a.k_sn * (int)sizeof(T), vsb = a.v_sn * (int)sizeof(T);
   float pr[2] = {0.f, 0.f};
   // Start the loads of keys [k0, e) into buffer `buf`; their positions wait
   // in registers.
@@ -97,15 +83,15 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) v
     const int left = e - k0;
     DGMC_LDS char* kt = lds + buf * 2 * TB;
     const auto ok = [&](int r) { return r < left; };
-    S::fill(kbase + (int64_t)k0 * a.k_sn, a.D, a.vec_k, kt, ok,
-            [&](int r) { return r * ksb; });
+    S::fill(kbase + (int64_t)k0 * a.k_sn, a.D, a.vec_k, kt, ok, [&](int r) {
+      return r * (a.k_sn * (int)sizeof(T));
+    });
     S::fill(vbase + (int64_t)k0 * a.v_sn, a.D, a.vec_v, kt + TB, ok,
-            [&](int r) { return r * vsb; });
+            [&](int r) { return r * (a.v_sn * (int)sizeof(T)); });
     if constexpr (POS > 0) {
       if (tid < KT && tid < left) {
-        const int64_t j = (int64_t)k0 + tid;
-        pr[0] = load_pos(a.pos_k, j, POS, 0);
-        if (POS == 2) pr[1] = load_pos(a.pos_k, j, POS, 1);
+        pr[0] = load_pos(a.pos_k, (int64_t)k0 + tid, POS, 0);
+        if (POS == 2) pr[1] = load_pos(a.pos_k, (int64_t)k0 + tid, POS, 1);
       }
     }
   };
@@ -123,147 +109,135 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : 1) v
   // Plain scores stay unscaled: 2^(s1 z - m) is one fma and one exp2.
   const bool plain = POS == 0 && a.cap <= 0.f && s1 > 0.f;
   const float ex = plain ? s1 : 1.f;
+  const int rows0 = row_base<CH>(), cols0 = Mma<T>::template cols<CH>();
 
   // Pass b0 - 1: all rows over all keys of the tile; passes b0 .. b1 (only
   // after a non-finite result): segment by segment.
-  for (int pass = b0 - 1;; ++pass) {
-  int p_lo = k_lo, p_hi = k_hi;
-  if (pass >= b0) {
-    seg_range(a.ptr_k, pass, a.B, a.Nk, p_lo, p_hi);
-    p_lo = max(p_lo, k_lo);
-    p_hi = min(p_hi, k_hi);
-    stage_barrier();
-  }
-  f32x16 acc[DP / 32];
+  for (int pass = w.b0 - 1;; ++pass) {
+    int p_lo, p_hi;
+    w.pass_range(a.ptr_k, a.B, a.Nk, pass, k_lo, k_hi, p_lo, p_hi);
+    f32x16 acc[DP / 32];
 #pragma unroll
-  for (int k = 0; k < DP / 32; ++k)
+    for (int k = 0; k < DP / 32; ++k) acc[k] = f32x16{};
+    float m = -INFINITY, l = 0.f;
+    if (pass >= w.b0) stage_barrier();
+    if (p_lo < p_hi) fetch(p_lo, p_hi, 0);
+    for (int k0 = p_lo, buf = 0; k0 < p_hi; k0 += KT, buf ^= 1) {
+      put_pos(buf);
+      stage_barrier();
+      if (k0 + KT < p_hi) fetch(k0 + KT, p_hi, buf ^ 1);
+      if (w.skip(k0, KT)) continue;
+      const int rows = lane_base<CH>(rows0 + buf * 2 * TB);
+      const int cols = lane_base<CH>(cols0 + buf * 2 * TB);
+      f32x16 z[KT / 32];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) acc[k][r] = 0.f;
-  float m = -INFINITY, l = 0.f;
-  if (p_lo < p_hi) fetch(p_lo, p_hi, 0);
-  for (int k0 = p_lo, buf = 0; k0 < p_hi; k0 += KT, buf ^= 1) {
-    put_pos(buf);
-    stage_barrier();
-    if (k0 + KT < p_hi) fetch(k0 + KT, p_hi, buf ^ 1);
-    if (k0 >= l_hi || k0 + KT <= f_lo) continue;    // none of this wave's
-    const DGMC_LDS char* kt = lds + buf * 2 * TB;
-    f32x16 z[KT / 32];
+      for (int u = 0; u < KT / 32; ++u)
+        z[u] = row_dot<T, CH>(lds + u * UB, rows, qf);
+      if (!plain) {
 #pragma unroll
-    for (int u = 0; u < KT / 32; ++u) {
+        for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) z[u][r] = 0.f;
+          for (int r = 0; r < 16; ++r) z[u][r] *= s1;
+        if (a.cap > 0.f) {
 #pragma unroll
-      for (int s = 0; s < CH / 2; ++s)
-        z[u] = Mma<T>::dot(lds_chunk<CH>(kt, 32 * u + c, 2 * s + h), qf[s],
-                           z[u]);
-    }
-    if (a.cap > 0.f) {
+          for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              z[u][r] = s2 * tanh_<sizeof(T) == 4>(z[u][r]);
+        }
+      }
+      if constexpr (POS > 0) {
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u) {
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const int row = 32 * u + 8 * r4 + 4 * h;
+            const f32x4 kx =
+                *(const DGMC_LDS f32x4*)(kpos + (buf * 2 + 0) * KT + row);
+            f32x4 ky = kx;
+            if (POS == 2)
+              ky = *(const DGMC_LDS f32x4*)(kpos + (buf * 2 + 1) * KT + row);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              int s = bk.slot(kx[r] - px);
+              if (POS == 2) s = s * W + bk.slot(ky[r] - py);
+              z[u][4 * r4 + r] += mytab[s];
+            }
+          }
+        }
+      }
+      if (!w.whole(k0, KT)) {
+        const unsigned n = w.r_hi - w.r_lo;
+        const int j0 = k0 + 4 * h - w.r_lo;
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if ((unsigned)(j0 + 32 * u + 8 * (r >> 2) + (r & 3)) >= n)
+              z[u][r] = -INFINITY;
+      }
+      float mt = z[0][0];
 #pragma unroll
       for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          z[u][r] = s2 * tanh_<sizeof(T) == 4>(z[u][r] * s1);
-    } else if (!plain) {
+        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, z[u][r]);
+      mt = max_half(mt) * ex;
+      if (__any(mt > m + 8.f)) {
+        const float mn = fmaxf(m, mt);
+        const float al = mn == m ? 1.f : exp2_(m - mn);
+        l *= al;
 #pragma unroll
-      for (int u = 0; u < KT / 32; ++u)
+        for (int k = 0; k < DP / 32; ++k)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) z[u][r] *= s1;
-    }
-    if constexpr (POS > 0) {
+          for (int r = 0; r < 16; ++r) acc[k][r] *= al;
+        m = mn;
+      }
+      const float ms = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int u = 0; u < KT / 32; ++u) {
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const int row = 32 * u + 8 * r4 + 4 * h;
-          const f32x4 kx =
-              *(const DGMC_LDS f32x4*)(kpos + (buf * 2 + 0) * KT + row);
-          f32x4 ky = kx;
-          if (POS == 2)
-            ky = *(const DGMC_LDS f32x4*)(kpos + (buf * 2 + 1) * KT + row);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            int s = bk.slot(kx[r] - px);
-            if (POS == 2) s = s * W + bk.slot(ky[r] - py);
-            z[u][4 * r4 + r] += mytab[s];
-          }
-        }
-      }
-    }
-    if (k0 < l_lo || k0 + KT > f_hi) {
-      const unsigned n = r_hi - r_lo;
-      const int j0 = k0 + 4 * h - r_lo;
-#pragma unroll
-      for (int u = 0; u < KT / 32; ++u)
-#pragma unroll
         for (int r = 0; r < 16; ++r)
-          if ((unsigned)(j0 + 32 * u + 8 * (r >> 2) + (r & 3)) >= n)
-            z[u][r] = -INFINITY;
-    }
-    float mt = z[0][0];
-#pragma unroll
-    for (int u = 0; u < KT / 32; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mt = fmaxf(mt, z[u][r]);
-    mt = max_half(mt) * ex;
-    if (__any(mt > m + 8.f)) {
-      const float mn = fmaxf(m, mt);
-      const float al = mn == m ? 1.f : exp2_(m - mn);
-      l *= al;
-#pragma unroll
-      for (int k = 0; k < DP / 32; ++k)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[k][r] *= al;
-      m = mn;
-    }
-    const float ms = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int u = 0; u < KT / 32; ++u) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) z[u][r] = exp2_(fmaf(z[u][r], ex, -ms));
-      float s = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s += z[u][r];
-      l += s;
-      Mma<T>::template accum<DP, FINE>(acc, kt + TB, 32 * u,
-                                              z[u]);
-    }
-  }
-  l = sum_half(l);
-  const bool redo =
-      pass < b0 && b1 > b0 && any_lane<NW>(live && not_finite(acc));
-  const int64_t row = qi * a.H + head;
-  if (!redo && live && (pass < b0 || seg == pass)) {
-    if (per < ntile) {          // joined by join_kernel
-      const int64_t prow = (int64_t)split * a.Nq * a.H + row;
-      if (h == 0) {
-        a.part_ml[prow * 2] = m;
-        a.part_ml[prow * 2 + 1] = l;
+          z[u][r] = exp2_(fmaf(z[u][r], ex, -ms));
+        l = Mma<T>::template sum<FINE>(z[u], l);
+        Mma<T>::template accum<DP, FINE>(acc, lds + TB + u * UB, cols, z[u]);
       }
-      put_acc<DP>(a.part_o + prow * a.D, acc, a.D, 1.f);
-    } else {
-      // l is 0 only without a key of finite score: such a row is 0.
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      if (h == 0 && a.lse) a.lse[row] = l == 0.f ? INFINITY : m + log2f(l);
-      T* orow = (T*)a.out + row * a.D;
-#pragma unroll
-      for (int k = 0; k < DP / 32; ++k)
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const int d = 32 * k + 8 * r4 + 4 * h;
-          T o[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[r] = (T)(acc[k][4 * r4 + r] * inv);
-          put4(orow, d, a.D, o);
-          if constexpr (FINE) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              o[r] = (T)(acc[k][4 * r4 + r] * inv - (float)o[r]);
-            put4((T*)a.out_lo + row * a.D, d, a.D, o);
-          }
-        }
     }
-  }
-  if (pass < b0 ? !redo : pass == b1) return;
+    l = sum_half(l);
+    const bool redo = pass < w.b0 && w.b1 > w.b0 &&
+                      any_lane<NW>(live && not_finite(acc));
+    const int64_t row = (int64_t)qi * a.H + head;
+    if (!redo && live && (pass < w.b0 || w.seg == pass)) {
+      if (per < ntile) {        // joined by join_kernel
+        const int64_t prow = (int64_t)split * a.Nq * a.H + row;
+        if (h == 0) {
+          a.part_ml[prow * 2] = m;
+          a.part_ml[prow * 2 + 1] = l;
+        }
+        put_acc<DP>(a.part_o + prow * a.D, acc, a.D, 1.f);
+      } else {
+        // l is 0 only without a key of finite score: such a row is 0.
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (h == 0 && a.lse) a.lse[row] = l == 0.f ? INFINITY : m + log2f(l);
+        T* orow = (T*)a.out + row * a.D;
+#pragma unroll
+        for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const int d = 32 * k + 8 * r4 + 4 * h;
+            T o[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = (T)(acc[k][4 * r4 + r] * inv);
+            put4(orow, d, a.D, o);
+            if constexpr (FINE) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                o[r] = (T)(acc[k][4 * r4 + r] * inv - (float)o[r]);
+              put4((T*)a.out_lo + row * a.D, d, a.D, o);
+            }
+          }
+      }
+    }
+    if (pass < w.b0 ? !redo : pass == w.b1) return;
   }
 }
 
