@@ -53,10 +53,10 @@ struct SegmentAttention
                         const OptTensor& bias, const Tensor& ptr_q,
                         const Tensor& ptr_k, const OptTensor& pos_q,
                         const OptTensor& pos_k, double scale, double cap,
-                        int64_t half, int64_t mbits, double dmax) {
+                        int64_t half, int64_t mbits, double dmax, bool x6) {
     auto [out, lo, lse] =
         segattn::forward(q, k, v, ptr_q, ptr_k, scale, cap, bias, pos_q,
-                         pos_k, {half, mbits, dmax}, true);
+                         pos_k, {half, mbits, dmax}, x6, true);
     ctx->save_for_backward({q, k, v, def(bias), ptr_q, ptr_k, def(pos_q),
                             def(pos_k), out, lo, lse});
     ctx->saved_data["scale"] = scale;
@@ -64,6 +64,7 @@ struct SegmentAttention
     ctx->saved_data["half"] = half;
     ctx->saved_data["mbits"] = mbits;
     ctx->saved_data["dmax"] = dmax;
+    ctx->saved_data["x6"] = x6;
     return out;
   }
 
@@ -76,9 +77,10 @@ struct SegmentAttention
         grad, s[0], s[1], s[2], s[8], s[9], s[10], s[4], s[5],
         d["scale"].toDouble(), d["cap"].toDouble(), opt(s[3]), opt(s[6]),
         opt(s[7]),
-        {d["half"].toInt(), d["mbits"].toInt(), d["dmax"].toDouble()});
+        {d["half"].toInt(), d["mbits"].toInt(), d["dmax"].toDouble()},
+        d["x6"].toBool());
     variable_list r = once({dq, dk, dv, s[3].defined() ? db : Tensor()});
-    r.resize(13);
+    r.resize(14);
     return r;
   }
 };
@@ -87,10 +89,10 @@ Tensor segment_attention(const Tensor& q, const Tensor& k, const Tensor& v,
                          const OptTensor& bias, const Tensor& ptr_q,
                          const Tensor& ptr_k, const OptTensor& pos_q,
                          const OptTensor& pos_k, double scale, double cap,
-                         int64_t half, int64_t mbits, double dmax) {
+                         int64_t half, int64_t mbits, double dmax, bool x6) {
   return std::get<0>(segattn::forward(q, k, v, ptr_q, ptr_k, scale, cap, bias,
                                       pos_q, pos_k, {half, mbits, dmax},
-                                      false));
+                                      x6, false));
 }
 
 Tensor segment_attention_autograd(const Tensor& q, const Tensor& k,
@@ -99,13 +101,13 @@ Tensor segment_attention_autograd(const Tensor& q, const Tensor& k,
                                   const OptTensor& pos_q,
                                   const OptTensor& pos_k, double scale,
                                   double cap, int64_t half, int64_t mbits,
-                                  double dmax) {
+                                  double dmax, bool x6) {
   if (wants_grad(q, k, v, bias))
     return SegmentAttention::apply(q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k,
-                                   scale, cap, half, mbits, dmax);
+                                   scale, cap, half, mbits, dmax, x6);
   at::AutoDispatchBelowADInplaceOrView below;
   return segment_attention(q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k, scale,
-                           cap, half, mbits, dmax);
+                           cap, half, mbits, dmax, x6);
 }
 
 // --------------------------------------------------------------------------
@@ -208,7 +210,7 @@ TORCH_LIBRARY_FRAGMENT(dgmc_amd, m) {
   m.def(
       "segment_attention(Tensor q, Tensor k, Tensor v, Tensor? bias, Tensor "
       "ptr_q, Tensor ptr_k, Tensor? pos_q, Tensor? pos_k, float scale, float "
-      "cap, int half, int mbits, float dmax) -> Tensor");
+      "cap, int half, int mbits, float dmax, bool x6) -> Tensor");
   m.def(
       "layer_norm(Tensor x, Tensor? residual, Tensor? weight, Tensor? bias, "
       "float eps) -> Tensor[]");

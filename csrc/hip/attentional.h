@@ -20,13 +20,14 @@ struct BucketLayout {
 
 namespace segattn {
 
+// `x6`: long fp32 segments on the bf16 matrix cores, three terms an operand.
 // (out, lo, lse): lo (bf16 rest of out's rounding, bf16 only) and lse are
 // empty unless `train`.
 std::tuple<at::Tensor, at::Tensor, at::Tensor> forward(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& ptr_q, const at::Tensor& ptr_k, double scale,
     double cap, const OptTensor& bias, const OptTensor& pos_q,
-    const OptTensor& pos_k, const BucketLayout& layout, bool train);
+    const OptTensor& pos_k, const BucketLayout& layout, bool x6, bool train);
 
 // (dq, dk, dv, dbias): dbias (fp32) is empty without a bias.
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
@@ -34,7 +35,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
     const at::Tensor& v, const at::Tensor& out, const at::Tensor& lo,
     const at::Tensor& lse, const at::Tensor& ptr_q, const at::Tensor& ptr_k,
     double scale, double cap, const OptTensor& bias, const OptTensor& pos_q,
-    const OptTensor& pos_k, const BucketLayout& layout);
+    const OptTensor& pos_k, const BucketLayout& layout, bool x6);
 
 }  // namespace segattn
 

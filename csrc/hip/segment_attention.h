@@ -33,8 +33,13 @@
 // accumulator's rows then serve directly as the K index of the second
 // product: its other operand is read from LDS in that same row order
 // (bf16: ds_read_b64_tr_b16, 4 rows a time; fp32: one value a lane), no
-// lane exchange of P.  bf16 runs on v_mfma_f32_32x32x16_bf16, fp32 on
-// v_mfma_f32_32x32x2_f32 (exact products, fp32 sums).
+// lane exchange of P.  bf16 runs on v_mfma_f32_32x32x16_bf16; fp32 either on
+// v_mfma_f32_32x32x2_f32 (exact products, fp32 sums) or, where segments are
+// long, as "x6": every operand as three bf16 terms (hi + mid + lo = all 24
+// bits), the six largest of their nine products on the bf16 instruction -
+// 192 matrix cycles in place of 512 for the same 32 x 32 x 16 block, terms
+// from 2^-24 on dropped.  The operands' planes are written once by a kernel
+// of their own, P and dS are split in registers.
 //
 // Bucket of an offset d = pos_j - pos_i on one axis: b(|d|) with `steps` =
 // 2^m buckets per octave, read off the float 2 (|d| / steps + 1): its
@@ -73,7 +78,8 @@ struct Args {
   const int *ptr_q, *ptr_k;
   const float* bias;                  // [H, nb]
   const int *pos_q, *pos_k;           // [N, axes]
-  int64_t q_sn, q_sh, k_sn, k_sh, v_sn, v_sh, o_sn, o_sh, g_sn, g_sh;
+  int64_t q_sn, q_sh, k_sn, k_sh, v_sn, v_sh, g_sn, g_sh;
+  int64_t q_sp, k_sp, v_sp, g_sp;     // between the planes (x6)
   int B, Nq, Nk, H, KV, G, gmul, D, nb, half, mbits, slots;
   float scale, cap, dmax, dmul;
   int vec_q, vec_k, vec_v, vec_o, vec_g;   // 16-byte rows
@@ -297,34 +303,41 @@ __device__ __forceinline__ u32x4 load_chunk(const T* row, int ch, int D,
 // --------------------------------------------------------------------------
 constexpr unsigned kNoRow = 0x80000000u;   // past every buffer's range
 
-template <typename T, int ROWS, int CH, int NT>
+template <typename P, int ROWS, int CH, int NT>
 struct Stager {
-  static constexpr int E = 16 / (int)sizeof(T);
+  using S = typename P::S;
+  static constexpr int E = 16 / (int)sizeof(S);
   static constexpr int N = (ROWS * CH + NT - 1) / NT;
   static constexpr bool kFull = N * NT == ROWS * CH;
 
   // `ok(row)`: the row is there, at `off(row)` bytes from `base` (below 2^31
-  // where vec is set).
+  // where vec is set); planes `sp` elements apart.
   template <typename Ok, typename Off>
-  __device__ __forceinline__ static void fill(const T* base, int D, int vec,
+  __device__ __forceinline__ static void fill(const S* base, int64_t sp,
+                                              int D, int vec,
                                               DGMC_LDS char* tile, Ok ok,
                                               Off off) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (vec) {
+    if (vec || P::kPlanes > 1) {
       // (a wave's many slots are computed anew every tile, a few are kept)
       const int tid = N > 2 ? opaque(threadIdx.x) : threadIdx.x;
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<T*>(base), 0, 0x80000000u, 0x00020000);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (!kFull && i * NT + wave * 64 >= ROWS * CH) continue;
-        const int r = (tid + i * NT) / CH;
-        const int ch = ((tid + i * NT) % CH) ^ swz<CH>(r);
-        const unsigned o =
-            ok(r) && ch * E < D ? (unsigned)off(r) + ch * 16 : kNoRow;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rs, (DGMC_LDS void*)(tile + (i * NT + wave * 64) * 16), 16, o, 0,
-            0, 0);
+      for (int p = 0; p < P::kPlanes; ++p) {
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<S*>(base + p * sp), 0, 0x80000000u, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (!kFull && i * NT + wave * 64 >= ROWS * CH) continue;
+          const int r = (tid + i * NT) / CH;
+          const int ch = ((tid + i * NT) % CH) ^ swz<CH>(r);
+          const unsigned o =
+              ok(r) && ch * E < D ? (unsigned)off(r) + ch * 16 : kNoRow;
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(
+              rs,
+              (DGMC_LDS void*)(tile + (p * ROWS * CH + i * NT + wave * 64) *
+                                          16),
+              16, o, 0, 0, 0);
+        }
       }
     } else {
       const int tid = opaque(threadIdx.x);
@@ -333,21 +346,21 @@ struct Stager {
         if (!kFull && tid + i * NT >= ROWS * CH) continue;
         const int r = (tid + i * NT) / CH;
         const int ch = ((tid + i * NT) % CH) ^ swz<CH>(r);
-        const u32x4 v = load_chunk<T>(
-            (const T*)((const char*)base + off(r)), ch, D, ok(r), 0);
+        const u32x4 v = load_chunk<S>(
+            (const S*)((const char*)base + off(r)), ch, D, ok(r), 0);
         *(DGMC_LDS u32x4*)(tile + (tid + i * NT) * 16) = v;
       }
     }
   }
 };
 
-// The 16-byte chunks h, h + 2, .. of this lane's own row (an MFMA operand):
-// at `off` bytes from the wave-uniform `base`, zeros where it is not `live`.
-// All loads are issued before the first is needed (no branch around them).
+// The 16-byte chunks h, h + 2, .. of this lane's own row: at `off` bytes from
+// the wave-uniform `base`, zeros where it is not `live`.  All loads are
+// issued before the first is needed (no branch around them).
 template <typename T, int N>
-__device__ __forceinline__ void load_frags(u32x4 (&f)[N], const T* base,
-                                           int64_t off, bool live, int D,
-                                           int vec) {
+__device__ __forceinline__ void load_row(u32x4 (&f)[N], const T* base,
+                                         int64_t off, bool live, int D,
+                                         int vec) {
   constexpr int E = 16 / (int)sizeof(T);
   const int h = (threadIdx.x >> 5) & 1;
   if (vec) {
@@ -367,6 +380,30 @@ __device__ __forceinline__ void load_frags(u32x4 (&f)[N], const T* base,
   }
 }
 
+// Of an fp32 row, the elements that load_row takes of a bf16 one: chunks 4 s
+// + 2 h and the next.
+template <int N>
+__device__ __forceinline__ void load_row8(u32x4 (&f)[N], const float* base,
+                                          int64_t off, bool live, int D,
+                                          int vec) {
+  const int h = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int s = 0; s < N; ++s)
+    f[s] = load_chunk<float>((const float*)((const char*)base + off),
+                             4 * (s >> 1) + 2 * h + (s & 1), D, live, vec);
+}
+
+// An MFMA operand of own rows: load_row of every plane.
+template <typename P, int N>
+__device__ __forceinline__ void load_frags(u32x4 (&f)[P::kPlanes][N],
+                                           const typename P::S* base,
+                                           int64_t sp, int64_t off, bool live,
+                                           int D, int vec) {
+#pragma unroll
+  for (int p = 0; p < P::kPlanes; ++p)
+    load_row(f[p], base + p * sp, off, live, D, vec || P::kPlanes > 1);
+}
+
 // Every wave's staged data (and LDS reads) done, then the barrier.
 __device__ __forceinline__ void stage_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -379,9 +416,11 @@ __device__ __forceinline__ void stage_barrier() {
 // staged tile for the two ways it is read: row operand (16-byte chunks of
 // row c) and transposed operand of accum().
 // --------------------------------------------------------------------------
-template <typename T> struct Mma;
-
-template <> struct Mma<__bf16> {
+// bf16 tensors: one plane.
+struct Bf16 {
+  using T = __bf16;                 // of the tensors
+  using S = __bf16;                 // staged
+  static constexpr int kPlanes = 1;
   template <int CH> __device__ __forceinline__ static int cols() {
     const int lane = threadIdx.x & 63;
     const int row = 4 * (lane >> 5) + ((lane >> 2) & 3);
@@ -394,9 +433,26 @@ template <> struct Mma<__bf16> {
         __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
         0);
   }
-  // acc[blk] += tile^T p: 32 rows of the tile are the K index, in the
-  // accumulator's row order.  FINE: p as the sum of two bf16 terms.
-  template <int DP, bool FINE = false>
+  // Transposed operand: columns of block k, rows of K half c.
+  template <int CH>
+  __device__ __forceinline__ static bf16x8 col_frag(const DGMC_LDS char* tile,
+                                                    int cols, int c, int k) {
+    i16x4 v[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = 16 * c + 8 * i;
+      v[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (DGMC_LDS i16x4*)(tile + (cols ^ swz_xor<CH>(row, 4 * k)) +
+                            row * CH * 16));
+    }
+    const i16x8 both = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5,
+                                               6, 7);
+    return __builtin_bit_cast(bf16x8, both);
+  }
+  // acc[blk] += tile^T p: 32 rows of the tile (planes of ROWS rows) are the K
+  // index, in the accumulator's row order.  FINE: p as the sum of two bf16
+  // terms.
+  template <int DP, int ROWS, bool FINE = false>
   __device__ __forceinline__ static void accum(f32x16 (&acc)[DP / 32],
                                                const DGMC_LDS char* tile,
                                                int cols, f32x16 p) {
@@ -413,21 +469,12 @@ template <> struct Mma<__bf16> {
       }
 #pragma unroll
       for (int k = 0; k < DP / 32; ++k) {
-        i16x4 v[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = 16 * c + 8 * i;
-          v[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (DGMC_LDS i16x4*)(tile + (cols ^ swz_xor<CH>(row, 4 * k)) +
-                                row * CH * 16));
-        }
-        const i16x8 both = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4,
-                                                   5, 6, 7);
-        acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            __builtin_bit_cast(bf16x8, both), b, acc[k], 0, 0, 0);
+        const bf16x8 a = col_frag<CH>(tile, cols, c, k);
+        acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc[k], 0, 0,
+                                                         0);
         if constexpr (FINE)
-          acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              __builtin_bit_cast(bf16x8, both), lo_b, acc[k], 0, 0, 0);
+          acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, lo_b, acc[k], 0,
+                                                           0, 0);
       }
     }
   }
@@ -461,7 +508,11 @@ template <> struct Mma<__bf16> {
   }
 };
 
-template <> struct Mma<float> {
+// fp32 tensors, exact products.
+struct F32 {
+  using T = float;
+  using S = float;
+  static constexpr int kPlanes = 1;
   template <int CH> __device__ __forceinline__ static int cols() {
     const int lane = threadIdx.x & 63, row = 4 * (lane >> 5), d = lane & 31;
     return row * CH * 16 + (((d >> 2) ^ swz<CH>(row)) * 16) + 4 * (d & 3);
@@ -474,7 +525,7 @@ template <> struct Mma<float> {
       c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
     return c;
   }
-  template <int DP, bool FINE = false>
+  template <int DP, int ROWS, bool FINE = false>
   __device__ __forceinline__ static void accum(f32x16 (&acc)[DP / 32],
                                                const DGMC_LDS char* tile,
                                                int cols, f32x16 p) {
@@ -505,21 +556,84 @@ template <> struct Mma<float> {
   }
 };
 
+// Terms of an x6 product, the smallest first: lo hi, hi lo, mid mid, mid hi,
+// hi mid, hi hi.
+__host__ __device__ constexpr int x6_a(int t) {
+  return t == 0 ? 2 : t == 2 || t == 3 ? 1 : 0;
+}
+__host__ __device__ constexpr int x6_b(int t) {
+  return t == 1 ? 2 : t == 2 || t == 4 ? 1 : 0;
+}
+
+// fp32 tensors in three bf16 planes.
+struct X6 {
+  using T = float;
+  using S = __bf16;
+  static constexpr int kPlanes = 3;
+  template <int CH> __device__ __forceinline__ static int cols() {
+    return Bf16::cols<CH>();
+  }
+  template <int DP, int ROWS, bool FINE = false>
+  __device__ __forceinline__ static void accum(f32x16 (&acc)[DP / 32],
+                                               const DGMC_LDS char* tile,
+                                               int cols, f32x16 p) {
+    constexpr int CH = DP / 8;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      bf16x8 b[3];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = p[8 * c + i];
+        b[0][i] = (__bf16)x;
+        const float r = x - (float)b[0][i];
+        b[1][i] = (__bf16)r;
+        b[2][i] = (__bf16)(r - (float)b[1][i]);
+      }
+#pragma unroll
+      for (int k = 0; k < DP / 32; ++k) {
+        bf16x8 a[3];
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+          a[q] = Bf16::col_frag<CH>(tile + q * ROWS * CH * 16, cols, c, k);
+#pragma unroll
+        for (int t = 0; t < 6; ++t)
+          acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              a[x6_a(t)], b[x6_b(t)], acc[k], 0, 0, 0);
+      }
+    }
+  }
+  template <bool FINE>
+  __device__ __forceinline__ static float sum(f32x16 p, float l) {
+    return F32::sum<FINE>(p, l);
+  }
+};
+
 // Row operand: chunks h, h + 2, .. of row c of a staged block of 32 rows.
 template <int CH>
 __device__ __forceinline__ int row_base() {
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   return c * CH * 16 + ((h ^ swz<CH>(c)) * 16);
 }
-template <typename T, int CH>
-__device__ __forceinline__ f32x16 row_dot(const DGMC_LDS char* tile, int rows,
-                                          const u32x4 (&f)[CH / 2]) {
-  f32x16 acc = Mma<T>::dot(*(const DGMC_LDS u32x4*)(tile + rows), f[0],
-                           f32x16{});
+template <typename P, int CH, int ROWS>
+__device__ __forceinline__ f32x16 row_dot(
+    const DGMC_LDS char* tile, int rows,
+    const u32x4 (&f)[P::kPlanes][CH / 2]) {
+  f32x16 acc = {};
 #pragma unroll
-  for (int s = 1; s < CH / 2; ++s)
-    acc = Mma<T>::dot(*(const DGMC_LDS u32x4*)(tile + (rows ^ (32 * s))),
-                      f[s], acc);
+  for (int s = 0; s < CH / 2; ++s) {
+    u32x4 a[P::kPlanes];
+#pragma unroll
+    for (int p = 0; p < P::kPlanes; ++p)
+      a[p] = *(const DGMC_LDS u32x4*)(tile + (rows ^ (32 * s)) +
+                                      p * ROWS * CH * 16);
+    if constexpr (P::kPlanes == 1) {
+      acc = P::dot(a[0], f[0][s], acc);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 6; ++t)
+        acc = Bf16::dot(a[x6_a(t)], f[x6_b(t)][s], acc);
+    }
+  }
   return acc;
 }
 
@@ -601,11 +715,10 @@ __device__ __forceinline__ float load_pos(const int* pos, int64_t i, int axes,
   return (float)min(max(p, -(1 << 23)), 1 << 23);
 }
 
-// Keys of a forward tile: 64 while both buffers of K and V fit 64 KB of LDS
-// (128 KB at dim 128, fp32: 32).
-inline int fwd_keys(int D, int nw, bool f32) {
-  const int DP = D <= 32 ? 32 : D <= 64 ? 64 : 128;
-  return nw > 1 && DP * (f32 ? 4 : 2) <= 256 ? 64 : 32;
+// Keys of a forward tile: 64 where four waves share it and both buffers of K
+// and V stay within 64 KB of LDS.
+constexpr int fwd_keys(int DP, int nw, int row_bytes) {
+  return nw > 1 && DP * row_bytes <= 256 ? 64 : 32;
 }
 
 // Dynamic LDS past 64 KB has to be asked for.

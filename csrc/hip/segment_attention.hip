@@ -10,10 +10,56 @@ namespace segattn {
 void fwd_bf16(const Args& a, int axes, int nw, hipStream_t st);
 void fwd_bf16_fine(const Args& a, int axes, int nw, hipStream_t st);
 void fwd_f32(const Args& a, int axes, int nw, hipStream_t st);
+void fwd_x6(const Args& a, int axes, hipStream_t st);
 void dq_bf16(const Args& a, int axes, int nw, int nblk, hipStream_t st);
 void dq_f32(const Args& a, int axes, int nw, int nblk, hipStream_t st);
+void dq_x6(const Args& a, int axes, int nblk, hipStream_t st);
 void dkv_bf16(const Args& a, int axes, int nw, hipStream_t st);
 void dkv_f32(const Args& a, int axes, int nw, hipStream_t st);
+void dkv_x6(const Args& a, int axes, hipStream_t st);
+
+// fp32 [N, heads, D] tensors -> bf16 planes [3][N][heads][D8] (hi, mid, lo;
+// D8: D rounded up to 8, zeros behind D), 8 values a thread.
+struct Planes {
+  const float* src[4];
+  __bf16* dst[4];
+  int64_t sn[4], sh[4], n[4];       // strides, N * heads * D8 / 8
+  int heads[4];
+  int D;
+};
+
+__global__ __launch_bounds__(256) void planes_kernel(const Planes p) {
+  const int t = blockIdx.y, c8 = (p.D + 7) / 8;
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= p.n[t]) return;
+  const int64_t row = e / c8;
+  const int d0 = (int)(e - row * c8) * 8;
+  const int64_t i = row / p.heads[t];
+  const int hd = (int)(row - i * p.heads[t]);
+  const float* src = p.src[t] + i * p.sn[t] + hd * p.sh[t];
+  float x[8];
+  if (d0 + 8 <= p.D && aligned16(src + d0)) {
+    load_vec<float, 4>(src + d0, x);
+    load_vec<float, 4>(src + d0 + 4, x + 4);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = d0 + k < p.D ? src[d0 + k] : 0.f;
+  }
+  bf16x8 v[3];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    __bf16 h, m, l;
+    split3_bf16(x[k], h, m, l);
+    // (the terms of inf and NaN stay in the first: inf - inf is NaN)
+    const bool fin = fabsf(x[k]) < INFINITY;
+    v[0][k] = h;
+    v[1][k] = fin ? m : (__bf16)0.f;
+    v[2][k] = fin ? l : (__bf16)0.f;
+  }
+#pragma unroll
+  for (int q = 0; q < 3; ++q)
+    *(bf16x8*)(p.dst[t] + (q * p.n[t] + e) * 8) = v[q];
+}
 
 constexpr int kMaxSplits = 512;
 
@@ -287,6 +333,50 @@ static int waves_for(int64_t rows, int64_t B) {
   return rows > 64 * std::max<int64_t>(B, 1) ? 4 : 1;
 }
 
+// Whether an fp32 call takes the x6 kernels: long segments on both sides (the
+// planes cost a pass over the tensors and 1.5 times their memory), heads of
+// up to 64 (wider ones' planes exceed the LDS beside the table's columns).
+static bool takes_x6(const Args& a, bool x6) {
+  return x6 && a.D <= 64 && waves_for((int64_t)a.Nq * a.G, a.B) == 4 &&
+         waves_for(a.Nk, a.B) == 4;
+}
+
+// Points q, k, v (and dout) of `a` to their planes; `ws` keeps them alive.
+static at::Tensor make_planes(Args& a, bool with_dout,
+                              const at::Tensor& like) {
+  const int64_t D8 = (a.D + 7) / 8 * 8;
+  const int64_t nq = (int64_t)a.Nq * a.H * D8, nk = (int64_t)a.Nk * a.KV * D8;
+  at::Tensor ws = at::empty({3 * (nq * (with_dout ? 2 : 1) + 2 * nk)},
+                            like.options().dtype(at::kBFloat16));
+  __bf16* w = (__bf16*)ws.data_ptr();
+  Planes p = {};
+  p.D = a.D;
+  int64_t most = 0;
+  auto add = [&](int t, const void*& ptr, int64_t& sn, int64_t& sh,
+                 int64_t& sp, int64_t n, int heads) {
+    p.src[t] = (const float*)ptr;
+    p.dst[t] = w;
+    p.sn[t] = sn;
+    p.sh[t] = sh;
+    p.n[t] = n / 8;
+    p.heads[t] = heads;
+    most = std::max(most, n / 8);
+    ptr = w;
+    sn = heads * D8;
+    sh = D8;
+    sp = n;
+    w += 3 * n;
+  };
+  add(0, a.q, a.q_sn, a.q_sh, a.q_sp, nq, a.H);
+  add(1, a.k, a.k_sn, a.k_sh, a.k_sp, nk, a.KV);
+  add(2, a.v, a.v_sn, a.v_sh, a.v_sp, nk, a.KV);
+  if (with_dout) add(3, a.dout, a.g_sn, a.g_sh, a.g_sp, nq, a.H);
+  planes_kernel<<<dim3((unsigned)((most + 255) / 256), with_dout ? 4 : 3), 256,
+                  0, stream()>>>(p);
+  DGMC_CHECK_LAUNCH();
+  return ws;
+}
+
 // Splits of the other axis (`n` rows in tiles of `tile`) where the `tiles`
 // of the own axis are too few or too uneven to fill the chip: up to 1024
 // workgroups, no split under kChunk tiles.  False: none.
@@ -304,7 +394,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> forward(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& ptr_q, const at::Tensor& ptr_k, double scale,
     double cap, const OptTensor& bias, const OptTensor& pos_q,
-    const OptTensor& pos_k, const BucketLayout& layout, bool train) {
+    const OptTensor& pos_k, const BucketLayout& layout, bool x6,
+    bool train) {
   int axes;
   Args a = make_args(q, k, v, ptr_q, ptr_k, scale, cap, bias, pos_q, pos_k,
                      layout, axes);
@@ -320,7 +411,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> forward(
   a.out_lo = fine ? lo.data_ptr() : nullptr;
   a.lse = train ? lse.data_ptr<float>() : nullptr;
   const int nw = waves_for((int64_t)a.Nq * a.G, a.B);
-  const int TQ = 32 / a.G * nw, KT = fwd_keys(a.D, nw, f);
+  const bool six = f && takes_x6(a, x6);
+  const int DP = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
+  const int TQ = 32 / a.G * nw,
+            KT = fwd_keys(DP, nw, six ? 6 : f ? 4 : 2);
+  at::Tensor ws;
+  if (six) ws = make_planes(a, false, q);
   at::Tensor po, pml;
   if (split_axis(a, a.Nq / TQ, a.Nk, KT)) {
     po = at::empty({a.splits, a.Nq, a.H, a.D}, f32);
@@ -328,7 +424,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> forward(
     a.part_o = po.data_ptr<float>();
     a.part_ml = pml.data_ptr<float>();
   }
-  f      ? fwd_f32(a, axes, nw, stream())
+  six    ? fwd_x6(a, axes, stream())
+  : f    ? fwd_f32(a, axes, nw, stream())
   : fine ? fwd_bf16_fine(a, axes, nw, stream())
          : fwd_bf16(a, axes, nw, stream());
   if (a.splits > 1) join<FWD>(a, f, TQ, KT);
@@ -340,7 +437,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
     const at::Tensor& v, const at::Tensor& out, const at::Tensor& lo,
     const at::Tensor& lse, const at::Tensor& ptr_q, const at::Tensor& ptr_k,
     double scale, double cap, const OptTensor& bias, const OptTensor& pos_q,
-    const OptTensor& pos_k, const BucketLayout& layout) {
+    const OptTensor& pos_k, const BucketLayout& layout, bool x6) {
   int axes;
   Args a = make_args(q, k, v, ptr_q, ptr_k, scale, cap, bias, pos_q, pos_k,
                      layout, axes);
@@ -385,7 +482,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
   const int nwq = waves_for((int64_t)a.Nq * a.G, a.B);
   const int nwk = waves_for(a.Nk, a.B);
   const int TQ = 32 / a.G * nwq;
-  at::Tensor pq, pk;
+  const bool six = f && takes_x6(a, x6);
+  at::Tensor pq, pk, ws;
+  if (six) ws = make_planes(a, true, q);
   if (split_axis(a, a.Nq / TQ, a.Nk, 32)) {
     pq = at::empty({a.splits, a.Nq, a.H, a.D}, f32);
     a.part_o = pq.data_ptr<float>();
@@ -400,15 +499,18 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
     part = at::empty({nblk, a.KV, a.G, a.slots}, f32);
     a.part_bias = part.data_ptr<float>();
   }
-  f ? dq_f32(a, axes, nwq, nblk, stream())
-    : dq_bf16(a, axes, nwq, nblk, stream());
+  six ? dq_x6(a, axes, nblk, stream())
+  : f ? dq_f32(a, axes, nwq, nblk, stream())
+      : dq_bf16(a, axes, nwq, nblk, stream());
   if (a.splits > 1) join<DQ>(a, f, TQ, 32);
   if (a.Nk > 0) {
     if (split_axis(a, a.Nk / (32 * nwk), a.Nq, 32 / a.G)) {
       pk = at::empty({2, a.splits, a.Nk, a.KV, a.D}, f32);
       a.part_o = pk.data_ptr<float>();
     }
-    f ? dkv_f32(a, axes, nwk, stream()) : dkv_bf16(a, axes, nwk, stream());
+    six ? dkv_x6(a, axes, stream())
+    : f ? dkv_f32(a, axes, nwk, stream())
+        : dkv_bf16(a, axes, nwk, stream());
     if (a.splits > 1) join<DKV>(a, f, 32 * nwk, 32 / a.G);
   }
   if (axes) {

@@ -48,13 +48,16 @@ __device__ __forceinline__ void add_slots(DGMC_LDS float* hist,
   hist[d * 64] = hd + vd;
 }
 
-template <typename T, int DP, int NW, int POS>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(
-    const Args a, int ntiles) {
+template <typename P, int DP, int NW, int POS>
+__global__ __launch_bounds__(
+    NW * 64, sizeof(typename P::S) == 2 ? 2 : 1) void
+dq_kernel(const Args a, int ntiles) {
+  using T = typename P::T;
+  using S = typename P::S;
   constexpr int KT = 32;
-  constexpr int CH = DP * (int)sizeof(T) / 16;
+  constexpr int CH = DP * (int)sizeof(S) / 16;
   constexpr int NT = NW * 64;
-  constexpr int TB = KT * CH * 16;
+  constexpr int TB = P::kPlanes * KT * CH * 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   DGMC_LDS char* lds = (DGMC_LDS char*)smem;
   DGMC_LDS float* kpos = (DGMC_LDS float*)(lds + 4 * TB);   // [2][2][KT]
@@ -75,12 +78,12 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(
     load_table(a, kvh, tab, POS);
     for (int s = 0; s < a.slots; ++s) myhist[s * 64] = 0.f;
   }
-  const T* kbase = (const T*)a.k + (int64_t)kvh * a.k_sh;
-  const T* vbase = (const T*)a.v + (int64_t)kvh * a.v_sh;
+  const S* kbase = (const S*)a.k + (int64_t)kvh * a.k_sh;
+  const S* vbase = (const S*)a.v + (int64_t)kvh * a.v_sh;
   const bool capped = a.cap > 0.f;
   const float s1 = capped ? a.scale / a.cap : a.scale * kLog2e;
   const float s2 = a.cap * kLog2e;
-  const int rows0 = row_base<CH>(), cols0 = Mma<T>::template cols<CH>();
+  const int rows0 = row_base<CH>(), cols0 = P::template cols<CH>();
 
   for (int it = blk; it < ntiles * a.splits; it += nblk) {
     const int split = it % a.splits;
@@ -88,17 +91,17 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(
     const int qi = q_lo + qo;
     const bool live = c < QW * a.G && qi < q_hi;
     const int64_t row = (int64_t)qi * a.H + head;
-    u32x4 qf[CH / 2], gf[CH / 2];
-    load_frags<T>(qf,
-                  (const T*)a.q + (int64_t)q_lo * a.q_sn +
+    u32x4 qf[P::kPlanes][CH / 2], gf[P::kPlanes][CH / 2];
+    load_frags<P>(qf,
+                  (const S*)a.q + (int64_t)q_lo * a.q_sn +
                       (int64_t)kvh * a.G * a.q_sh,
-                  (qo * a.q_sn + g * a.q_sh) * (int64_t)sizeof(T), live, a.D,
-                  a.vec_q);
-    load_frags<T>(gf,
-                  (const T*)a.dout + (int64_t)q_lo * a.g_sn +
+                  a.q_sp, (qo * a.q_sn + g * a.q_sh) * (int64_t)sizeof(S),
+                  live, a.D, a.vec_q);
+    load_frags<P>(gf,
+                  (const S*)a.dout + (int64_t)q_lo * a.g_sn +
                       (int64_t)kvh * a.G * a.g_sh,
-                  (qo * a.g_sn + g * a.g_sh) * (int64_t)sizeof(T), live, a.D,
-                  a.vec_g);
+                  a.g_sp, (qo * a.g_sn + g * a.g_sh) * (int64_t)sizeof(S),
+                  live, a.D, a.vec_g);
     const int wrows = min(QW, q_hi - q_lo - wave * QW);
     const Rows w =
         Rows::find<NW>(a.ptr_q, a.ptr_k, a.B, a.Nq, a.Nk, q_lo, q_hi, qi,
@@ -114,15 +117,34 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(
     {
       const int64_t ob = ((int64_t)q_lo * a.H + kvh * a.G) * a.D;
       const int64_t oo = ((int64_t)qo * a.H + g) * a.D * (int64_t)sizeof(T);
-      u32x4 of[CH / 2];
-      load_frags<T>(of, (const T*)a.o + ob, oo, live, a.D, a.vec_o);
-#pragma unroll
-      for (int s = 0; s < CH / 2; ++s) dl += Mma<T>::chunk_dot(gf[s], of[s]);
-      if constexpr (sizeof(T) == 2) {
-        load_frags<T>(of, (const T*)a.out_lo + ob, oo, live, a.D, a.vec_o);
+      if constexpr (P::kPlanes > 1) {
+        // (the planes' sum is the value)
+        u32x4 of[CH];
+        load_row8(of, (const T*)a.o + ob, oo, live, a.D, a.vec_o);
 #pragma unroll
         for (int s = 0; s < CH / 2; ++s)
-          dl += Mma<T>::chunk_dot(gf[s], of[s]);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) {
+            const bf16x8 x = __builtin_bit_cast(bf16x8, gf[2 - p][s]);
+            const f32x4 y0 = __builtin_bit_cast(f32x4, of[2 * s]),
+                        y1 = __builtin_bit_cast(f32x4, of[2 * s + 1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              dl = fmaf((float)x[i], y0[i], dl);
+              dl = fmaf((float)x[4 + i], y1[i], dl);
+            }
+          }
+      } else {
+        u32x4 of[CH / 2];
+        load_row(of, (const T*)a.o + ob, oo, live, a.D, a.vec_o);
+#pragma unroll
+        for (int s = 0; s < CH / 2; ++s) dl += P::chunk_dot(gf[0][s], of[s]);
+        if constexpr (sizeof(T) == 2) {
+          load_row(of, (const T*)a.out_lo + ob, oo, live, a.D, a.vec_o);
+#pragma unroll
+          for (int s = 0; s < CH / 2; ++s)
+            dl += P::chunk_dot(gf[0][s], of[s]);
+        }
       }
     }
     dl = sum_half(dl);
@@ -136,14 +158,14 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(
 
     float pr[2] = {0.f, 0.f};
     auto fetch = [&](int k0, int e, int buf) {
-      using S = Stager<T, KT, CH, NT>;
+      using St = Stager<P, KT, CH, NT>;
       const int left = e - k0;
       DGMC_LDS char* kt = lds + buf * 2 * TB;
       const auto ok = [&](int r) { return r < left; };
-      S::fill(kbase + (int64_t)k0 * a.k_sn, a.D, a.vec_k, kt, ok,
-              [&](int r) { return r * (a.k_sn * (int)sizeof(T)); });
-      S::fill(vbase + (int64_t)k0 * a.v_sn, a.D, a.vec_v, kt + TB, ok,
-              [&](int r) { return r * (a.v_sn * (int)sizeof(T)); });
+      St::fill(kbase + (int64_t)k0 * a.k_sn, a.k_sp, a.D, a.vec_k, kt, ok,
+               [&](int r) { return r * (a.k_sn * (int)sizeof(S)); });
+      St::fill(vbase + (int64_t)k0 * a.v_sn, a.v_sp, a.D, a.vec_v, kt + TB,
+               ok, [&](int r) { return r * (a.v_sn * (int)sizeof(S)); });
       if constexpr (POS > 0) {
         if (tid < KT && tid < left) {
           pr[0] = load_pos(a.pos_k, (int64_t)k0 + tid, POS, 0);
@@ -177,8 +199,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(
         if (w.skip(k0, KT)) continue;
         const int rows = lane_base<CH>(rows0 + buf * 2 * TB);
         const int cols = lane_base<CH>(cols0 + buf * 2 * TB);
-        f32x16 z = row_dot<T, CH>(lds, rows, qf);
-        const f32x16 dp = row_dot<T, CH>(lds + TB, rows, gf);
+        f32x16 z = row_dot<P, CH, KT>(lds, rows, qf);
+        const f32x16 dp = row_dot<P, CH, KT>(lds + TB, rows, gf);
         const bool whole = w.whole(k0, KT);
         const unsigned n = w.r_hi - w.r_lo;
         const int j0 = k0 + 4 * h - w.r_lo;
@@ -225,7 +247,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(
           for (int r = 0; r < 4; ++r)
             z[4 * r4 + r] = v[r] * fmaf(-t[r], t[r], 1.f);
         }
-        Mma<T>::template accum<DP>(acc, lds, cols, z);
+        P::template accum<DP, KT>(acc, lds, cols, z);
       }
       const bool redo = pass < w.b0 && w.b1 > w.b0 &&
                         any_lane<NW>(live && not_finite(acc));
@@ -260,13 +282,16 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dq_kernel(
   }
 }
 
-template <typename T, int DP, int NW, int POS>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(
-    const Args a) {
+template <typename P, int DP, int NW, int POS>
+__global__ __launch_bounds__(
+    NW * 64, sizeof(typename P::S) == 2 ? 2 : 1) void
+dkv_kernel(const Args a) {
+  using T = typename P::T;
+  using S = typename P::S;
   constexpr int QT = 32;                         // packed rows per tile
-  constexpr int CH = DP * (int)sizeof(T) / 16;
+  constexpr int CH = DP * (int)sizeof(S) / 16;
   constexpr int NT = NW * 64;
-  constexpr int TB = QT * CH * 16;
+  constexpr int TB = P::kPlanes * QT * CH * 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   DGMC_LDS char* lds = (DGMC_LDS char*)smem;
   DGMC_LDS float* rowv = (DGMC_LDS float*)(lds + 4 * TB);   // [2][4][QT]
@@ -280,15 +305,15 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(
   const int k_hi = min(k_lo + 32 * NW, a.Nk);
   const int ko = wave * 32 + c, kj = k_lo + ko;
   const bool live = kj < k_hi;
-  u32x4 kf[CH / 2], vf[CH / 2];
-  load_frags<T>(kf,
-                (const T*)a.k + (int64_t)k_lo * a.k_sn +
+  u32x4 kf[P::kPlanes][CH / 2], vf[P::kPlanes][CH / 2];
+  load_frags<P>(kf,
+                (const S*)a.k + (int64_t)k_lo * a.k_sn +
                     (int64_t)kvh * a.k_sh,
-                ko * a.k_sn * (int64_t)sizeof(T), live, a.D, a.vec_k);
-  load_frags<T>(vf,
-                (const T*)a.v + (int64_t)k_lo * a.v_sn +
+                a.k_sp, ko * a.k_sn * (int64_t)sizeof(S), live, a.D, a.vec_k);
+  load_frags<P>(vf,
+                (const S*)a.v + (int64_t)k_lo * a.v_sn +
                     (int64_t)kvh * a.v_sh,
-                ko * a.v_sn * (int64_t)sizeof(T), live, a.D, a.vec_v);
+                a.v_sp, ko * a.v_sn * (int64_t)sizeof(S), live, a.D, a.vec_v);
   const int wrows = min(32, k_hi - k_lo - wave * 32);
   const Rows w = Rows::find<NW>(a.ptr_k, a.ptr_q, a.B, a.Nk, a.Nq, k_lo, k_hi,
                                 kj, wrows > 0 ? wrows - 1 : -1);
@@ -310,22 +335,22 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(
     }
   }
 
-  const T* qbase = (const T*)a.q + (int64_t)kvh * a.G * a.q_sh;
-  const T* gbase = (const T*)a.dout + (int64_t)kvh * a.G * a.g_sh;
+  const S* qbase = (const S*)a.q + (int64_t)kvh * a.G * a.q_sh;
+  const S* gbase = (const S*)a.dout + (int64_t)kvh * a.G * a.g_sh;
   float rv[4] = {INFINITY, 0.f, 0.f, 0.f};
   auto fetch = [&](int q0, int e, int buf) {
-    using S = Stager<T, QT, CH, NT>;
+    using St = Stager<P, QT, CH, NT>;
     const int left = e - q0;
     DGMC_LDS char* qt = lds + buf * 2 * TB;
     const auto ok = [&](int r) { return r < RW && div_group(a, r) < left; };
     const auto off = [&](int r, int64_t sn, int64_t sh) {
       const int i = div_group(a, r);
-      return (i * sn + (r - i * a.G) * sh) * (int64_t)sizeof(T);
+      return (i * sn + (r - i * a.G) * sh) * (int64_t)sizeof(S);
     };
-    S::fill(qbase + (int64_t)q0 * a.q_sn, a.D, a.vec_q, qt, ok,
-            [&](int r) { return off(r, a.q_sn, a.q_sh); });
-    S::fill(gbase + (int64_t)q0 * a.g_sn, a.D, a.vec_g, qt + TB, ok,
-            [&](int r) { return off(r, a.g_sn, a.g_sh); });
+    St::fill(qbase + (int64_t)q0 * a.q_sn, a.q_sp, a.D, a.vec_q, qt, ok,
+             [&](int r) { return off(r, a.q_sn, a.q_sh); });
+    St::fill(gbase + (int64_t)q0 * a.g_sn, a.g_sp, a.D, a.vec_g, qt + TB, ok,
+             [&](int r) { return off(r, a.g_sn, a.g_sh); });
     if (tid < QT) {
       const int i = div_group(a, tid), qi = q0 + i;
       const bool there = tid < RW && qi < e;
@@ -348,7 +373,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(
   const bool capped = a.cap > 0.f;
   const float s1 = capped ? a.scale / a.cap : a.scale * kLog2e;
   const float s2 = a.cap * kLog2e;
-  const int rows0 = row_base<CH>(), cols0 = Mma<T>::template cols<CH>();
+  const int rows0 = row_base<CH>(), cols0 = P::template cols<CH>();
 
   // Passes as in the forward.
   for (int pass = w.b0 - 1;; ++pass) {
@@ -367,8 +392,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(
       const DGMC_LDS float* rw = rowv + buf * 4 * QT;
       const int rows = lane_base<CH>(rows0 + buf * 2 * TB);
       const int cols = lane_base<CH>(cols0 + buf * 2 * TB);
-      f32x16 z = row_dot<T, CH>(lds, rows, kf);
-      f32x16 dp = row_dot<T, CH>(lds + TB, rows, vf);
+      f32x16 z = row_dot<P, CH, QT>(lds, rows, kf);
+      f32x16 dp = row_dot<P, CH, QT>(lds + TB, rows, vf);
       const bool whole = w.whole(q0, QW);
       const unsigned n = (w.r_hi - w.r_lo) * a.G;
       const int j0 = (q0 - w.r_lo) * a.G + 4 * h;
@@ -419,8 +444,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(
           dp[4 * r4 + r] = ds[r] * fmaf(-t[r], t[r], 1.f);
         }
       }
-      Mma<T>::template accum<DP>(av, lds + TB, cols, z);
-      Mma<T>::template accum<DP>(ak, lds, cols, dp);
+      P::template accum<DP, QT>(av, lds + TB, cols, z);
+      P::template accum<DP, QT>(ak, lds, cols, dp);
     }
     const bool redo =
         pass < w.b0 && w.b1 > w.b0 &&
@@ -441,64 +466,34 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(
   }
 }
 
-template <typename T, int DP, int NW, int POS>
-void launch_dq(const Args& a, int nblk, hipStream_t st) {
+template <typename P, int DP, int NW>
+void launch_dq(const Args& a, int axes, int nblk, hipStream_t st) {
+  constexpr int B = P::kPlanes * (int)sizeof(typename P::S);
   const int TQ = 32 / a.G * NW, ntiles = (a.Nq + TQ - 1) / TQ;
-  const size_t sm = 4 * 32 * DP * sizeof(T) +
-                    (POS ? 16 * 32 + a.G * kSlots * 4 +
-                               (size_t)NW * a.slots * 256 : 0);
-  auto kern = dq_kernel<T, DP, NW, POS>;
+  const size_t sm = 4 * 32 * DP * B +
+                    (axes ? 16 * 32 + a.G * kSlots * 4 +
+                                (size_t)NW * a.slots * 256 : 0);
+  auto kern = axes == 0   ? dq_kernel<P, DP, NW, 0>
+              : axes == 1 ? dq_kernel<P, DP, NW, 1>
+                          : dq_kernel<P, DP, NW, 2>;
   allow_lds(reinterpret_cast<const void*>(kern), sm);
-  kern<<<dim3((POS ? nblk : ntiles * a.splits) * a.KV), dim3(NW * 64), sm,
+  kern<<<dim3((axes ? nblk : ntiles * a.splits) * a.KV), dim3(NW * 64), sm,
          st>>>(a, ntiles);
   DGMC_CHECK_LAUNCH();
 }
 
-template <typename T, int DP, int NW, int POS>
-void launch_dkv(const Args& a, hipStream_t st) {
-  const size_t sm = 4 * 32 * DP * sizeof(T) + 8 * 32 * 4 +
-                    (POS ? a.G * kSlots * 4 : 0);
-  auto kern = dkv_kernel<T, DP, NW, POS>;
+template <typename P, int DP, int NW>
+void launch_dkv(const Args& a, int axes, hipStream_t st) {
+  constexpr int B = P::kPlanes * (int)sizeof(typename P::S);
+  const size_t sm =
+      4 * 32 * DP * B + 8 * 32 * 4 + (axes ? a.G * kSlots * 4 : 0);
+  auto kern = axes == 0   ? dkv_kernel<P, DP, NW, 0>
+              : axes == 1 ? dkv_kernel<P, DP, NW, 1>
+                          : dkv_kernel<P, DP, NW, 2>;
   allow_lds(reinterpret_cast<const void*>(kern), sm);
   kern<<<dim3((a.Nk + 32 * NW - 1) / (32 * NW) * a.KV, a.splits),
          dim3(NW * 64), sm, st>>>(a);
   DGMC_CHECK_LAUNCH();
-}
-
-template <typename T, int DP, int NW>
-void dq_axes(const Args& a, int axes, int nblk, hipStream_t st) {
-  axes == 0   ? launch_dq<T, DP, NW, 0>(a, nblk, st)
-  : axes == 1 ? launch_dq<T, DP, NW, 1>(a, nblk, st)
-              : launch_dq<T, DP, NW, 2>(a, nblk, st);
-}
-template <typename T, int DP, int NW>
-void dkv_axes(const Args& a, int axes, hipStream_t st) {
-  axes == 0   ? launch_dkv<T, DP, NW, 0>(a, st)
-  : axes == 1 ? launch_dkv<T, DP, NW, 1>(a, st)
-              : launch_dkv<T, DP, NW, 2>(a, st);
-}
-template <typename T>
-void run_dq(const Args& a, int axes, int nw, int nblk, hipStream_t st) {
-  if (a.D <= 32)
-    nw == 1 ? dq_axes<T, 32, 1>(a, axes, nblk, st)
-            : dq_axes<T, 32, 4>(a, axes, nblk, st);
-  else if (a.D <= 64)
-    nw == 1 ? dq_axes<T, 64, 1>(a, axes, nblk, st)
-            : dq_axes<T, 64, 4>(a, axes, nblk, st);
-  else
-    nw == 1 ? dq_axes<T, 128, 1>(a, axes, nblk, st)
-            : dq_axes<T, 128, 4>(a, axes, nblk, st);
-}
-
-template <typename T>
-void run_dkv(const Args& a, int axes, int nw, hipStream_t st) {
-  if (a.D <= 32)
-    nw == 1 ? dkv_axes<T, 32, 1>(a, axes, st) : dkv_axes<T, 32, 4>(a, axes, st);
-  else if (a.D <= 64)
-    nw == 1 ? dkv_axes<T, 64, 1>(a, axes, st) : dkv_axes<T, 64, 4>(a, axes, st);
-  else
-    nw == 1 ? dkv_axes<T, 128, 1>(a, axes, st)
-            : dkv_axes<T, 128, 4>(a, axes, st);
 }
 
 }  // namespace segattn

@@ -1,0 +1,11 @@
+// Segment attention backward, dq: fp32 in three bf16 planes.
+#include "segment_attention_bwd.h"
+
+namespace dgmc {
+namespace segattn {
+void dq_x6(const Args& a, int axes, int nblk, hipStream_t st) {
+  a.D <= 32 ? launch_dq<X6, 32, 4>(a, axes, nblk, st)
+            : launch_dq<X6, 64, 4>(a, axes, nblk, st);
+}
+}  // namespace segattn
+}  // namespace dgmc

@@ -21,13 +21,20 @@
 namespace dgmc {
 namespace segattn {
 
-template <typename T, int DP, int NW, int KT, int POS, bool FINE>
-__global__ __launch_bounds__(
-    NW * 64, sizeof(T) == 2 ? (DP <= 64 ? 4 : 2) : 1) void
-fwd_kernel(const Args a) {
-  constexpr int CH = DP * (int)sizeof(T) / 16;   // 16-byte chunks per row
+// Waves per SIMD the registers are cut to.
+template <typename P>
+constexpr int fwd_waves(int DP) {
+  return P::kPlanes > 1 ? 2 : sizeof(typename P::S) == 2 ? DP <= 64 ? 4 : 2 : 1;
+}
+
+template <typename P, int DP, int NW, int KT, int POS, bool FINE>
+__global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
+    const Args a) {
+  using T = typename P::T;
+  using S = typename P::S;
+  constexpr int CH = DP * (int)sizeof(S) / 16;   // 16-byte chunks per row
   constexpr int NT = NW * 64;
-  constexpr int TB = KT * CH * 16;               // bytes of one tile
+  constexpr int TB = P::kPlanes * KT * CH * 16;  // bytes of one tile
   constexpr int UB = 32 * CH * 16;               // bytes of 32 rows
   extern __shared__ __attribute__((aligned(16))) char smem[];
   DGMC_LDS char* lds = (DGMC_LDS char*)smem;
@@ -45,12 +52,12 @@ fwd_kernel(const Args a) {
   const int qo = wave * QW + cq, qi = q_lo + qo;
   const bool live = c < QW * a.G && qi < q_hi;
   const int head = kvh * a.G + g;
-  u32x4 qf[CH / 2];
-  load_frags<T>(qf,
-                (const T*)a.q + (int64_t)q_lo * a.q_sn +
+  u32x4 qf[P::kPlanes][CH / 2];
+  load_frags<P>(qf,
+                (const S*)a.q + (int64_t)q_lo * a.q_sn +
                     (int64_t)kvh * a.G * a.q_sh,
-                (qo * a.q_sn + g * a.q_sh) * (int64_t)sizeof(T), live, a.D,
-                a.vec_q);
+                a.q_sp, (qo * a.q_sn + g * a.q_sh) * (int64_t)sizeof(S), live,
+                a.D, a.vec_q);
   const int wrows = min(QW, q_hi - q_lo - wave * QW);
   const Rows w = Rows::find<NW>(a.ptr_q, a.ptr_k, a.B, a.Nq, a.Nk, q_lo, q_hi,
                                 qi, wrows > 0 ? (wrows - 1) * a.G : -1);
@@ -73,21 +80,20 @@ fwd_kernel(const Args a) {
   const DGMC_LDS float* mytab = tab + g * kSlots;
   const int W = 2 * a.half + 2;
 
-  const T* kbase = (const T*)a.k + (int64_t)kvh * a.k_sh;
-  const T* vbase = (const T*)a.v + (int64_t)kvh * a.v_sh;
+  const S* kbase = (const S*)a.k + (int64_t)kvh * a.k_sh;
+  const S* vbase = (const S*)a.v + (int64_t)kvh * a.v_sh;
   float pr[2] = {0.f, 0.f};
   // Start the loads of keys [k0, e) into buffer `buf`; their positions wait
   // in registers.
   auto fetch = [&](int k0, int e, int buf) {
-    using S = Stager<T, KT, CH, NT>;
+    using St = Stager<P, KT, CH, NT>;
     const int left = e - k0;
     DGMC_LDS char* kt = lds + buf * 2 * TB;
     const auto ok = [&](int r) { return r < left; };
-    S::fill(kbase + (int64_t)k0 * a.k_sn, a.D, a.vec_k, kt, ok, [&](int r) {
-      return r * (a.k_sn * (int)sizeof(T));
-    });
-    S::fill(vbase + (int64_t)k0 * a.v_sn, a.D, a.vec_v, kt + TB, ok,
-            [&](int r) { return r * (a.v_sn * (int)sizeof(T)); });
+    St::fill(kbase + (int64_t)k0 * a.k_sn, a.k_sp, a.D, a.vec_k, kt, ok,
+             [&](int r) { return r * (a.k_sn * (int)sizeof(S)); });
+    St::fill(vbase + (int64_t)k0 * a.v_sn, a.v_sp, a.D, a.vec_v, kt + TB, ok,
+             [&](int r) { return r * (a.v_sn * (int)sizeof(S)); });
     if constexpr (POS > 0) {
       if (tid < KT && tid < left) {
         pr[0] = load_pos(a.pos_k, (int64_t)k0 + tid, POS, 0);
@@ -109,7 +115,7 @@ fwd_kernel(const Args a) {
   // Plain scores stay unscaled: 2^(s1 z - m) is one fma and one exp2.
   const bool plain = POS == 0 && a.cap <= 0.f && s1 > 0.f;
   const float ex = plain ? s1 : 1.f;
-  const int rows0 = row_base<CH>(), cols0 = Mma<T>::template cols<CH>();
+  const int rows0 = row_base<CH>(), cols0 = P::template cols<CH>();
 
   // Pass b0 - 1: all rows over all keys of the tile; passes b0 .. b1 (only
   // after a non-finite result): segment by segment.
@@ -132,7 +138,7 @@ fwd_kernel(const Args a) {
       f32x16 z[KT / 32];
 #pragma unroll
       for (int u = 0; u < KT / 32; ++u)
-        z[u] = row_dot<T, CH>(lds + u * UB, rows, qf);
+        z[u] = row_dot<P, CH, KT>(lds + u * UB, rows, qf);
       if (!plain) {
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u)
@@ -198,8 +204,8 @@ fwd_kernel(const Args a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           z[u][r] = exp2_(fmaf(z[u][r], ex, -ms));
-        l = Mma<T>::template sum<FINE>(z[u], l);
-        Mma<T>::template accum<DP, FINE>(acc, lds + TB + u * UB, cols, z[u]);
+        l = P::template sum<FINE>(z[u], l);
+        P::template accum<DP, KT, FINE>(acc, lds + TB + u * UB, cols, z[u]);
       }
     }
     l = sum_half(l);
@@ -241,33 +247,19 @@ fwd_kernel(const Args a) {
   }
 }
 
-template <typename T, int DP, int NW, bool FINE>
+template <typename P, int DP, int NW, bool FINE>
 void launch_fwd(const Args& a, int axes, hipStream_t st) {
-  constexpr int KT =                // (fwd_keys)
-      (NW > 1 && DP * (int)sizeof(T) <= 256) ? 64 : 32;
+  constexpr int B = P::kPlanes * (int)sizeof(typename P::S);
+  constexpr int KT = fwd_keys(DP, NW, B);
   const int TQ = 32 / a.G * NW;
   const dim3 grid((a.Nq + TQ - 1) / TQ * a.KV, a.splits), blk(NW * 64);
-  const size_t sm = 4 * KT * DP * sizeof(T) +
-                    (axes ? 16 * KT + a.G * kSlots * 4 : 0);
-  auto kern = axes == 0   ? fwd_kernel<T, DP, NW, KT, 0, FINE>
-              : axes == 1 ? fwd_kernel<T, DP, NW, KT, 1, FINE>
-                          : fwd_kernel<T, DP, NW, KT, 2, FINE>;
+  const size_t sm = 4 * KT * DP * B + (axes ? 16 * KT + a.G * kSlots * 4 : 0);
+  auto kern = axes == 0   ? fwd_kernel<P, DP, NW, KT, 0, FINE>
+              : axes == 1 ? fwd_kernel<P, DP, NW, KT, 1, FINE>
+                          : fwd_kernel<P, DP, NW, KT, 2, FINE>;
   allow_lds(reinterpret_cast<const void*>(kern), sm);
   kern<<<grid, blk, sm, st>>>(a);
   DGMC_CHECK_LAUNCH();
-}
-
-template <typename T, bool FINE>
-void run_fwd(const Args& a, int axes, int nw, hipStream_t st) {
-  if (a.D <= 32)
-    nw == 1 ? launch_fwd<T, 32, 1, FINE>(a, axes, st)
-            : launch_fwd<T, 32, 4, FINE>(a, axes, st);
-  else if (a.D <= 64)
-    nw == 1 ? launch_fwd<T, 64, 1, FINE>(a, axes, st)
-            : launch_fwd<T, 64, 4, FINE>(a, axes, st);
-  else
-    nw == 1 ? launch_fwd<T, 128, 1, FINE>(a, axes, st)
-            : launch_fwd<T, 128, 4, FINE>(a, axes, st);
 }
 
 }  // namespace segattn

@@ -1,10 +1,18 @@
-// bf16 instances of the segment attention forward.
+// Segment attention forward: bf16.
 #include "segment_attention_fwd.h"
 
 namespace dgmc {
 namespace segattn {
 void fwd_bf16(const Args& a, int axes, int nw, hipStream_t st) {
-  run_fwd<__bf16, false>(a, axes, nw, st);
+  if (a.D <= 32)
+    nw == 1 ? launch_fwd<Bf16, 32, 1, false>(a, axes, st)
+            : launch_fwd<Bf16, 32, 4, false>(a, axes, st);
+  else if (a.D <= 64)
+    nw == 1 ? launch_fwd<Bf16, 64, 1, false>(a, axes, st)
+            : launch_fwd<Bf16, 64, 4, false>(a, axes, st);
+  else
+    nw == 1 ? launch_fwd<Bf16, 128, 1, false>(a, axes, st)
+            : launch_fwd<Bf16, 128, 4, false>(a, axes, st);
 }
 }  // namespace segattn
 }  // namespace dgmc

@@ -1,10 +1,18 @@
-// bf16 instances of the segment attention forward, training form.
+// Segment attention forward: bf16, training.
 #include "segment_attention_fwd.h"
 
 namespace dgmc {
 namespace segattn {
 void fwd_bf16_fine(const Args& a, int axes, int nw, hipStream_t st) {
-  run_fwd<__bf16, true>(a, axes, nw, st);
+  if (a.D <= 32)
+    nw == 1 ? launch_fwd<Bf16, 32, 1, true>(a, axes, st)
+            : launch_fwd<Bf16, 32, 4, true>(a, axes, st);
+  else if (a.D <= 64)
+    nw == 1 ? launch_fwd<Bf16, 64, 1, true>(a, axes, st)
+            : launch_fwd<Bf16, 64, 4, true>(a, axes, st);
+  else
+    nw == 1 ? launch_fwd<Bf16, 128, 1, true>(a, axes, st)
+            : launch_fwd<Bf16, 128, 4, true>(a, axes, st);
 }
 }  // namespace segattn
 }  // namespace dgmc

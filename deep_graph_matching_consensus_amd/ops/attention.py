@@ -11,12 +11,15 @@ On the GPU one HIP kernel per direction walks the keys of each segment with
 the running softmax of ``csrc/hip/segment_attention.h``: the score matrix is
 never formed, the work list is derived from ``ptr`` on the device (no host
 copy; a captured graph may change ``ptr`` and the rows between replays) and
-every sum has a fixed order.  CPU tensors use the oracle in
-:mod:`.reference`.
+every sum has a fixed order.  fp32 calls on long segments run as "x6" (three
+bf16 terms an operand, six products, fp32 sums: ``DGMC_AMD_X6``, as in
+:mod:`.gemm`), short ones on exact fp32 products.  CPU tensors use the oracle
+in :mod:`.reference`.
 """
 import torch
 
 from . import _backend
+from . import gemm
 from . import reference as ref
 
 #: Distances from this on share a bucket in any layout.
@@ -179,4 +182,4 @@ def segment_attention(q, k, v, ptr_q, ptr_k=None, scale=None, cap=0.0,
         bias = bias.float().contiguous()
     return _backend.ops().segment_attention.default(
         q, k, v, bias, ptr_q.contiguous(), ptr_k.contiguous(), pos_q, pos_k,
-        scale, float(cap), *layout)
+        scale, float(cap), *layout, gemm.NT_X6)

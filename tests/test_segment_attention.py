@@ -186,6 +186,8 @@ SHAPES = [
     ([150], [140], 2, 2, 24),
     ([7, 9], None, 3, 1, 7),                 # unaligned rows
     ([129, 200], [66, 31], 1, 1, 128),
+    ([129, 0, 200], [266, 40, 131], 2, 1, 64),   # long on both sides
+    ([300], None, 3, 1, 20),
 ]
 
 
