@@ -132,9 +132,7 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
     Tensor dx = ds, dw, db;
     if (g[0].defined()) {
       std::tie(dx, dw, db) = layer_norm_bwd(
-          g[0].contiguous(),
-          ds.defined() ? OptTensor(ds.contiguous()) : OptTensor(), s[0], s[2],
-          opt(s[1]), s[1].defined());
+          g[0], opt(ds), s[0], s[2], opt(s[1]), s[1].defined());
       if (!s[1].defined()) dw = Tensor();
       if (!ctx->saved_data["bias"].toBool()) db = Tensor();
     }

@@ -39,8 +39,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
 
 }  // namespace segattn
 
-// x: contiguous [rows, C].  (y, s, stat): s is empty without a residual,
-// stat [rows, 2] (mean, rstd) empty unless `train`.
+// x: [..., C].  (y, s, stat): s is empty without a residual, stat [rows, 2]
+// (mean, rstd) empty unless `train`.
 std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd(
     const at::Tensor& x, const OptTensor& residual, const OptTensor& weight,
     const OptTensor& bias, double eps, bool train);

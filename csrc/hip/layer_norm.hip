@@ -298,34 +298,41 @@ void ln_width(bool vec, int C, F f) {
 // Rows of whole 16-byte vectors.
 bool ln_vec(const at::Tensor& t) {
   return t.numel() == 0 || (aligned16(t.data_ptr()) &&
-                            t.size(1) * t.element_size() % 16 == 0);
+                            t.size(-1) * t.element_size() % 16 == 0);
 }
 
 void ln_check(const at::Tensor& t, const at::Tensor& x, const char* name) {
   TORCH_CHECK(t.device() == x.device() &&
-                  t.scalar_type() == x.scalar_type() &&
-                  t.sizes() == x.sizes() && t.is_contiguous(),
-              "layer_norm: ", name, " must be contiguous and like x");
+                  t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes(),
+              "layer_norm: ", name, " must be like x");
+}
+
+int64_t ln_cols(const at::Tensor& x) {
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= kLnMaxCols,
+              "layer_norm: x must be [..., 1 to ", kLnMaxCols, "]");
+  return x.size(-1);
 }
 
 void ln_check_w(const OptTensor& w, const at::Tensor& x) {
   TORCH_CHECK(!w.has_value() ||
                   (w->device() == x.device() &&
                    w->scalar_type() == at::kFloat && w->is_contiguous() &&
-                   w->dim() == 1 && w->size(0) == x.size(1)),
+                   w->dim() == 1 && w->size(0) == x.size(-1)),
               "layer_norm: weight and bias must be fp32 [columns]");
 }
 
 }  // namespace
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd(
-    const at::Tensor& x, const OptTensor& residual,
-    const OptTensor& weight,
-    const OptTensor& bias, double eps, bool train) {
-  TORCH_CHECK(x.dim() == 2 && x.size(1) >= 1 && x.size(1) <= kLnMaxCols,
-              "layer_norm: x must be [rows, 1 to ", kLnMaxCols, "]");
-  ln_check(x, x, "x");
-  if (residual.has_value()) ln_check(*residual, x, "residual");
+    const at::Tensor& x_in, const OptTensor& residual_in,
+    const OptTensor& weight, const OptTensor& bias, double eps, bool train) {
+  const int64_t C = ln_cols(x_in);
+  const at::Tensor x = x_in.contiguous();
+  OptTensor residual;
+  if (residual_in.has_value()) {
+    ln_check(*residual_in, x, "residual");
+    residual = residual_in->contiguous();
+  }
   ln_check_w(weight, x);
   ln_check_w(bias, x);
   TORCH_CHECK(weight.has_value() || !bias.has_value(),
@@ -334,9 +341,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd(
   at::Tensor y = at::empty_like(x);
   at::Tensor s = residual.has_value() ? at::empty_like(x)
                                       : at::empty({0}, x.options());
-  at::Tensor stat = at::empty({train ? x.size(0) : 0, 2},
-                              x.options().dtype(at::kFloat));
-  if (x.size(0) == 0) return {y, s, stat};
+  const int64_t rows = x.numel() / C;
+  at::Tensor stat =
+      at::empty({train ? rows : 0, 2}, x.options().dtype(at::kFloat));
+  if (rows == 0) return {y, s, stat};
   LnArgs a = {};
   a.x = x.data_ptr();
   a.y = y.data_ptr();
@@ -345,8 +353,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd(
   a.w = weight.has_value() ? weight->data_ptr<float>() : nullptr;
   a.b = bias.has_value() ? bias->data_ptr<float>() : nullptr;
   a.stat = train ? (float2*)stat.data_ptr<float>() : nullptr;
-  a.rows = x.size(0);
-  a.C = (int)x.size(1);
+  a.rows = rows;
+  a.C = (int)C;
   a.eps = (float)eps;
   const bool vec = ln_vec(x) && (!residual.has_value() || ln_vec(*residual));
   DGMC_DISPATCH_FLOAT(x.scalar_type(), T, [&] {
@@ -364,26 +372,28 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd(
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_bwd(
-    const at::Tensor& dy, const OptTensor& ds,
-    const at::Tensor& s, const at::Tensor& stat,
-    const OptTensor& weight, bool with_weight) {
-  TORCH_CHECK(s.dim() == 2 && s.size(1) >= 1 && s.size(1) <= kLnMaxCols,
-              "layer_norm: s must be [rows, 1 to ", kLnMaxCols, "]");
-  ln_check(s, s, "s");
+    const at::Tensor& dy_in, const OptTensor& ds_in, const at::Tensor& s_in,
+    const at::Tensor& stat, const OptTensor& weight, bool with_weight) {
+  const int C = (int)ln_cols(s_in);
+  const at::Tensor s = s_in.contiguous(), dy = dy_in.contiguous();
   ln_check(dy, s, "dy");
-  if (ds.has_value()) ln_check(*ds, s, "ds");
+  OptTensor ds;
+  if (ds_in.has_value()) {
+    ln_check(*ds_in, s, "ds");
+    ds = ds_in->contiguous();
+  }
+  const int64_t rows = s.numel() / C;
   ln_check_w(weight, s);
   TORCH_CHECK(stat.device() == s.device() && stat.is_contiguous() &&
                   stat.scalar_type() == at::kFloat && stat.dim() == 2 &&
-                  stat.size(0) == s.size(0) && stat.size(1) == 2,
+                  stat.size(0) == rows && stat.size(1) == 2,
               "layer_norm: stat must be fp32 [rows, 2]");
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(s.device());
   const auto f32 = s.options().dtype(at::kFloat);
-  const int C = (int)s.size(1);
   at::Tensor dx = at::empty_like(s);
   at::Tensor dw = at::empty({with_weight ? C : 0}, f32);
   at::Tensor db = at::empty({with_weight ? C : 0}, f32);
-  if (s.size(0) == 0) {
+  if (rows == 0) {
     dw.zero_();
     db.zero_();
     return {dx, dw, db};
@@ -395,7 +405,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_bwd(
   a.dx = dx.data_ptr();
   a.w = weight.has_value() ? weight->data_ptr<float>() : nullptr;
   a.stat = (float2*)stat.data_ptr<float>();
-  a.rows = s.size(0);
+  a.rows = rows;
   a.C = C;
   const bool vec = ln_vec(s) && ln_vec(dy) && (!ds.has_value() || ln_vec(*ds));
   at::Tensor part;

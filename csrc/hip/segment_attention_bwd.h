@@ -10,7 +10,10 @@
 // (writing delta on the way), dkv_kernel a key per column and walks the
 // packed query rows of the whole head group, so shared key heads need no
 // second reduction.  Each recomputes the scores: 7 products in place of 5,
-// against atomics on dq.
+// against atomics on dq.  P and dS enter their bf16 products rounded to bf16
+// (an error of the output's own rounding's size, averaged over the keys), on
+// short segments as two bf16 terms (no error to average there, and products
+// are not what takes the time).
 //
 // The table's gradient: every lane adds its dz into its own LDS column of
 // [slots][64] (no address is shared: no conflicts and a fixed order); a
@@ -247,7 +250,7 @@ dq_kernel(const Args a, int ntiles) {
           for (int r = 0; r < 4; ++r)
             z[4 * r4 + r] = v[r] * fmaf(-t[r], t[r], 1.f);
         }
-        P::template accum<DP, KT>(acc, lds, cols, z);
+        P::template accum<DP, KT, NW == 1>(acc, lds, cols, z);
       }
       const bool redo = pass < w.b0 && w.b1 > w.b0 &&
                         any_lane<NW>(live && not_finite(acc));
@@ -444,8 +447,8 @@ dkv_kernel(const Args a) {
           dp[4 * r4 + r] = ds[r] * fmaf(-t[r], t[r], 1.f);
         }
       }
-      P::template accum<DP, QT>(av, lds + TB, cols, z);
-      P::template accum<DP, QT>(ak, lds, cols, dp);
+      P::template accum<DP, QT, NW == 1>(av, lds + TB, cols, z);
+      P::template accum<DP, QT, NW == 1>(ak, lds, cols, dp);
     }
     const bool redo =
         pass < w.b0 && w.b1 > w.b0 &&

@@ -9,11 +9,12 @@
 // the output accumulators is skipped otherwise; P <= 2^8 changes no
 // relative rounding), the sum is kept per lane and joined once at the end.
 // P is rounded to bf16 for the bf16 product (fp32: not at all); maximum,
-// sum and outputs are fp32.  FINE (bf16, training): P enters as two bf16
-// terms and the rounding rest of the output is kept beside it, because the
-// backward's delta = <do, o> multiplies whole rows of P - its error does not
-// average out over the keys (the table's gradient would lose 2 of bf16's 8
-// bits).
+// sum and outputs are fp32.  FINE (bf16): P enters as two bf16 terms - in
+// training, where the rounding rest of the output is kept beside it too,
+// because the backward's delta = <do, o> multiplies whole rows of P and its
+// error does not average out over the keys (the table's gradient would lose
+// 2 of bf16's 8 bits); and on short segments, whose few keys average nothing
+// out and whose time is latency, not products.
 #pragma once
 
 #include "segment_attention.h"
@@ -234,7 +235,7 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = (T)(acc[k][4 * r4 + r] * inv);
             put4(orow, d, a.D, o);
-            if constexpr (FINE) {
+            if (FINE && a.out_lo) {
 #pragma unroll
               for (int r = 0; r < 4; ++r)
                 o[r] = (T)(acc[k][4 * r4 + r] * inv - (float)o[r]);

@@ -50,11 +50,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
     if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise ValueError('layer_norm takes fp32, bf16 and fp16, got '
                          '{}'.format(x.dtype))
-    flat = x.reshape(-1, C).contiguous()
-    res = None if residual is None else residual.reshape(-1, C).contiguous()
     weight, bias = (None if t is None else t.float().contiguous()
                     for t in (weight, bias))
-    out = _backend.ops().layer_norm.default(flat, res, weight, bias,
+    out = _backend.ops().layer_norm.default(x, residual, weight, bias,
                                             float(eps))
-    out = [t.view(x.shape) for t in out]
     return out[0] if residual is None else tuple(out)
