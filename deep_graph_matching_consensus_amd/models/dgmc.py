@@ -37,6 +37,7 @@ from ..ops import dense as dense_ops
 from ..ops.gemm import mixed_matmul
 from ..ops import relconv as relconv_ops
 from ..ops import sparse_corr
+from ..ops.logprob import match_log_probs
 from ..ops.plans import _IdentityCache
 from ..runtime import loopgrad
 from ..runtime.cache import forward_cache
@@ -155,8 +156,17 @@ class _FoldProduct(torch.autograd.Function):
         return gw1, gwf, gbf
 
 
+class _RawCandidates(object):
+    """Sparse-path candidate scores before the softmax (``DGMC.log_probs``),
+    packed ``[sum N_s, k]``."""
+
+    def __init__(self, S_hat_0, S_hat_L, S_idx):
+        self.S_hat_0, self.S_hat_L, self.S_idx = S_hat_0, S_hat_L, S_idx
+
+
 class _RawScores(object):
-    """Dense-path scores before the output softmax (``DGMC.objective``)."""
+    """Dense-path scores before the output softmax (``DGMC.objective``,
+    ``DGMC.log_probs``)."""
 
     def __init__(self, S_hat_0, S_hat_L, lay_s, lay_t):
         self.S_hat_0, self.S_hat_L = S_hat_0, S_hat_L
@@ -458,11 +468,10 @@ class DGMC(torch.nn.Module):
                     S_hat = hs @ ht.transpose(-1, -2)        # [B, N_s, N_t]
                 if two:
                     S_hat_0, S_hat = S_hat
-                    raw = dense_ops.softmax_nll_supported(S_hat, lay_s)
                 else:
-                    raw = raw and dense_ops.softmax_nll_supported(S_hat,
-                                                                  lay_s)
                     S_hat_0 = S_hat
+                raw = raw == 'scores' or (
+                    raw and dense_ops.softmax_nll_supported(S_hat, lay_s))
                 S_0 = None if raw else \
                     dense_ops.masked_softmax_packed(S_hat, lay_s, lay_t)
                 # Fused pair encoding: the transport kernel writes r_t
@@ -549,6 +558,7 @@ class DGMC(torch.nn.Module):
                 if device.type == 'cuda' and not is_reference_mode() else None
 
             S_hat = sparse_corr.gather_dot(hs, ht, S_idx, cand)  # [B,N_s,k]
+            S_hat_0 = S_hat
             S = S_hat.softmax(dim=-1)      # S_0 and step 0's S (one softmax)
             S_0 = lay_s.to_sparse(S)
             # psi_2's final Linear folded into the MLP's first layer, as in
@@ -614,6 +624,10 @@ class DGMC(torch.nn.Module):
                 S_hat = sparse_corr.consensus_update(
                     S_hat, lay_s.to_dense(o_s.to(f32)),
                     lay_t.to_dense(o_t.to(f32)), S_idx, self.mlp, cand)
+            if raw == 'scores':
+                return _RawCandidates(lay_s.to_sparse(S_hat_0),
+                                      lay_s.to_sparse(S_hat),
+                                      lay_s.to_sparse(S_idx))
             S_L = lay_s.to_sparse(S if (fused_soft or steps == 0) else
                                   S_hat.softmax(dim=-1))
             S_idx = lay_s.to_sparse(S_idx)
@@ -764,6 +778,58 @@ class DGMC(torch.nn.Module):
             loss_L, count, correct = self.loss_stats(S_L, y, mask)
             return loss_L + self.loss(S_0, y, mask=mask), count, correct
         return self.loss_stats(S_0, y, mask)
+
+    def log_probs(self, x_s, edge_index_s, edge_attr_s, batch_s, x_t,
+                  edge_index_t, edge_attr_t, batch_t, y_col=None, top=0):
+        r"""How sure the model is: log-probabilities of the given matches,
+        the rows' entropies and the best alternatives, for the initial and
+        the refined correspondences (an extension; inputs as in
+        :meth:`forward`).
+
+        They are computed from the scores in one pass
+        (:func:`~..ops.logprob.match_log_probs`): the probabilities of
+        :meth:`forward` are never formed, and a ``log`` of one that has
+        underflowed is not taken.
+
+        Args:
+            y_col (Tensor, optional): int64 ``[sum N_s]`` given target of
+                every source row (a target-graph column, as in
+                :meth:`objective`), -1 for none.
+            top (int): number of alternatives per row (sparse models: of the
+                candidates).
+
+        Returns ``(first, last)``, two
+        :class:`~..ops.logprob.MatchLogProbs`.  Sparse models: a given match
+        that is not among the row's candidates has ``-inf``."""
+        if self.normalization != 'softmax':
+            raise ValueError('log_probs needs the softmax normalization')
+        with forward_cache():
+            out = self._forward(x_s, edge_index_s, edge_attr_s, batch_s, x_t,
+                                edge_index_t, edge_attr_t, batch_t, None,
+                                raw='scores')
+        if y_col is None:
+            y_col = torch.full((x_s.size(0), ), -1, dtype=torch.long,
+                               device=x_s.device)
+        if isinstance(out, _RawScores):
+            lay_s, lay_t = out.lay_s, out.lay_t
+            # valid columns of every packed row (padding rows: graph B, none)
+            counts = torch.cat([lay_t.counts, lay_t.counts.new_zeros(1)])
+            n_cols = counts[lay_s.index // lay_s.N].to(torch.int32)
+            return tuple(match_log_probs(lay_s.to_sparse(S), y_col, n_cols,
+                                         top)
+                         for S in (out.S_hat_0, out.S_hat_L))
+        hit = (out.S_idx == y_col.view(-1, 1)) & (y_col.view(-1, 1) >= 0)
+        found = hit.any(dim=-1)
+        slot = torch.where(found, hit.to(torch.int8).argmax(dim=-1), -1)
+        absent = (y_col >= 0) & ~found
+        res = []
+        for S in (out.S_hat_0, out.S_hat_L):
+            r = match_log_probs(S, slot, top=top)
+            col = out.S_idx.gather(1, r.top_index.clamp(min=0))
+            res.append(r._replace(
+                log_prob=r.log_prob.masked_fill(absent, -float('inf')),
+                top_index=torch.where(r.top_index < 0, r.top_index, col)))
+        return tuple(res)
 
     def loss(self, S, y, reduction='mean', mask=None):
         r"""Negative log-likelihood of the ground-truth correspondences.
