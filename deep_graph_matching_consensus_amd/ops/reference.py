@@ -13,15 +13,19 @@ import torch
 # --------------------------------------------------------------------------
 def spmm(row, col, val, num_rows, x, self_x=None, self_scale=None,
          bias=None, relu=False, out_dtype=torch.float32):
-    xf = x.float()
-    out = torch.zeros(num_rows, x.size(1), dtype=torch.float32,
-                      device=x.device)
+    # 64-bit inputs (a 64-bit oracle) sum in 64 bits: index_add_ adds in any
+    # order on the GPU, and in 32 bits that order decides the sign of a value
+    # of 1e-7 - a ReLU, and with it a gradient, differently from run to run.
+    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+    xf = x.to(acc)
+    out = torch.zeros(num_rows, x.size(1), dtype=acc, device=x.device)
     if col.numel() > 0:
-        out.index_add_(0, row.long(), val.view(-1, 1) * xf[col.long()])
+        out.index_add_(0, row.long(), val.to(acc).view(-1, 1) *
+                       xf[col.long()])
     if self_x is not None:
-        out = out + self_scale.float() * self_x.float()
+        out = out + self_scale.to(acc) * self_x.to(acc)
     if bias is not None:
-        out = out + bias.float()
+        out = out + bias.to(acc)
     if relu:
         out = torch.relu(out)
     return out.to(out_dtype)
