@@ -58,12 +58,14 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kSlots = 64;            // LDS slots of one head's bias table
+constexpr int kSlots = 64;            // slots of one head's bias table
+constexpr int kTab = kSlots + 1;      // its LDS row: one slot, many banks
 // Finite biases below this count as it: times log2(e) they stay finite, so
 // a row masked everywhere by a type's lowest value is uniform, not empty.
 constexpr float kLowest = -1e38f;
@@ -72,8 +74,10 @@ struct Args {
   const void *q, *k, *v, *o, *dout;
   void *out, *out_lo, *dq, *dk, *dv;  // out_lo: bf16 rest of out (training)
   float *lse, *delta;                 // [Nq, H]
-  // Splits: [S][Nq, H, D] (dk, dv: [2][S][Nk, KV, D]) and [S][Nq, H, 2].
+  // Splits: [S][Nq, H, D] (dk, dv: [2][S][Nk, KV, D]), [S][Nq, H, 2] and
+  // the number of every [tile, KV]'s.
   float *part_o, *part_ml;
+  int* part_n;
   float *part_bias;                   // [blocks][KV][G][kSlots]
   const int *ptr_q, *ptr_k;
   const float* bias;                  // [H, nb]
@@ -82,7 +86,7 @@ struct Args {
   int64_t q_sp, k_sp, v_sp, g_sp;     // between the planes (x6)
   int B, Nq, Nk, H, KV, G, gmul, D, nb, half, mbits, slots;
   float scale, cap, dmax, dmul;
-  int vec_q, vec_k, vec_v, vec_o, vec_g;   // 16-byte rows
+  int vec_o;                          // o has 16-byte rows
   int splits, chunk;                  // most splits, least tiles of one
 };
 
@@ -90,6 +94,13 @@ struct Args {
 // least `chunk` (a join costs more than a short split gains).
 __device__ __forceinline__ int split_tiles(const Args& a, int n) {
   return max(a.chunk, (n + a.splits - 1) / a.splits);
+}
+
+// Leaves the number of splits of `n` tiles, `per` each, to the join.
+__device__ __forceinline__ void put_splits(const Args& a, int where, int split,
+                                           int n, int per) {
+  if (a.splits > 1 && split == 0 && threadIdx.x == 0)
+    a.part_n[where] = (n + per - 1) / per;
 }
 
 // First row of segment `b` (clamped to [0, N]; the first segment starts at
@@ -294,12 +305,12 @@ __device__ __forceinline__ u32x4 load_chunk(const T* row, int ch, int D,
 
 // --------------------------------------------------------------------------
 // Staging.  A tile is ROWS x CH 16-byte chunks, chunk ch of row r at slot
-// (r, ch ^ swz(r)).  Rows of 16-byte chunks go straight from global memory
-// to LDS (buffer_load_dwordx4 ... lds: no register in between, the loads of
-// the next tile stay in flight over the current one's products); a lane
-// fills slot (r, s) with chunk s ^ swz(r) and lanes without a row (or past
-// the width) carry an offset beyond the buffer's range, which reads zeros.
-// Other layouts are loaded value by value and written with ds_write.
+// (r, ch ^ swz(r)).  Rows are 16-byte chunks (the entry points pack other
+// layouts first) and go straight from global memory to LDS
+// (buffer_load_dwordx4 ... lds: no register in between, the loads of the
+// next tile stay in flight over the current one's products); a lane fills
+// slot (r, s) with chunk s ^ swz(r) and lanes without a row (or past the
+// width) carry an offset beyond the buffer's range, which reads zeros.
 // --------------------------------------------------------------------------
 constexpr unsigned kNoRow = 0x80000000u;   // past every buffer's range
 
@@ -310,45 +321,31 @@ struct Stager {
   static constexpr int N = (ROWS * CH + NT - 1) / NT;
   static constexpr bool kFull = N * NT == ROWS * CH;
 
-  // `ok(row)`: the row is there, at `off(row)` bytes from `base` (below 2^31
-  // where vec is set); planes `sp` elements apart.
+  // `ok(row)`: the row is there, at `off(row)` bytes from `base` (below
+  // 2^31); planes `sp` elements apart.
   template <typename Ok, typename Off>
   __device__ __forceinline__ static void fill(const S* base, int64_t sp,
-                                              int D, int vec,
-                                              DGMC_LDS char* tile, Ok ok,
-                                              Off off) {
+                                              int D, DGMC_LDS char* tile,
+                                              Ok ok, Off off) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (vec || P::kPlanes > 1) {
-      // (a wave's many slots are computed anew every tile, a few are kept)
-      const int tid = N > 2 ? opaque(threadIdx.x) : threadIdx.x;
+    // (a wave's many slots are computed anew every tile, a few are kept)
+    const int tid = N > 2 ? opaque(threadIdx.x) : threadIdx.x;
 #pragma unroll
-      for (int p = 0; p < P::kPlanes; ++p) {
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<S*>(base + p * sp), 0, 0x80000000u, 0x00020000);
+    for (int p = 0; p < P::kPlanes; ++p) {
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<S*>(base + p * sp), 0, 0x80000000u, 0x00020000);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          if (!kFull && i * NT + wave * 64 >= ROWS * CH) continue;
-          const int r = (tid + i * NT) / CH;
-          const int ch = ((tid + i * NT) % CH) ^ swz<CH>(r);
-          const unsigned o =
-              ok(r) && ch * E < D ? (unsigned)off(r) + ch * 16 : kNoRow;
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(
-              rs,
-              (DGMC_LDS void*)(tile + (p * ROWS * CH + i * NT + wave * 64) *
-                                          16),
-              16, o, 0, 0, 0);
-        }
-      }
-    } else {
-      const int tid = opaque(threadIdx.x);
-#pragma unroll 1
       for (int i = 0; i < N; ++i) {
-        if (!kFull && tid + i * NT >= ROWS * CH) continue;
+        if (!kFull && i * NT + wave * 64 >= ROWS * CH) continue;
         const int r = (tid + i * NT) / CH;
         const int ch = ((tid + i * NT) % CH) ^ swz<CH>(r);
-        const u32x4 v = load_chunk<S>(
-            (const S*)((const char*)base + off(r)), ch, D, ok(r), 0);
-        *(DGMC_LDS u32x4*)(tile + (tid + i * NT) * 16) = v;
+        const unsigned o =
+            ok(r) && ch * E < D ? (unsigned)off(r) + ch * 16 : kNoRow;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rs,
+            (DGMC_LDS void*)(tile +
+                             (p * ROWS * CH + i * NT + wave * 64) * 16),
+            16, o, 0, 0, 0);
       }
     }
   }
@@ -398,17 +395,36 @@ template <typename P, int N>
 __device__ __forceinline__ void load_frags(u32x4 (&f)[P::kPlanes][N],
                                            const typename P::S* base,
                                            int64_t sp, int64_t off, bool live,
-                                           int D, int vec) {
+                                           int D) {
 #pragma unroll
   for (int p = 0; p < P::kPlanes; ++p)
-    load_row(f[p], base + p * sp, off, live, D, vec || P::kPlanes > 1);
+    load_row(f[p], base + p * sp, off, live, D, 1);
 }
 
-// Every wave's staged data (and LDS reads) done, then the barrier.
+// Every wave's staged data (and LDS reads) done, then the barrier.  (The
+// wait as a builtin: the compiler so knows that nothing is in flight behind
+// it, and does not wait for older loads with the next tile's among them.)
 __device__ __forceinline__ void stage_barrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);      // vmcnt(0) lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+}
+
+// load(t) and use(t) for t = 0 .. N - 1, every load kAhead steps ahead of its
+// use and no further: where registers are short the compiler otherwise loads
+// and waits one step at a time.
+constexpr int kAhead = 2;
+template <int N, typename L, typename U>
+__device__ __forceinline__ void stepped(L load, U use) {
+#pragma unroll
+  for (int t = 0; t < kAhead; ++t) load(t);
+#pragma unroll
+  for (int t = 0; t < N; ++t) {
+    if (t + kAhead < N) load(t + kAhead);
+    __builtin_amdgcn_sched_barrier(0);
+    use(t);
+  }
 }
 
 // --------------------------------------------------------------------------
@@ -457,6 +473,28 @@ struct Bf16 {
                                                const DGMC_LDS char* tile,
                                                int cols, f32x16 p) {
     constexpr int CH = DP / 8;
+    if constexpr (CH >= 16) {
+      bf16x8 a[2 * (DP / 32)], b[2], lo_b[2];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        b[i >> 3][i & 7] = (__bf16)p[i];
+        if (FINE)
+          lo_b[i >> 3][i & 7] = (__bf16)(p[i] - (float)b[i >> 3][i & 7]);
+      }
+      stepped<2 * (DP / 32)>(
+          [&](int t) {
+            a[t] = col_frag<CH>(tile, cols, t / (DP / 32), t % (DP / 32));
+          },
+          [&](int t) {
+            const int c = t / (DP / 32), k = t % (DP / 32);
+            acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[t], b[c],
+                                                             acc[k], 0, 0, 0);
+            if constexpr (FINE)
+              acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                  a[t], lo_b[c], acc[k], 0, 0, 0);
+          });
+      return;
+    }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       bf16x8 b, lo_b;
@@ -637,6 +675,28 @@ __device__ __forceinline__ f32x16 row_dot(
   return acc;
 }
 
+// Two row products of the backward: z of tile 0 with fz(s), dp of the tile TB
+// bytes on with fd(s), the chunks of the lane's own rows.
+template <typename P, int CH, int ROWS, typename Z, typename D>
+__device__ __forceinline__ void row_dot2(f32x16& z, f32x16& dp,
+                                         const DGMC_LDS char* lds, int TB,
+                                         int rows, Z fz, D fd) {
+  constexpr int N = CH / 2;
+  u32x4 a[2 * N], b[2 * N];
+  z = dp = f32x16{};
+  stepped<2 * N>(
+      [&](int t) {
+        const int s = t % N;
+        a[t] = *(const DGMC_LDS u32x4*)(lds + (t < N ? 0 : TB) +
+                                        (rows ^ (32 * s)));
+        b[t] = t < N ? fz(s) : fd(s);
+      },
+      [&](int t) {
+        f32x16& acc = t < N ? z : dp;
+        acc = P::dot(a[t], b[t], acc);
+      });
+}
+
 // Four values of an output row of D at d (d % 4 == 0).
 template <typename T>
 __device__ __forceinline__ void put4(T* row, int d, int D, const T* v) {
@@ -709,10 +769,14 @@ struct Bucket {
 };
 
 // Positions as floats, clamped to +-2^23 (their differences are exact).
+// (What is fetched for the next tile is converted when it is put there: a
+// conversion right behind its load would wait for the whole tile.)
+__device__ __forceinline__ float to_pos(int p) {
+  return (float)min(max(p, -(1 << 23)), 1 << 23);
+}
 __device__ __forceinline__ float load_pos(const int* pos, int64_t i, int axes,
                                           int axis) {
-  const int p = pos[i * axes + axis];
-  return (float)min(max(p, -(1 << 23)), 1 << 23);
+  return to_pos(pos[i * axes + axis]);
 }
 
 // Keys of a forward tile: 64 where four waves share it and both buffers of K
@@ -750,8 +814,33 @@ __device__ __forceinline__ void load_table(const Args& a, int kvh,
       if (v < kLowest && v > -INFINITY) v = kLowest;
       v *= kLog2e;
     }
-    tab[e] = v;
+    tab[g * kTab + s] = v;
   }
+}
+
+// Whether all offsets between this lane's position `p` and the 16 x 2 other
+// positions `o` of a 32-row block (this half's at o + 4 h) fall into one
+// bucket, in every lane of the wave that `live`s; `s`: the bucket.  Slots
+// ascend with the offset, so the least and the greatest position tell (a
+// neighbour's rows may be among them: they can only say no).  Blocks of nodes
+// in order that lie far apart share a bucket: one look-up and one sum then
+// serve 16 pairs of a lane.  KEY: offsets are o - p, else p - o.
+template <bool KEY>
+__device__ __forceinline__ bool one_bucket(const Bucket& bk,
+                                           const DGMC_LDS float* o, float p,
+                                           bool live, int& s) {
+  const int h = (threadIdx.x >> 5) & 1;
+  float mn = INFINITY, mx = -INFINITY;
+#pragma unroll
+  for (int r4 = 0; r4 < 4; ++r4) {
+    const f32x4 x = *(const DGMC_LDS f32x4*)(o + 8 * r4 + 4 * h);
+    mn = fminf(fminf(mn, fminf(x[0], x[1])), fminf(x[2], x[3]));
+    mx = fmaxf(fmaxf(mx, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
+  }
+  mn = -max_half(-mn);
+  mx = max_half(mx);
+  s = bk.slot(KEY ? mn - p : p - mn);
+  return __all(!live || s == bk.slot(KEY ? mx - p : p - mx));
 }
 
 }  // namespace segattn

@@ -1,6 +1,7 @@
-// Segment attention: entry points, the join of split keys and the sum of the
-// bias table's gradient.  The kernels are in segment_attention_{fwd,bwd}.h,
-// instantiated per type in segment_attention_{fwd,bwd}_{bf16,f32}.hip.
+// Segment attention: entry points, copies of inputs, the join of split keys
+// and the sum of the bias table's gradient.  The kernels are in
+// segment_attention_{fwd,bwd}.h, instantiated per kernel and type in
+// segment_attention_{fwd,dq,dkv}_*.hip.
 #include "attentional.h"
 #include "segment_attention.h"
 
@@ -18,33 +19,55 @@ void dkv_bf16(const Args& a, int axes, int nw, hipStream_t st);
 void dkv_f32(const Args& a, int axes, int nw, hipStream_t st);
 void dkv_x6(const Args& a, int axes, hipStream_t st);
 
-// fp32 [N, heads, D] tensors -> bf16 planes [3][N][heads][D8] (hi, mid, lo;
-// D8: D rounded up to 8, zeros behind D), 8 values a thread.
-struct Planes {
-  const float* src[4];
-  __bf16* dst[4];
-  int64_t sn[4], sh[4], n[4];       // strides, N * heads * D8 / 8
+// Copies of strided [N, heads, D] tensors in the form the kernels read: rows
+// padded with zeros to DC, a whole number of chunks of E values, one chunk a
+// thread.
+struct Copies {
+  const void* src[4];
+  void* dst[4];
+  int64_t sn[4], sh[4], n[4];       // strides, chunks (0: none to make)
   int heads[4];
   int D;
 };
 
-__global__ __launch_bounds__(256) void planes_kernel(const Planes p) {
-  const int t = blockIdx.y, c8 = (p.D + 7) / 8;
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= p.n[t]) return;
-  const int64_t row = e / c8;
-  const int d0 = (int)(e - row * c8) * 8;
+// This thread's chunk of tensor blockIdx.y; false: there is none.
+template <typename T, int E>
+__device__ __forceinline__ bool copy_chunk(const Copies& p, int64_t& e,
+                                           T (&x)[E]) {
+  const int t = blockIdx.y, ce = (p.D + E - 1) / E;
+  e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= p.n[t]) return false;
+  const int64_t row = e / ce;
+  const int d0 = (int)(e - row * ce) * E;
   const int64_t i = row / p.heads[t];
   const int hd = (int)(row - i * p.heads[t]);
-  const float* src = p.src[t] + i * p.sn[t] + hd * p.sh[t];
-  float x[8];
-  if (d0 + 8 <= p.D && aligned16(src + d0)) {
-    load_vec<float, 4>(src + d0, x);
-    load_vec<float, 4>(src + d0 + 4, x + 4);
+  const T* src = (const T*)p.src[t] + i * p.sn[t] + hd * p.sh[t] + d0;
+  if (d0 + E <= p.D && aligned16(src)) {
+    __builtin_memcpy(x, __builtin_assume_aligned(src, 16), E * sizeof(T));
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = d0 + k < p.D ? src[d0 + k] : 0.f;
+    for (int k = 0; k < E; ++k) x[k] = d0 + k < p.D ? src[k] : (T)0.f;
   }
+  return true;
+}
+
+// Rows that are not 16-byte chunks: the same values, padded.
+template <typename T>
+__global__ __launch_bounds__(256) void pad_kernel(const Copies p) {
+  constexpr int E = 16 / sizeof(T);
+  int64_t e;
+  T x[E];
+  if (!copy_chunk(p, e, x)) return;
+  T* dst = (T*)p.dst[blockIdx.y] + e * E;
+  __builtin_memcpy(__builtin_assume_aligned(dst, 16), x, 16);
+}
+
+// fp32 -> bf16 planes [3][N][heads][D8] (hi, mid, lo).
+__global__ __launch_bounds__(256) void planes_kernel(const Copies p) {
+  const int t = blockIdx.y;
+  int64_t e;
+  float x[8];
+  if (!copy_chunk(p, e, x)) return;
   bf16x8 v[3];
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
@@ -58,94 +81,118 @@ __global__ __launch_bounds__(256) void planes_kernel(const Planes p) {
   }
 #pragma unroll
   for (int q = 0; q < 3; ++q)
-    *(bf16x8*)(p.dst[t] + (q * p.n[t] + e) * 8) = v[q];
+    *(bf16x8*)((__bf16*)p.dst[t] + (q * p.n[t] + e) * 8) = v[q];
 }
 
 constexpr int kMaxSplits = 512;
 
 // Join of the split rows (FWD: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M)
-// l_s; DQ, DKV: plain sums), in order of the splits.  A workgroup takes the
-// rows of one tile of the kernel whose splits it joins; 16 threads a row, 8
-// values each (dim <= 128), and where a tile has few rows the splits of a row are shared
-// out to several such groups (their sums added in order).
+// l_s; DQ, DKV: plain sums), in a fixed order of the splits.  A workgroup
+// takes rows of one tile of the kernel whose splits it joins (that kernel
+// left the number of the tile's splits); 1 << lt threads a row, 8 values
+// each, and `ways` (a power of two) such groups share the splits of a row,
+// kJoin of them loaded at a time; their sums are added in order.
 enum { FWD, DQ, DKV };
+constexpr int kJoin = 4;
 
 template <typename T, int MODE>
 __global__ __launch_bounds__(256) void join_kernel(const Args a, int per_tile,
-                                                   int key_tile, int ways) {
+                                                   int ways, int lt) {
   __shared__ float red[256][9];
-  __shared__ float wsum[16];
+  __shared__ float2 wml[64];
+  const int ns = a.part_n[blockIdx.x];
+  if (ns <= 1) return;
   const int kvh = blockIdx.x % a.KV;
-  const int* own = MODE == DKV ? a.ptr_k : a.ptr_q;
-  const int* other = MODE == DKV ? a.ptr_q : a.ptr_k;
-  const int N = MODE == DKV ? a.Nk : a.Nq, No = MODE == DKV ? a.Nq : a.Nk;
+  const int N = MODE == DKV ? a.Nk : a.Nq;
   const int lo = blockIdx.x / a.KV * per_tile, hi = min(lo + per_tile, N);
-  const Rows w = Rows::find<4>(own, other, a.B, N, No, lo, hi, lo, 0);
-  const int ntile = (w.hi - w.lo + key_tile - 1) / key_tile;
-  const int per = split_tiles(a, ntile);
-  if (per >= ntile) return;
-  const int ns = (ntile + per - 1) / per;
-
   const int G = MODE == DKV ? 1 : a.G, heads = G * a.KV;
   const int rows = (hi - lo) * G;
   const int64_t all = (int64_t)N * heads;
-  const int grp = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
-  // `ways` (a power of two) groups share a row; 16 / ways rows a round.
-  const int rpr = 16 / ways, rr = grp / ways, way = grp % ways;
+  const int tid = threadIdx.x, tpr = 1 << lt, d0 = (tid & (tpr - 1)) * 8;
+  const int grp = tid >> lt, rpr = (256 >> lt) / ways;
+  const int rr = grp / ways, way = grp % ways;
+  const bool vec = a.D % 4 == 0 && d0 + 8 <= a.D;
   const float* part =
       a.part_o + (MODE == DKV ? blockIdx.y * a.splits * all * a.D : 0);
   for (int r0 = blockIdx.z * rpr; r0 < rows; r0 += rpr * gridDim.z) {
     const int r = r0 + rr;
     const bool live = r < rows;
-    const int64_t row =
-        (int64_t)(lo + r / G) * heads + kvh * G + r % G;
+    const int64_t row = (int64_t)(lo + r / G) * heads + kvh * G + r % G;
     float M = -INFINITY, L = 0.f, o[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) o[k] = 0.f;
-    if (live) {
-      const float* ml = a.part_ml + row * 2;
-      if (MODE == FWD) {
-#pragma unroll 4
-        for (int s = threadIdx.x & 15; s < ns; s += 16)
-          M = fmaxf(M, ml[s * all * 2]);
+    for (int s0 = way; live && s0 < ns; s0 += kJoin * ways) {
+      float2 ml[kJoin];
+      f32x4 x[kJoin], y[kJoin];
 #pragma unroll
-        for (int o = 1; o < 16; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
-        if (M == -INFINITY) M = 0.f;
-      }
-#pragma unroll 4
-      for (int s = way; s < ns; s += ways) {
-        float wt = 1.f;
-        if (MODE == FWD) {
-          const float2 x = *(const float2*)(ml + s * all * 2);
-          wt = exp2_(x.x - M);
-          L += wt * x.y;
-        }
-        const float* p = part + (s * all + row) * a.D;
-        if (a.D % 4 == 0 && d0 + 8 <= a.D) {
-          const f32x4 x = *(const f32x4*)(p + d0),
-                      y = *(const f32x4*)(p + d0 + 4);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            o[k] += wt * x[k];
-            o[4 + k] += wt * y[k];
-          }
+      for (int i = 0; i < kJoin; ++i) {
+        const int s = s0 + i * ways;
+        ml[i] = make_float2(-INFINITY, 0.f);
+        x[i] = y[i] = f32x4{};
+        if (s >= ns) continue;
+        if (MODE == FWD)
+          ml[i] = *(const float2*)(a.part_ml + (s * all + row) * 2);
+        const float* p = part + (s * all + row) * a.D + d0;
+        if (vec) {
+          x[i] = *(const f32x4*)p;
+          y[i] = *(const f32x4*)(p + 4);
         } else {
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (d0 + k < a.D) o[k] += wt * p[d0 + k];
+          for (int k = 0; k < 4; ++k) {
+            if (d0 + k < a.D) x[i][k] = p[k];
+            if (d0 + 4 + k < a.D) y[i][k] = p[4 + k];
+          }
         }
       }
+      float wt[kJoin];
+      if (MODE == FWD) {
+        float m = M;
+#pragma unroll
+        for (int i = 0; i < kJoin; ++i) m = fmaxf(m, ml[i].x);
+        const float ms = m == -INFINITY ? 0.f : m, f = exp2_(M - ms);
+        L *= f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] *= f;
+        M = m;
+#pragma unroll
+        for (int i = 0; i < kJoin; ++i) {
+          wt[i] = exp2_(ml[i].x - ms);
+          L = fmaf(wt[i], ml[i].y, L);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kJoin; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          o[k] = MODE == FWD ? fmaf(wt[i], x[i][k], o[k]) : o[k] + x[i][k];
+          o[4 + k] =
+              MODE == FWD ? fmaf(wt[i], y[i][k], o[4 + k]) : o[4 + k] + y[i][k];
+        }
     }
     if (ways > 1) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) red[threadIdx.x][k] = o[k];
-      if ((threadIdx.x & 15) == 0) wsum[grp] = L;
+      for (int k = 0; k < 8; ++k) red[tid][k] = o[k];
+      if ((tid & (tpr - 1)) == 0) wml[grp] = make_float2(M, L);
       __syncthreads();
       if (way == 0) {
-        for (int k2 = 1; k2 < ways; ++k2) {
+        if (MODE == FWD) {
+          for (int w = 1; w < ways; ++w) M = fmaxf(M, wml[grp + w].x);
+          const float ms = M == -INFINITY ? 0.f : M;
+          L = 0.f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) o[k] += red[threadIdx.x + 16 * k2][k];
-          L += wsum[grp + k2];
+          for (int k = 0; k < 8; ++k) o[k] = 0.f;
+          for (int w = 0; w < ways; ++w) {
+            const float2 x = wml[grp + w];
+            const float f = exp2_(x.x - ms);
+            L = fmaf(f, x.y, L);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              o[k] = fmaf(f, red[tid + tpr * w][k], o[k]);
+          }
+        } else {
+          for (int w = 1; w < ways; ++w)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[k] += red[tid + tpr * w][k];
         }
       }
       __syncthreads();
@@ -158,34 +205,40 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int per_tile,
                   : MODE == DQ ? a.dq
                                : (blockIdx.y ? a.dv : a.dk)) +
              row * a.D;
+    T v[8], v_lo[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (d0 + k < a.D) {
-        const T v = (T)(o[k] * f);
-        out[d0 + k] = v;
-        if (MODE == FWD && a.out_lo)
-          ((T*)a.out_lo)[row * a.D + d0 + k] = (T)(o[k] * f - (float)v);
-      }
+    for (int k = 0; k < 8; ++k) {
+      v[k] = (T)(o[k] * f);
+      v_lo[k] = (T)(o[k] * f - (float)v[k]);
+    }
+    put4(out, d0, a.D, v);
+    put4(out, d0 + 4, a.D, v + 4);
+    if (MODE == FWD && a.out_lo) {
+      T* lo_row = (T*)a.out_lo + row * a.D;
+      put4(lo_row, d0, a.D, v_lo);
+      put4(lo_row, d0 + 4, a.D, v_lo + 4);
+    }
     if (MODE == FWD && a.lse && d0 == 0)
       a.lse[row] = L == 0.f ? INFINITY : M + log2f(L);
   }
 }
 
 template <int MODE>
-static void join(const Args& a, bool f32, int per_tile, int key_tile) {
+static void join(const Args& a, bool f32, int per_tile) {
   const int N = MODE == DKV ? a.Nk : a.Nq;
   const int G = MODE == DKV ? 1 : a.G;
-  int ways = 1;                     // at most four splits of a row a group
-  while (ways < 16 && 4 * ways < a.splits) ways *= 2;
-  // (workgroups along z share a tile's rows, 16 / ways a round)
+  const int lt = a.D > 64 ? 4 : a.D > 32 ? 3 : 2, groups = 256 >> lt;
+  int ways = 1;
+  while (ways < groups && kJoin * ways < a.splits) ways *= 2;
+  // (workgroups along z share a tile's rows, groups / ways a round)
   const dim3 grid((N + per_tile - 1) / per_tile * a.KV, MODE == DKV ? 2 : 1,
-                  std::min((per_tile * G * ways + 15) / 16, 128));
+                  std::min((per_tile * G * ways + groups - 1) / groups, 128));
   if (f32)
-    join_kernel<float, MODE><<<grid, 256, 0, stream()>>>(a, per_tile,
-                                                         key_tile, ways);
+    join_kernel<float, MODE><<<grid, 256, 0, stream()>>>(a, per_tile, ways,
+                                                         lt);
   else
-    join_kernel<__bf16, MODE><<<grid, 256, 0, stream()>>>(a, per_tile,
-                                                          key_tile, ways);
+    join_kernel<__bf16, MODE><<<grid, 256, 0, stream()>>>(a, per_tile, ways,
+                                                          lt);
   DGMC_CHECK_LAUNCH();
 }
 
@@ -239,13 +292,13 @@ static void check_index(const at::Tensor& t, const char* name, int dim,
 }
 
 // 16-byte loads of whole rows: base, row and head strides and the width are
-// multiples of 16 bytes, and a tile (64 rows, 32 heads) spans less than the
+// multiples of 16 bytes, and a tile (128 rows, 32 heads) spans less than the
 // 2^31 bytes of a buffer's offsets.
-static int rows16(const at::Tensor& t) {
+static bool rows16(const at::Tensor& t) {
   const int64_t e = 16 / t.element_size();
   return t.size(2) % e == 0 && t.stride(0) % e == 0 && t.stride(1) % e == 0 &&
          aligned16(t.data_ptr()) &&
-         (64 * t.stride(0) + 32 * t.stride(1) + 128) * t.element_size() <
+         (128 * t.stride(0) + 32 * t.stride(1) + 128) * t.element_size() <
              ((int64_t)1 << 31);
 }
 
@@ -293,7 +346,6 @@ static Args make_args(const at::Tensor& q, const at::Tensor& k,
   a.Nq = (int)q.size(0); a.Nk = (int)k.size(0);
   a.ptr_q = ptr_q.data_ptr<int>(); a.ptr_k = ptr_k.data_ptr<int>();
   a.scale = (float)scale; a.cap = (float)cap;
-  a.vec_q = rows16(q); a.vec_k = rows16(k); a.vec_v = rows16(v);
   a.splits = 1;
   axes = 0;
   if (bias.has_value()) {
@@ -341,53 +393,87 @@ static bool takes_x6(const Args& a, bool x6) {
          waves_for(a.Nk, a.B) == 4;
 }
 
-// Points q, k, v (and dout) of `a` to their planes; `ws` keeps them alive.
-static at::Tensor make_planes(Args& a, bool with_dout,
-                              const at::Tensor& like) {
-  const int64_t D8 = (a.D + 7) / 8 * 8;
-  const int64_t nq = (int64_t)a.Nq * a.H * D8, nk = (int64_t)a.Nk * a.KV * D8;
-  at::Tensor ws = at::empty({3 * (nq * (with_dout ? 2 : 1) + 2 * nk)},
-                            like.options().dtype(at::kBFloat16));
-  __bf16* w = (__bf16*)ws.data_ptr();
-  Planes p = {};
+// Points q, k, v (and dout, if defined) of `a` to copies of them: all of them
+// to their planes (`six`), else those whose rows are not 16-byte chunks to
+// padded ones.  The result keeps the copies alive.
+static at::Tensor make_copies(Args& a, bool six, const at::Tensor& q,
+                              const at::Tensor& k, const at::Tensor& v,
+                              const at::Tensor& dout) {
+  const bool f = q.scalar_type() == at::kFloat;
+  const int E = six ? 8 : f ? 4 : 8, planes = six ? 3 : 1;
+  const int64_t DC = (a.D + E - 1) / E * E;
+  const at::Tensor* ts[4] = {&q, &k, &v, &dout};
+  Copies p = {};
   p.D = a.D;
-  int64_t most = 0;
+  int64_t total = 0, most = 0;
+  for (int t = 0; t < 4; ++t) {
+    if (!ts[t]->defined() || (!six && rows16(*ts[t]))) continue;
+    p.heads[t] = (int)ts[t]->size(1);
+    p.n[t] = ts[t]->size(0) * p.heads[t] * DC / E;
+    total += planes * p.n[t] * E;
+    most = std::max(most, p.n[t]);
+  }
+  if (most == 0) return at::Tensor();
+  at::Tensor ws = at::empty({total}, q.options().dtype(
+                                         six ? at::kBFloat16
+                                             : q.scalar_type()));
+  char* w = (char*)ws.data_ptr();
   auto add = [&](int t, const void*& ptr, int64_t& sn, int64_t& sh,
-                 int64_t& sp, int64_t n, int heads) {
-    p.src[t] = (const float*)ptr;
+                 int64_t& sp) {
+    if (p.n[t] == 0) return;
+    p.src[t] = ptr;
     p.dst[t] = w;
     p.sn[t] = sn;
     p.sh[t] = sh;
-    p.n[t] = n / 8;
-    p.heads[t] = heads;
-    most = std::max(most, n / 8);
     ptr = w;
-    sn = heads * D8;
-    sh = D8;
-    sp = n;
-    w += 3 * n;
+    sn = p.heads[t] * DC;
+    sh = DC;
+    sp = p.n[t] * E;
+    w += planes * p.n[t] * 16;
   };
-  add(0, a.q, a.q_sn, a.q_sh, a.q_sp, nq, a.H);
-  add(1, a.k, a.k_sn, a.k_sh, a.k_sp, nk, a.KV);
-  add(2, a.v, a.v_sn, a.v_sh, a.v_sp, nk, a.KV);
-  if (with_dout) add(3, a.dout, a.g_sn, a.g_sh, a.g_sp, nq, a.H);
-  planes_kernel<<<dim3((unsigned)((most + 255) / 256), with_dout ? 4 : 3), 256,
-                  0, stream()>>>(p);
+  add(0, a.q, a.q_sn, a.q_sh, a.q_sp);
+  add(1, a.k, a.k_sn, a.k_sh, a.k_sp);
+  add(2, a.v, a.v_sn, a.v_sh, a.v_sp);
+  add(3, a.dout, a.g_sn, a.g_sh, a.g_sp);
+  const dim3 grid((unsigned)((most + 255) / 256), 4);
+  six ? planes_kernel<<<grid, 256, 0, stream()>>>(p)
+  : f ? pad_kernel<float><<<grid, 256, 0, stream()>>>(p)
+      : pad_kernel<__bf16><<<grid, 256, 0, stream()>>>(p);
   DGMC_CHECK_LAUNCH();
   return ws;
 }
 
 // Splits of the other axis (`n` rows in tiles of `tile`) where the `tiles`
-// of the own axis are too few or too uneven to fill the chip: up to 1024
-// workgroups, no split under kChunk tiles.  False: none.
-constexpr int kChunk = 8;
-static bool split_axis(Args& a, int64_t tiles, int64_t n, int tile) {
+// of the own axis are too few or too uneven to fill the chip: up to two
+// rounds of the workgroups of four waves that it holds at `waves` a SIMD
+// (knowledge graphs' evaluation, 4 a SIMD: 1024 workgroups 540 us, 2048 516;
+// 2 a SIMD: 1024 444 us of the ragged case, 1536 509, 768 487), no split
+// under 16 tiles (ragged case: 8 650 us, 16 604, 32 659), 8 where one wave
+// walks them (new entities: 16 44 us, 8 35).  False: none.
+static bool split_axis(Args& a, int64_t tiles, int64_t n, int tile, int nw,
+                       int waves) {
   tiles = std::max<int64_t>(tiles, 1) * a.KV;
-  a.chunk = kChunk;
+  a.chunk = nw == 4 ? 16 : 8;
   a.splits = (int)std::max<int64_t>(
-      1, std::min<int64_t>({(1024 + tiles - 1) / tiles,
-                            n / ((int64_t)tile * kChunk), kMaxSplits}));
+      1, std::min<int64_t>({(512 * waves + tiles - 1) / tiles,
+                            n / ((int64_t)tile * a.chunk), kMaxSplits}));
   return a.splits > 1;
+}
+
+// Workspace of the splits: `outs` outputs and, for the forward (ml), maxima
+// and sums of `rows` rows each, then the number of every tile's splits.
+static at::Tensor part_workspace(Args& a, int64_t rows, int outs, bool ml,
+                                 int64_t tiles, const at::Tensor& like) {
+  const int64_t no = outs * a.splits * rows * a.D;
+  const int64_t nml = ml ? 2 * a.splits * rows : 0;
+  // (pairs of floats and 16-byte rows keep their alignment)
+  const int64_t no4 = (no + 3) / 4 * 4;
+  at::Tensor ws = at::empty({no4 + nml + tiles * a.KV},
+                            like.options().dtype(at::kFloat));
+  a.part_o = ws.data_ptr<float>();
+  a.part_ml = a.part_o + no4;
+  a.part_n = (int*)(a.part_ml + nml);
+  return ws;
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> forward(
@@ -415,20 +501,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> forward(
   const int DP = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
   const int TQ = 32 / a.G * nw,
             KT = fwd_keys(DP, nw, six ? 6 : f ? 4 : 2);
-  at::Tensor ws;
-  if (six) ws = make_planes(a, false, q);
-  at::Tensor po, pml;
-  if (split_axis(a, a.Nq / TQ, a.Nk, KT)) {
-    po = at::empty({a.splits, a.Nq, a.H, a.D}, f32);
-    pml = at::empty({a.splits, a.Nq, a.H, 2}, f32);
-    a.part_o = po.data_ptr<float>();
-    a.part_ml = pml.data_ptr<float>();
-  }
+  const at::Tensor ws = make_copies(a, six, q, k, v, at::Tensor());
+  at::Tensor part;
+  if (split_axis(a, a.Nq / TQ, a.Nk, KT, nw, f || DP > 64 ? 2 : 4))
+    part = part_workspace(a, (int64_t)a.Nq * a.H, 1, true,
+                          (a.Nq + TQ - 1) / TQ, q);
   six    ? fwd_x6(a, axes, stream())
   : f    ? fwd_f32(a, axes, nw, stream())
   : fine ? fwd_bf16_fine(a, axes, nw, stream())
          : fwd_bf16(a, axes, nw, stream());
-  if (a.splits > 1) join<FWD>(a, f, TQ, KT);
+  if (a.splits > 1) join<FWD>(a, f, TQ);
   return {out, lo, lse};
 }
 
@@ -472,7 +554,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
   a.out_lo = lo.data_ptr();
   a.dout = dout.data_ptr();
   a.g_sn = dout.stride(0); a.g_sh = dout.stride(1);
-  a.vec_g = rows16(dout); a.vec_o = rows16(out);
+  a.vec_o = rows16(out);
   a.lse = lse.data_ptr<float>();
   a.delta = delta.data_ptr<float>();
   a.dq = dq.data_ptr();
@@ -483,12 +565,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
   const int nwk = waves_for(a.Nk, a.B);
   const int TQ = 32 / a.G * nwq;
   const bool six = f && takes_x6(a, x6);
-  at::Tensor pq, pk, ws;
-  if (six) ws = make_planes(a, true, q);
-  if (split_axis(a, a.Nq / TQ, a.Nk, 32)) {
-    pq = at::empty({a.splits, a.Nq, a.H, a.D}, f32);
-    a.part_o = pq.data_ptr<float>();
-  }
+  at::Tensor pq, pk;
+  const at::Tensor ws = make_copies(a, six, q, k, v, dout);
+  if (split_axis(a, a.Nq / TQ, a.Nk, 32, nwq, 2))
+    pq = part_workspace(a, (int64_t)a.Nq * a.H, 1, false,
+                        (a.Nq + TQ - 1) / TQ, q);
   // Workgroups of the dq kernel with a table: each keeps its LDS columns
   // over all of its tiles.
   int nblk = 0;
@@ -502,16 +583,15 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
   six ? dq_x6(a, axes, nblk, stream())
   : f ? dq_f32(a, axes, nwq, nblk, stream())
       : dq_bf16(a, axes, nwq, nblk, stream());
-  if (a.splits > 1) join<DQ>(a, f, TQ, 32);
+  if (a.splits > 1) join<DQ>(a, f, TQ);
   if (a.Nk > 0) {
-    if (split_axis(a, a.Nk / (32 * nwk), a.Nq, 32 / a.G)) {
-      pk = at::empty({2, a.splits, a.Nk, a.KV, a.D}, f32);
-      a.part_o = pk.data_ptr<float>();
-    }
+    if (split_axis(a, a.Nk / (32 * nwk), a.Nq, 32 / a.G, nwk, 2))
+      pk = part_workspace(a, (int64_t)a.Nk * a.KV, 2, false,
+                          (a.Nk + 32 * nwk - 1) / (32 * nwk), q);
     six ? dkv_x6(a, axes, stream())
     : f ? dkv_f32(a, axes, nwk, stream())
         : dkv_bf16(a, axes, nwk, stream());
-    if (a.splits > 1) join<DKV>(a, f, 32 * nwk, 32 / a.G);
+    if (a.splits > 1) join<DKV>(a, f, 32 * nwk);
   }
   if (axes) {
     bias_sum_kernel<<<a.H, kSlots * kSumWays, 0, stream()>>>(

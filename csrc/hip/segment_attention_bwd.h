@@ -51,12 +51,19 @@ __device__ __forceinline__ void add_slots(DGMC_LDS float* hist,
   hist[d * 64] = hd + vd;
 }
 
+// Wide heads at two waves per SIMD: registers are short.
+template <typename P>
+constexpr bool tight(int DP) {
+  return P::kPlanes == 1 && sizeof(typename P::S) == 2 && DP == 128;
+}
+
 template <typename P, int DP, int NW, int POS>
 __global__ __launch_bounds__(
     NW * 64, sizeof(typename P::S) == 2 ? 2 : 1) void
 dq_kernel(const Args a, int ntiles) {
   using T = typename P::T;
   using S = typename P::S;
+  constexpr bool kTight = tight<P>(DP);
   constexpr int KT = 32;
   constexpr int CH = DP * (int)sizeof(S) / 16;
   constexpr int NT = NW * 64;
@@ -64,8 +71,8 @@ dq_kernel(const Args a, int ntiles) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   DGMC_LDS char* lds = (DGMC_LDS char*)smem;
   DGMC_LDS float* kpos = (DGMC_LDS float*)(lds + 4 * TB);   // [2][2][KT]
-  DGMC_LDS float* tab = kpos + (POS ? 4 * KT : 0);          // [G][kSlots]
-  DGMC_LDS float* hist = tab + (POS ? a.G * kSlots : 0);    // [NW][slots][64]
+  DGMC_LDS float* tab = kpos + (POS ? 4 * KT : 0);          // [G][kTab]
+  DGMC_LDS float* hist = tab + (POS ? a.G * kTab : 0);    // [NW][slots][64]
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int h = lane >> 5, c = lane & 31;
@@ -75,7 +82,7 @@ dq_kernel(const Args a, int ntiles) {
   const int cq = div_group(a, c), g = c - cq * a.G, W = 2 * a.half + 2;
   const int head = kvh * a.G + g, qo = wave * QW + cq;
   const Bucket bk(a);
-  const DGMC_LDS float* mytab = tab + g * kSlots;
+  const DGMC_LDS float* mytab = tab + g * kTab;
   DGMC_LDS float* myhist = hist + wave * a.slots * 64 + lane;
   if constexpr (POS > 0) {
     load_table(a, kvh, tab, POS);
@@ -99,12 +106,12 @@ dq_kernel(const Args a, int ntiles) {
                   (const S*)a.q + (int64_t)q_lo * a.q_sn +
                       (int64_t)kvh * a.G * a.q_sh,
                   a.q_sp, (qo * a.q_sn + g * a.q_sh) * (int64_t)sizeof(S),
-                  live, a.D, a.vec_q);
+                  live, a.D);
     load_frags<P>(gf,
                   (const S*)a.dout + (int64_t)q_lo * a.g_sn +
                       (int64_t)kvh * a.G * a.g_sh,
                   a.g_sp, (qo * a.g_sn + g * a.g_sh) * (int64_t)sizeof(S),
-                  live, a.D, a.vec_g);
+                  live, a.D);
     const int wrows = min(QW, q_hi - q_lo - wave * QW);
     const Rows w =
         Rows::find<NW>(a.ptr_q, a.ptr_k, a.B, a.Nq, a.Nk, q_lo, q_hi, qi,
@@ -112,6 +119,7 @@ dq_kernel(const Args a, int ntiles) {
     const int ntile = (w.hi - w.lo + KT - 1) / KT;
     const int per = split_tiles(a, ntile);
     if (split > 0 && split * per >= ntile) continue;
+    put_splits(a, it / a.splits * a.KV + kvh, split, ntile, per);
     const int k_lo = w.lo + split * per * KT;
     const int k_hi = min(k_lo + per * KT, w.hi);
 
@@ -159,28 +167,28 @@ dq_kernel(const Args a, int ntiles) {
       if (POS == 2) py = load_pos(a.pos_q, qi, POS, 1);
     }
 
-    float pr[2] = {0.f, 0.f};
+    int pr[2] = {0, 0};
     auto fetch = [&](int k0, int e, int buf) {
       using St = Stager<P, KT, CH, NT>;
       const int left = e - k0;
       DGMC_LDS char* kt = lds + buf * 2 * TB;
       const auto ok = [&](int r) { return r < left; };
-      St::fill(kbase + (int64_t)k0 * a.k_sn, a.k_sp, a.D, a.vec_k, kt, ok,
+      St::fill(kbase + (int64_t)k0 * a.k_sn, a.k_sp, a.D, kt, ok,
                [&](int r) { return r * (a.k_sn * (int)sizeof(S)); });
-      St::fill(vbase + (int64_t)k0 * a.v_sn, a.v_sp, a.D, a.vec_v, kt + TB,
+      St::fill(vbase + (int64_t)k0 * a.v_sn, a.v_sp, a.D, kt + TB,
                ok, [&](int r) { return r * (a.v_sn * (int)sizeof(S)); });
       if constexpr (POS > 0) {
         if (tid < KT && tid < left) {
-          pr[0] = load_pos(a.pos_k, (int64_t)k0 + tid, POS, 0);
-          if (POS == 2) pr[1] = load_pos(a.pos_k, (int64_t)k0 + tid, POS, 1);
+          pr[0] = a.pos_k[((int64_t)k0 + tid) * POS];
+          if (POS == 2) pr[1] = a.pos_k[((int64_t)k0 + tid) * POS + 1];
         }
       }
     };
     auto put_pos = [&](int buf) {
       if constexpr (POS > 0) {
         if (tid < KT) {
-          kpos[(buf * 2 + 0) * KT + tid] = pr[0];
-          if (POS == 2) kpos[(buf * 2 + 1) * KT + tid] = pr[1];
+          kpos[(buf * 2 + 0) * KT + tid] = to_pos(pr[0]);
+          if (POS == 2) kpos[(buf * 2 + 1) * KT + tid] = to_pos(pr[1]);
         }
       }
     };
@@ -202,11 +210,25 @@ dq_kernel(const Args a, int ntiles) {
         if (w.skip(k0, KT)) continue;
         const int rows = lane_base<CH>(rows0 + buf * 2 * TB);
         const int cols = lane_base<CH>(cols0 + buf * 2 * TB);
-        f32x16 z = row_dot<P, CH, KT>(lds, rows, qf);
-        const f32x16 dp = row_dot<P, CH, KT>(lds + TB, rows, gf);
+        f32x16 z, dp;
+        if constexpr (kTight) {
+          row_dot2<P, CH, KT>(
+              z, dp, lds, TB, rows, [&](int s) { return qf[0][s]; },
+              [&](int s) { return gf[0][s]; });
+        } else {
+          z = row_dot<P, CH, KT>(lds, rows, qf);
+          dp = row_dot<P, CH, KT>(lds + TB, rows, gf);
+        }
         const bool whole = w.whole(k0, KT);
         const unsigned n = w.r_hi - w.r_lo;
         const int j0 = k0 + 4 * h - w.r_lo;
+        int one = 0;
+        bool same = false;
+        float bias1 = 0.f, sum1 = 0.f;
+        if constexpr (POS == 1 && NW > 1) {
+          same = one_bucket<true>(bk, kpos + buf * 2 * KT, px, live, one);
+          if (same) bias1 = mytab[one];
+        }
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
           float v[4], t[4] = {0.f, 0.f, 0.f, 0.f};
@@ -221,17 +243,22 @@ dq_kernel(const Args a, int ntiles) {
             }
           }
           if constexpr (POS > 0) {
-            const int o = 8 * r4 + 4 * h;
-            const f32x4 kx =
-                *(const DGMC_LDS f32x4*)(kpos + (buf * 2 + 0) * KT + o);
-            f32x4 ky = kx;
-            if (POS == 2)
-              ky = *(const DGMC_LDS f32x4*)(kpos + (buf * 2 + 1) * KT + o);
+            if (same) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              sl[r] = bk.slot(kx[r] - px);
-              if (POS == 2) sl[r] = sl[r] * W + bk.slot(ky[r] - py);
-              v[r] += mytab[sl[r]];
+              for (int r = 0; r < 4; ++r) v[r] += bias1;
+            } else {
+              const int o = 8 * r4 + 4 * h;
+              const f32x4 kx =
+                  *(const DGMC_LDS f32x4*)(kpos + (buf * 2 + 0) * KT + o);
+              f32x4 ky = kx;
+              if (POS == 2)
+                ky = *(const DGMC_LDS f32x4*)(kpos + (buf * 2 + 1) * KT + o);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                sl[r] = bk.slot(kx[r] - px);
+                if (POS == 2) sl[r] = sl[r] * W + bk.slot(ky[r] - py);
+                v[r] += mytab[sl[r]];
+              }
             }
           }
 #pragma unroll
@@ -244,11 +271,15 @@ dq_kernel(const Args a, int ntiles) {
               if ((unsigned)(j0 + 8 * r4 + r) >= n) v[r] = t[r] = 0.f;
           }
           if constexpr (POS > 0) {
-            if (pass < w.b0) add_slots(myhist, sl, v);
+            if (same) sum1 += (v[0] + v[1]) + (v[2] + v[3]);
+            else if (pass < w.b0) add_slots(myhist, sl, v);
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             z[4 * r4 + r] = v[r] * fmaf(-t[r], t[r], 1.f);
+        }
+        if constexpr (POS == 1 && NW > 1) {
+          if (same && pass < w.b0) myhist[one * 64] += sum1;
         }
         P::template accum<DP, KT, NW == 1>(acc, lds, cols, z);
       }
@@ -298,7 +329,14 @@ dkv_kernel(const Args a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   DGMC_LDS char* lds = (DGMC_LDS char*)smem;
   DGMC_LDS float* rowv = (DGMC_LDS float*)(lds + 4 * TB);   // [2][4][QT]
-  DGMC_LDS float* tab = rowv + 8 * QT;                      // [G][kSlots]
+  DGMC_LDS int* toff = (DGMC_LDS int*)(rowv + 8 * QT);      // [QT]
+  // Wide heads: the lanes' own rows of V and the last KL chunks of K, too
+  // many for the registers (a spilled one's load in the loop waits for the
+  // next tile's, in order: 14 segments of 30 to 1350 nodes, 297 us; so 204).
+  constexpr bool VL = tight<P>(DP);
+  constexpr int KL = VL ? 2 : 0, OWN = VL ? CH / 2 + KL : 0;
+  DGMC_LDS u32x4* own = (DGMC_LDS u32x4*)(toff + QT);       // [OWN][NT]
+  DGMC_LDS float* tab = (DGMC_LDS float*)(own + OWN * NT);  // [G][kTab]
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int h = lane >> 5, c = lane & 31;
@@ -312,11 +350,18 @@ dkv_kernel(const Args a) {
   load_frags<P>(kf,
                 (const S*)a.k + (int64_t)k_lo * a.k_sn +
                     (int64_t)kvh * a.k_sh,
-                a.k_sp, ko * a.k_sn * (int64_t)sizeof(S), live, a.D, a.vec_k);
+                a.k_sp, ko * a.k_sn * (int64_t)sizeof(S), live, a.D);
   load_frags<P>(vf,
                 (const S*)a.v + (int64_t)k_lo * a.v_sn +
                     (int64_t)kvh * a.v_sh,
-                a.v_sp, ko * a.v_sn * (int64_t)sizeof(S), live, a.D, a.vec_v);
+                a.v_sp, ko * a.v_sn * (int64_t)sizeof(S), live, a.D);
+  if constexpr (VL) {
+#pragma unroll
+    for (int s = 0; s < CH / 2; ++s) own[s * NT + tid] = vf[0][s];
+#pragma unroll
+    for (int s = CH / 2 - KL; s < CH / 2; ++s)
+      own[(s + KL) * NT + tid] = kf[0][s];
+  }
   const int wrows = min(32, k_hi - k_lo - wave * 32);
   const Rows w = Rows::find<NW>(a.ptr_k, a.ptr_q, a.B, a.Nk, a.Nq, k_lo, k_hi,
                                 kj, wrows > 0 ? wrows - 1 : -1);
@@ -324,6 +369,7 @@ dkv_kernel(const Args a) {
   const int ntile = (w.hi - w.lo + QW - 1) / QW;
   const int per = split_tiles(a, ntile);
   if (split > 0 && split * per >= ntile) return;
+  put_splits(a, blockIdx.x, split, ntile, per);
   const int q_lo = w.lo + split * per * QW;
   const int q_hi = min(q_lo + per * QW, w.hi);
 
@@ -332,6 +378,7 @@ dkv_kernel(const Args a) {
   const int W = 2 * a.half + 2;
   if constexpr (POS > 0) {
     load_table(a, kvh, tab, POS);
+    if (tid < QT) toff[tid] = (tid - div_group(a, tid) * a.G) * kTab;
     if (live) {
       px = load_pos(a.pos_k, kj, POS, 0);
       if (POS == 2) py = load_pos(a.pos_k, kj, POS, 1);
@@ -340,7 +387,8 @@ dkv_kernel(const Args a) {
 
   const S* qbase = (const S*)a.q + (int64_t)kvh * a.G * a.q_sh;
   const S* gbase = (const S*)a.dout + (int64_t)kvh * a.G * a.g_sh;
-  float rv[4] = {INFINITY, 0.f, 0.f, 0.f};
+  float rv[2] = {INFINITY, 0.f};
+  int rp[2] = {0, 0};
   auto fetch = [&](int q0, int e, int buf) {
     using St = Stager<P, QT, CH, NT>;
     const int left = e - q0;
@@ -350,10 +398,7 @@ dkv_kernel(const Args a) {
       const int i = div_group(a, r);
       return (i * sn + (r - i * a.G) * sh) * (int64_t)sizeof(S);
     };
-    St::fill(qbase + (int64_t)q0 * a.q_sn, a.q_sp, a.D, a.vec_q, qt, ok,
-             [&](int r) { return off(r, a.q_sn, a.q_sh); });
-    St::fill(gbase + (int64_t)q0 * a.g_sn, a.g_sp, a.D, a.vec_g, qt + TB, ok,
-             [&](int r) { return off(r, a.g_sn, a.g_sh); });
+    // (first: a wait among these few is not one for the tile)
     if (tid < QT) {
       const int i = div_group(a, tid), qi = q0 + i;
       const bool there = tid < RW && qi < e;
@@ -361,16 +406,22 @@ dkv_kernel(const Args a) {
       rv[0] = there ? a.lse[row] : INFINITY;   // p = 0 in a row not there
       rv[1] = there ? a.delta[row] : 0.f;
       if (POS > 0) {
-        rv[2] = there ? load_pos(a.pos_q, qi, POS, 0) : 0.f;
-        if (POS == 2) rv[3] = there ? load_pos(a.pos_q, qi, POS, 1) : 0.f;
+        // (rows not there: the first one's)
+        const int64_t i = there ? qi : q0;
+        rp[0] = a.pos_q[i * POS];
+        if (POS == 2) rp[1] = a.pos_q[i * POS + 1];
       }
     }
+    St::fill(qbase + (int64_t)q0 * a.q_sn, a.q_sp, a.D, qt, ok,
+             [&](int r) { return off(r, a.q_sn, a.q_sh); });
+    St::fill(gbase + (int64_t)q0 * a.g_sn, a.g_sp, a.D, qt + TB, ok,
+             [&](int r) { return off(r, a.g_sn, a.g_sh); });
   };
   auto put_rows = [&](int buf) {
     if (tid < QT) {
 #pragma unroll
       for (int k = 0; k < 2 + POS; ++k)
-        rowv[(buf * 4 + k) * QT + tid] = rv[k];
+        rowv[(buf * 4 + k) * QT + tid] = k < 2 ? rv[k] : to_pos(rp[k - 2]);
     }
   };
   const bool capped = a.cap > 0.f;
@@ -395,11 +446,25 @@ dkv_kernel(const Args a) {
       const DGMC_LDS float* rw = rowv + buf * 4 * QT;
       const int rows = lane_base<CH>(rows0 + buf * 2 * TB);
       const int cols = lane_base<CH>(cols0 + buf * 2 * TB);
-      f32x16 z = row_dot<P, CH, QT>(lds, rows, kf);
-      f32x16 dp = row_dot<P, CH, QT>(lds + TB, rows, vf);
+      f32x16 z, dp;
+      if constexpr (VL) {
+        row_dot2<P, CH, QT>(
+            z, dp, lds, TB, rows,
+            [&](int s) {
+              return s < CH / 2 - KL ? kf[0][s] : own[(s + KL) * NT + tid];
+            },
+            [&](int s) { return own[s * NT + tid]; });
+      } else {
+        z = row_dot<P, CH, QT>(lds, rows, kf);
+        dp = row_dot<P, CH, QT>(lds + TB, rows, vf);
+      }
       const bool whole = w.whole(q0, QW);
       const unsigned n = (w.r_hi - w.r_lo) * a.G;
       const int j0 = (q0 - w.r_lo) * a.G + 4 * h;
+      int one = 0;
+      bool same = false;
+      if constexpr (POS == 1 && NW > 1)
+        same = one_bucket<false>(bk, rw + 2 * QT, px, live, one);
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
         const int o = 8 * r4 + 4 * h;
@@ -416,17 +481,21 @@ dkv_kernel(const Args a) {
           }
         }
         if constexpr (POS > 0) {
-          const f32x4 qx = *(const DGMC_LDS f32x4*)(rw + 2 * QT + o);
-          f32x4 qy = qx;
-          if (POS == 2) qy = *(const DGMC_LDS f32x4*)(rw + 3 * QT + o);
+          // (toff: the row's head's table)
+          const i32x4 to = *(const DGMC_LDS i32x4*)(toff + o);
+          if (same) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            int s = bk.slot(px - qx[r]);
-            if (POS == 2) s = s * W + bk.slot(py - qy[r]);
-            // (the row's head: its table)
-            const int i = o + r;
-            if (a.G > 1) s += (i - div_group(a, i) * a.G) * kSlots;
-            p[r] += tab[s];
+            for (int r = 0; r < 4; ++r) p[r] += tab[one + to[r]];
+          } else {
+            const f32x4 qx = *(const DGMC_LDS f32x4*)(rw + 2 * QT + o);
+            f32x4 qy = qx;
+            if (POS == 2) qy = *(const DGMC_LDS f32x4*)(rw + 3 * QT + o);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              int s = bk.slot(px - qx[r]);
+              if (POS == 2) s = s * W + bk.slot(py - qy[r]);
+              p[r] += tab[s + to[r]];
+            }
           }
         }
 #pragma unroll
@@ -474,7 +543,7 @@ void launch_dq(const Args& a, int axes, int nblk, hipStream_t st) {
   constexpr int B = P::kPlanes * (int)sizeof(typename P::S);
   const int TQ = 32 / a.G * NW, ntiles = (a.Nq + TQ - 1) / TQ;
   const size_t sm = 4 * 32 * DP * B +
-                    (axes ? 16 * 32 + a.G * kSlots * 4 +
+                    (axes ? 16 * 32 + a.G * kTab * 4 +
                                 (size_t)NW * a.slots * 256 : 0);
   auto kern = axes == 0   ? dq_kernel<P, DP, NW, 0>
               : axes == 1 ? dq_kernel<P, DP, NW, 1>
@@ -488,8 +557,9 @@ void launch_dq(const Args& a, int axes, int nblk, hipStream_t st) {
 template <typename P, int DP, int NW>
 void launch_dkv(const Args& a, int axes, hipStream_t st) {
   constexpr int B = P::kPlanes * (int)sizeof(typename P::S);
-  const size_t sm =
-      4 * 32 * DP * B + 8 * 32 * 4 + (axes ? a.G * kSlots * 4 : 0);
+  const size_t sm = 4 * 32 * DP * B + 9 * 32 * 4 +
+                    (tight<P>(DP) ? (8 + 2) * NW * 64 * 16 : 0) +
+                    (axes ? a.G * kTab * 4 : 0);
   auto kern = axes == 0   ? dkv_kernel<P, DP, NW, 0>
               : axes == 1 ? dkv_kernel<P, DP, NW, 1>
                           : dkv_kernel<P, DP, NW, 2>;

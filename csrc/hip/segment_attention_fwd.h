@@ -40,7 +40,7 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
   extern __shared__ __attribute__((aligned(16))) char smem[];
   DGMC_LDS char* lds = (DGMC_LDS char*)smem;
   DGMC_LDS float* kpos = (DGMC_LDS float*)(lds + 4 * TB);   // [2][2][KT]
-  DGMC_LDS float* tab = kpos + (POS ? 4 * KT : 0);          // [G][kSlots]
+  DGMC_LDS float* tab = kpos + (POS ? 4 * KT : 0);          // [G][kTab]
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int h = lane >> 5, c = lane & 31;
@@ -58,7 +58,7 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
                 (const S*)a.q + (int64_t)q_lo * a.q_sn +
                     (int64_t)kvh * a.G * a.q_sh,
                 a.q_sp, (qo * a.q_sn + g * a.q_sh) * (int64_t)sizeof(S), live,
-                a.D, a.vec_q);
+                a.D);
   const int wrows = min(QW, q_hi - q_lo - wave * QW);
   const Rows w = Rows::find<NW>(a.ptr_q, a.ptr_k, a.B, a.Nq, a.Nk, q_lo, q_hi,
                                 qi, wrows > 0 ? (wrows - 1) * a.G : -1);
@@ -66,6 +66,7 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
   const int ntile = (w.hi - w.lo + KT - 1) / KT;
   const int per = split_tiles(a, ntile);
   if (split > 0 && split * per >= ntile) return;
+  put_splits(a, blockIdx.x, split, ntile, per);
   const int k_lo = w.lo + split * per * KT;
   const int k_hi = min(k_lo + per * KT, w.hi);
 
@@ -78,12 +79,12 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
       if (POS == 2) py = load_pos(a.pos_q, qi, POS, 1);
     }
   }
-  const DGMC_LDS float* mytab = tab + g * kSlots;
+  const DGMC_LDS float* mytab = tab + g * kTab;
   const int W = 2 * a.half + 2;
 
   const S* kbase = (const S*)a.k + (int64_t)kvh * a.k_sh;
   const S* vbase = (const S*)a.v + (int64_t)kvh * a.v_sh;
-  float pr[2] = {0.f, 0.f};
+  int pr[2] = {0, 0};
   // Start the loads of keys [k0, e) into buffer `buf`; their positions wait
   // in registers.
   auto fetch = [&](int k0, int e, int buf) {
@@ -91,22 +92,22 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
     const int left = e - k0;
     DGMC_LDS char* kt = lds + buf * 2 * TB;
     const auto ok = [&](int r) { return r < left; };
-    St::fill(kbase + (int64_t)k0 * a.k_sn, a.k_sp, a.D, a.vec_k, kt, ok,
+    St::fill(kbase + (int64_t)k0 * a.k_sn, a.k_sp, a.D, kt, ok,
              [&](int r) { return r * (a.k_sn * (int)sizeof(S)); });
-    St::fill(vbase + (int64_t)k0 * a.v_sn, a.v_sp, a.D, a.vec_v, kt + TB, ok,
+    St::fill(vbase + (int64_t)k0 * a.v_sn, a.v_sp, a.D, kt + TB, ok,
              [&](int r) { return r * (a.v_sn * (int)sizeof(S)); });
     if constexpr (POS > 0) {
       if (tid < KT && tid < left) {
-        pr[0] = load_pos(a.pos_k, (int64_t)k0 + tid, POS, 0);
-        if (POS == 2) pr[1] = load_pos(a.pos_k, (int64_t)k0 + tid, POS, 1);
+        pr[0] = a.pos_k[((int64_t)k0 + tid) * POS];
+        if (POS == 2) pr[1] = a.pos_k[((int64_t)k0 + tid) * POS + 1];
       }
     }
   };
   auto put_pos = [&](int buf) {
     if constexpr (POS > 0) {
       if (tid < KT) {
-        kpos[(buf * 2 + 0) * KT + tid] = pr[0];
-        if (POS == 2) kpos[(buf * 2 + 1) * KT + tid] = pr[1];
+        kpos[(buf * 2 + 0) * KT + tid] = to_pos(pr[0]);
+        if (POS == 2) kpos[(buf * 2 + 1) * KT + tid] = to_pos(pr[1]);
       }
     }
   };
@@ -156,6 +157,16 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
       if constexpr (POS > 0) {
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u) {
+          if constexpr (POS == 1 && NW > 1) {
+            int s;
+            if (one_bucket<true>(bk, kpos + buf * 2 * KT + 32 * u, px, live,
+                                 s)) {
+              const float t = mytab[s];
+#pragma unroll
+              for (int r = 0; r < 16; ++r) z[u][r] += t;
+              continue;
+            }
+          }
 #pragma unroll
           for (int r4 = 0; r4 < 4; ++r4) {
             const int row = 32 * u + 8 * r4 + 4 * h;
@@ -254,7 +265,7 @@ void launch_fwd(const Args& a, int axes, hipStream_t st) {
   constexpr int KT = fwd_keys(DP, NW, B);
   const int TQ = 32 / a.G * NW;
   const dim3 grid((a.Nq + TQ - 1) / TQ * a.KV, a.splits), blk(NW * 64);
-  const size_t sm = 4 * KT * DP * B + (axes ? 16 * KT + a.G * kSlots * 4 : 0);
+  const size_t sm = 4 * KT * DP * B + (axes ? 16 * KT + a.G * kTab * 4 : 0);
   auto kern = axes == 0   ? fwd_kernel<P, DP, NW, KT, 0, FINE>
               : axes == 1 ? fwd_kernel<P, DP, NW, KT, 1, FINE>
                           : fwd_kernel<P, DP, NW, KT, 2, FINE>;

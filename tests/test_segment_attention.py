@@ -527,6 +527,45 @@ def test_offsets_past_32_bits():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('H,KV,D', [(1, 1, 128), (2, 1, 32), (3, 1, 64)])
+def test_positions_in_order(dtype, H, KV, D):
+    """Nodes in order, as a node ordering numbers them: whole blocks of
+    pairs share a bucket, others cross from one to the next.  (400 keys: the
+    sums of the table's gradient have 200 terms a lane and 256 columns, fewer
+    than the n + 80 roundings its tolerance holds.)"""
+    st = _case([400], None, H, KV, D, dtype, axes=1, half=7)
+    for order in (torch.arange(400), torch.arange(400).flip(0) * 3 - 700):
+        st['pos_q'] = st['pos_k'] = order.int().view(-1, 1)
+        for steps in (1, 2):
+            val, tol = _plain(st, cap=2.0, half=7, steps=steps)
+            _close(_run(st, 'cuda', cap=2.0, steps=steps), val, tol)
+
+
+@pytest.mark.gpu
+def test_tiles_wider_than_a_buffers_range():
+    """Row strides at which 64 rows of a tile stay within 2^31 bytes and 128
+    do not."""
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip('needs 16 GB')
+    n, stride = 200, 10 << 20
+    base = torch.empty(n * stride, dtype=torch.bfloat16, device='cuda')
+    wide = base.as_strided((n, 1, 32), (stride, 32, 1))
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(n, 1, 32, generator=g).to(torch.bfloat16).cuda()
+    wide.copy_(x)
+    ptr = torch.tensor([0, n], dtype=torch.int32, device='cuda')
+
+    def run(t):
+        leaf = t.detach().requires_grad_(True)
+        out = segment_attention(leaf, leaf, leaf, ptr)
+        return out, torch.autograd.grad(out, leaf, x)[0]
+
+    for a, b in zip(run(wide), run(x)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_second_derivatives_are_refused():
     q = torch.randn(5, 1, 16, device='cuda', requires_grad=True)
     ptr = torch.tensor([0, 5], dtype=torch.int32, device='cuda')
