@@ -88,6 +88,7 @@ struct Args {
   float scale, cap, dmax, dmul;
   int vec_o;                          // o has 16-byte rows
   int splits, chunk;                  // most splits, least tiles of one
+  int bufs;                           // see stage_bufs
 };
 
 // Tiles of one split of an axis of n tiles: an even share of the splits, at
@@ -777,6 +778,16 @@ __device__ __forceinline__ float to_pos(int p) {
 __device__ __forceinline__ float load_pos(const int* pos, int64_t i, int axes,
                                           int axis) {
   return to_pos(pos[i * axes + axis]);
+}
+
+// LDS buffers of the staged tiles: two, or (a.bufs) one where a wave walks
+// the few fp32 tiles of short segments alone - what it then waits for them is
+// less than what the waves gain that fit beside it (1024 graphs of 3 to 19
+// nodes, heads of 64: forward 37 -> 26 us, dkv 46 -> 39; heads of 128: dq 190
+// -> 81).  Few rows of long segments stream through two.
+template <typename P, int NW>
+__device__ __forceinline__ int stage_bufs(const Args& a) {
+  return NW == 1 && sizeof(typename P::S) == 4 ? a.bufs : 2;
 }
 
 // Keys of a forward tile: 64 where four waves share it and both buffers of K

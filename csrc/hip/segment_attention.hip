@@ -385,6 +385,14 @@ static int waves_for(int64_t rows, int64_t B) {
   return rows > 64 * std::max<int64_t>(B, 1) ? 4 : 1;
 }
 
+// See stage_bufs.
+static void pick_bufs(Args& a, bool f32) {
+  a.bufs = f32 && waves_for((int64_t)a.Nq * a.G, a.B) == 1 &&
+                   waves_for(a.Nk, a.B) == 1
+               ? 1
+               : 2;
+}
+
 // Whether an fp32 call takes the x6 kernels: long segments on both sides (the
 // planes cost a pass over the tensors and 1.5 times their memory), heads of
 // up to 64 (wider ones' planes exceed the LDS beside the table's columns).
@@ -449,11 +457,14 @@ static at::Tensor make_copies(Args& a, bool six, const at::Tensor& q,
 // (knowledge graphs' evaluation, 4 a SIMD: 1024 workgroups 540 us, 2048 516;
 // 2 a SIMD: 1024 444 us of the ragged case, 1536 509, 768 487), no split
 // under 16 tiles (ragged case: 8 650 us, 16 604, 32 659), 8 where one wave
-// walks them (new entities: 16 44 us, 8 35).  False: none.
+// walks them (new entities: 16 44 us, 8 35).  None where the mean segment is
+// short: a join with nothing to join takes 4 us.  False: none.
 static bool split_axis(Args& a, int64_t tiles, int64_t n, int tile, int nw,
                        int waves) {
   tiles = std::max<int64_t>(tiles, 1) * a.KV;
   a.chunk = nw == 4 ? 16 : 8;
+  a.splits = 1;
+  if (waves_for(n, a.B) == 1) return false;
   a.splits = (int)std::max<int64_t>(
       1, std::min<int64_t>({(512 * waves + tiles - 1) / tiles,
                             n / ((int64_t)tile * a.chunk), kMaxSplits}));
@@ -498,6 +509,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> forward(
   a.lse = train ? lse.data_ptr<float>() : nullptr;
   const int nw = waves_for((int64_t)a.Nq * a.G, a.B);
   const bool six = f && takes_x6(a, x6);
+  pick_bufs(a, f);
   const int DP = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
   const int TQ = 32 / a.G * nw,
             KT = fwd_keys(DP, nw, six ? 6 : f ? 4 : 2);
@@ -565,6 +577,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
   const int nwk = waves_for(a.Nk, a.B);
   const int TQ = 32 / a.G * nwq;
   const bool six = f && takes_x6(a, x6);
+  pick_bufs(a, f);
   at::Tensor pq, pk;
   const at::Tensor ws = make_copies(a, six, q, k, v, dout);
   if (split_axis(a, a.Nq / TQ, a.Nk, 32, nwq, 2))

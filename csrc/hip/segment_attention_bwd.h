@@ -16,9 +16,9 @@
 // are not what takes the time).
 //
 // The table's gradient: every lane adds its dz into its own LDS column of
-// [slots][64] (no address is shared: no conflicts and a fixed order); a
-// workgroup keeps its columns over all the tiles it walks and sums them
-// once, a last kernel adds the workgroups' parts in order.
+// [slots][64] (no address is shared at a time: no conflicts and a fixed
+// order); a workgroup keeps its columns over all the tiles it walks and sums
+// them once, a last kernel adds the workgroups' parts in order.
 #pragma once
 
 #include "segment_attention.h"
@@ -32,24 +32,45 @@ namespace segattn {
 // the four take the earlier ones' values along and the last write counts;
 // where all four are one slot in every lane (nodes in order, far apart) they
 // are added first.
+//
+// HC = 32: lanes l and l ^ 32 (one query's) share a column, one half of the
+// wave after the other - half the LDS, and the waves that fit beside it are
+// what a short segment's time depends on.
+template <int HC>
 __device__ __forceinline__ void add_slots(DGMC_LDS float* hist,
                                           const int (&sl)[4],
                                           const float (&v)[4]) {
   const int a = sl[0], b = sl[1], c = sl[2], d = sl[3];
+  const auto halves = [&](auto add) {
+    if constexpr (HC == 64) {
+      add();
+    } else {
+      if ((threadIdx.x & 32) == 0) add();
+      asm volatile("" ::: "memory");     // (one thread's two cases are two)
+      if ((threadIdx.x & 32) != 0) add();
+      asm volatile("" ::: "memory");
+    }
+  };
   if (__all(a == b && b == c && c == d)) {
-    hist[a * 64] += (v[0] + v[1]) + (v[2] + v[3]);
+    const float all = (v[0] + v[1]) + (v[2] + v[3]);
+    halves([&] { hist[a * HC] += all; });
     return;
   }
-  const float ha = hist[a * 64], hb = hist[b * 64], hc = hist[c * 64],
-              hd = hist[d * 64];
   const float va = v[0], vb = v[1] + (a == b ? va : 0.f);
   const float vc = v[2] + (b == c ? vb : a == c ? va : 0.f);
   const float vd = v[3] + (c == d ? vc : b == d ? vb : a == d ? va : 0.f);
-  hist[a * 64] = ha + va;
-  hist[b * 64] = hb + vb;
-  hist[c * 64] = hc + vc;
-  hist[d * 64] = hd + vd;
+  halves([&] {
+    const float ha = hist[a * HC], hb = hist[b * HC], hc = hist[c * HC],
+                hd = hist[d * HC];
+    hist[a * HC] = ha + va;
+    hist[b * HC] = hb + vb;
+    hist[c * HC] = hc + vc;
+    hist[d * HC] = hd + vd;
+  });
 }
+
+// Columns of a wave's table sums.
+constexpr int hist_cols(int nw) { return nw == 1 ? 32 : 64; }
 
 // Wide heads at two waves per SIMD: registers are short.
 template <typename P>
@@ -59,7 +80,8 @@ constexpr bool tight(int DP) {
 
 template <typename P, int DP, int NW, int POS>
 __global__ __launch_bounds__(
-    NW * 64, sizeof(typename P::S) == 2 ? 2 : 1) void
+    NW * 64,
+    sizeof(typename P::S) == 2 || (NW == 1 && DP <= 64) ? 2 : 1) void
 dq_kernel(const Args a, int ntiles) {
   using T = typename P::T;
   using S = typename P::S;
@@ -70,9 +92,11 @@ dq_kernel(const Args a, int ntiles) {
   constexpr int TB = P::kPlanes * KT * CH * 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   DGMC_LDS char* lds = (DGMC_LDS char*)smem;
-  DGMC_LDS float* kpos = (DGMC_LDS float*)(lds + 4 * TB);   // [2][2][KT]
-  DGMC_LDS float* tab = kpos + (POS ? 4 * KT : 0);          // [G][kTab]
-  DGMC_LDS float* hist = tab + (POS ? a.G * kTab : 0);    // [NW][slots][64]
+  const int NB = stage_bufs<P, NW>(a);
+  DGMC_LDS float* kpos = (DGMC_LDS float*)(lds + 2 * NB * TB);  // [NB][2][KT]
+  DGMC_LDS float* tab = kpos + (POS ? 2 * NB * KT : 0);          // [G][kTab]
+  DGMC_LDS float* hist = tab + (POS ? a.G * kTab : 0);    // [NW][slots][HC]
+  constexpr int HC = hist_cols(NW);
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int h = lane >> 5, c = lane & 31;
@@ -83,10 +107,10 @@ dq_kernel(const Args a, int ntiles) {
   const int head = kvh * a.G + g, qo = wave * QW + cq;
   const Bucket bk(a);
   const DGMC_LDS float* mytab = tab + g * kTab;
-  DGMC_LDS float* myhist = hist + wave * a.slots * 64 + lane;
+  DGMC_LDS float* myhist = hist + wave * a.slots * HC + (lane & (HC - 1));
   if constexpr (POS > 0) {
     load_table(a, kvh, tab, POS);
-    for (int s = 0; s < a.slots; ++s) myhist[s * 64] = 0.f;
+    for (int s = 0; s < a.slots; ++s) myhist[s * HC] = 0.f;
   }
   const S* kbase = (const S*)a.k + (int64_t)kvh * a.k_sh;
   const S* vbase = (const S*)a.v + (int64_t)kvh * a.v_sh;
@@ -203,10 +227,14 @@ dq_kernel(const Args a, int ntiles) {
       for (int k = 0; k < DP / 32; ++k) acc[k] = f32x16{};
       stage_barrier();     // the last tile staged before has been read
       if (p_lo < p_hi) fetch(p_lo, p_hi, 0);
-      for (int k0 = p_lo, buf = 0; k0 < p_hi; k0 += KT, buf ^= 1) {
+      for (int k0 = p_lo, buf = 0; k0 < p_hi; k0 += KT, buf ^= NB - 1) {
+        if (NB == 1 && k0 > p_lo) {
+          stage_barrier();
+          fetch(k0, p_hi, 0);
+        }
         put_pos(buf);
         stage_barrier();
-        if (k0 + KT < p_hi) fetch(k0 + KT, p_hi, buf ^ 1);
+        if (NB == 2 && k0 + KT < p_hi) fetch(k0 + KT, p_hi, buf ^ 1);
         if (w.skip(k0, KT)) continue;
         const int rows = lane_base<CH>(rows0 + buf * 2 * TB);
         const int cols = lane_base<CH>(cols0 + buf * 2 * TB);
@@ -272,14 +300,14 @@ dq_kernel(const Args a, int ntiles) {
           }
           if constexpr (POS > 0) {
             if (same) sum1 += (v[0] + v[1]) + (v[2] + v[3]);
-            else if (pass < w.b0) add_slots(myhist, sl, v);
+            else if (pass < w.b0) add_slots<HC>(myhist, sl, v);
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             z[4 * r4 + r] = v[r] * fmaf(-t[r], t[r], 1.f);
         }
         if constexpr (POS == 1 && NW > 1) {
-          if (same && pass < w.b0) myhist[one * 64] += sum1;
+          if (same && pass < w.b0) myhist[one * HC] += sum1;
         }
         P::template accum<DP, KT, NW == 1>(acc, lds, cols, z);
       }
@@ -297,7 +325,7 @@ dq_kernel(const Args a, int ntiles) {
   }
   if constexpr (POS > 0) {
     // Columns of this workgroup in a fixed order, started at a lane's own
-    // (64 different banks).
+    // (different banks).
     __syncthreads();
     const int RW = QW * a.G;
     for (int e = tid; e < a.G * a.slots; e += NT) {
@@ -305,9 +333,9 @@ dq_kernel(const Args a, int ntiles) {
       float sum = 0.f;
       for (int wv = 0; wv < NW; ++wv) {
 #pragma unroll 8
-        for (int j = 0; j < 64; ++j) {
-          const int col = (j + s) & 63, cc = col & 31;
-          const float x = hist[(wv * a.slots + s) * 64 + col];
+        for (int j = 0; j < HC; ++j) {
+          const int col = (j + s) & (HC - 1), cc = col & 31;
+          const float x = hist[(wv * a.slots + s) * HC + col];
           sum += cc < RW && cc - div_group(a, cc) * a.G == gg ? x : 0.f;
         }
       }
@@ -318,7 +346,8 @@ dq_kernel(const Args a, int ntiles) {
 
 template <typename P, int DP, int NW, int POS>
 __global__ __launch_bounds__(
-    NW * 64, sizeof(typename P::S) == 2 ? 2 : 1) void
+    NW * 64,
+    sizeof(typename P::S) == 2 || (NW == 1 && DP <= 64) ? 2 : 1) void
 dkv_kernel(const Args a) {
   using T = typename P::T;
   using S = typename P::S;
@@ -328,8 +357,9 @@ dkv_kernel(const Args a) {
   constexpr int TB = P::kPlanes * QT * CH * 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   DGMC_LDS char* lds = (DGMC_LDS char*)smem;
-  DGMC_LDS float* rowv = (DGMC_LDS float*)(lds + 4 * TB);   // [2][4][QT]
-  DGMC_LDS int* toff = (DGMC_LDS int*)(rowv + 8 * QT);      // [QT]
+  const int NB = stage_bufs<P, NW>(a);
+  DGMC_LDS float* rowv = (DGMC_LDS float*)(lds + 2 * NB * TB);  // [NB][4][QT]
+  DGMC_LDS int* toff = (DGMC_LDS int*)(rowv + 4 * NB * QT);     // [QT]
   // Wide heads: the lanes' own rows of V and the last KL chunks of K, too
   // many for the registers (a spilled one's load in the loop waits for the
   // next tile's, in order: 14 segments of 30 to 1350 nodes, 297 us; so 204).
@@ -438,10 +468,14 @@ dkv_kernel(const Args a) {
     for (int k = 0; k < DP / 32; ++k) ak[k] = av[k] = f32x16{};
     if (pass >= w.b0) stage_barrier();
     if (p_lo < p_hi) fetch(p_lo, p_hi, 0);
-    for (int q0 = p_lo, buf = 0; q0 < p_hi; q0 += QW, buf ^= 1) {
+    for (int q0 = p_lo, buf = 0; q0 < p_hi; q0 += QW, buf ^= NB - 1) {
+      if (NB == 1 && q0 > p_lo) {
+        stage_barrier();
+        fetch(q0, p_hi, 0);
+      }
       put_rows(buf);
       stage_barrier();
-      if (q0 + QW < p_hi) fetch(q0 + QW, p_hi, buf ^ 1);
+      if (NB == 2 && q0 + QW < p_hi) fetch(q0 + QW, p_hi, buf ^ 1);
       if (w.skip(q0, QW)) continue;
       const DGMC_LDS float* rw = rowv + buf * 4 * QT;
       const int rows = lane_base<CH>(rows0 + buf * 2 * TB);
@@ -542,9 +576,11 @@ template <typename P, int DP, int NW>
 void launch_dq(const Args& a, int axes, int nblk, hipStream_t st) {
   constexpr int B = P::kPlanes * (int)sizeof(typename P::S);
   const int TQ = 32 / a.G * NW, ntiles = (a.Nq + TQ - 1) / TQ;
-  const size_t sm = 4 * 32 * DP * B +
-                    (axes ? 16 * 32 + a.G * kTab * 4 +
-                                (size_t)NW * a.slots * 256 : 0);
+  const int NB = NW == 1 ? a.bufs : 2;
+  const size_t sm = NB * (2 * 32 * DP * B + (axes ? 8 * 32 : 0)) +
+                    (axes ? a.G * kTab * 4 +
+                                (size_t)NW * a.slots * hist_cols(NW) * 4
+                          : 0);
   auto kern = axes == 0   ? dq_kernel<P, DP, NW, 0>
               : axes == 1 ? dq_kernel<P, DP, NW, 1>
                           : dq_kernel<P, DP, NW, 2>;
@@ -557,7 +593,8 @@ void launch_dq(const Args& a, int axes, int nblk, hipStream_t st) {
 template <typename P, int DP, int NW>
 void launch_dkv(const Args& a, int axes, hipStream_t st) {
   constexpr int B = P::kPlanes * (int)sizeof(typename P::S);
-  const size_t sm = 4 * 32 * DP * B + 9 * 32 * 4 +
+  const int NB = NW == 1 ? a.bufs : 2;
+  const size_t sm = NB * (2 * 32 * DP * B + 4 * 32 * 4) + 32 * 4 +
                     (tight<P>(DP) ? (8 + 2) * NW * 64 * 16 : 0) +
                     (axes ? a.G * kTab * 4 : 0);
   auto kern = axes == 0   ? dkv_kernel<P, DP, NW, 0>

@@ -39,8 +39,9 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
   constexpr int UB = 32 * CH * 16;               // bytes of 32 rows
   extern __shared__ __attribute__((aligned(16))) char smem[];
   DGMC_LDS char* lds = (DGMC_LDS char*)smem;
-  DGMC_LDS float* kpos = (DGMC_LDS float*)(lds + 4 * TB);   // [2][2][KT]
-  DGMC_LDS float* tab = kpos + (POS ? 4 * KT : 0);          // [G][kTab]
+  const int NB = stage_bufs<P, NW>(a);
+  DGMC_LDS float* kpos = (DGMC_LDS float*)(lds + 2 * NB * TB);  // [NB][2][KT]
+  DGMC_LDS float* tab = kpos + (POS ? 2 * NB * KT : 0);          // [G][kTab]
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int h = lane >> 5, c = lane & 31;
@@ -130,10 +131,14 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
     float m = -INFINITY, l = 0.f;
     if (pass >= w.b0) stage_barrier();
     if (p_lo < p_hi) fetch(p_lo, p_hi, 0);
-    for (int k0 = p_lo, buf = 0; k0 < p_hi; k0 += KT, buf ^= 1) {
+    for (int k0 = p_lo, buf = 0; k0 < p_hi; k0 += KT, buf ^= NB - 1) {
+      if (NB == 1 && k0 > p_lo) {
+        stage_barrier();
+        fetch(k0, p_hi, 0);
+      }
       put_pos(buf);
       stage_barrier();
-      if (k0 + KT < p_hi) fetch(k0 + KT, p_hi, buf ^ 1);
+      if (NB == 2 && k0 + KT < p_hi) fetch(k0 + KT, p_hi, buf ^ 1);
       if (w.skip(k0, KT)) continue;
       const int rows = lane_base<CH>(rows0 + buf * 2 * TB);
       const int cols = lane_base<CH>(cols0 + buf * 2 * TB);
@@ -265,7 +270,9 @@ void launch_fwd(const Args& a, int axes, hipStream_t st) {
   constexpr int KT = fwd_keys(DP, NW, B);
   const int TQ = 32 / a.G * NW;
   const dim3 grid((a.Nq + TQ - 1) / TQ * a.KV, a.splits), blk(NW * 64);
-  const size_t sm = 4 * KT * DP * B + (axes ? 16 * KT + a.G * kTab * 4 : 0);
+  const int NB = NW == 1 ? a.bufs : 2;
+  const size_t sm =
+      NB * (2 * KT * DP * B + (axes ? 8 * KT : 0)) + (axes ? a.G * kTab * 4 : 0);
   auto kern = axes == 0   ? fwd_kernel<P, DP, NW, KT, 0, FINE>
               : axes == 1 ? fwd_kernel<P, DP, NW, KT, 1, FINE>
                           : fwd_kernel<P, DP, NW, KT, 2, FINE>;
