@@ -139,7 +139,8 @@ __device__ __forceinline__ int lane_segment(const int* ptr, int B, int N,
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1)
       if (__shfl(e, n + s - 1) <= row) n += s;
-    if (n == 63 && __shfl(e, 63) <= row) n = 64;
+    // (readlane: a shuffle in this condition needs lane 63 to be in it)
+    if (n == 63 && __builtin_amdgcn_readlane(e, 63) <= row) n = 64;
     seg += n;
     if (!__any(n == 64)) return seg;
   }
