@@ -584,7 +584,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
     pq = part_workspace(a, (int64_t)a.Nq * a.H, 1, false,
                         (a.Nq + TQ - 1) / TQ, q);
   // Workgroups of the dq kernel with a table: each keeps its LDS columns
-  // over all of its tiles.
+  // over all of its tiles.  2048 waves: ragged case 149 us (1024 222, 4096
+  // 168), one graph of 4096 nodes 222 (331, 248).
   int nblk = 0;
   at::Tensor part;
   if (axes) {
