@@ -220,6 +220,27 @@ def test_dgmc_log_probs_match_forward_on_the_gpu(k):
     _check_dgmc('cuda', k)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('k', [-1, 3])
+def test_dgmc_log_probs_under_autocast(k):
+    """The scores of the model's own bf16 path: the same as its
+    probabilities'."""
+    torch.manual_seed(0)
+    model = DGMC(GIN(16, 16, 2), GIN(8, 8, 2), num_steps=2, k=k).cuda().eval()
+    args, y = _graphs('cuda')
+    with torch.no_grad(), torch.autocast('cuda', torch.bfloat16):
+        torch.manual_seed(1)
+        S = model(*args)
+        torch.manual_seed(1)
+        res = model.log_probs(*args, y_col=y, top=2)
+    for s, r in zip(S, res):
+        p = s.to_dense() if s.is_sparse else s
+        best = p.max(dim=-1).values.double()
+        # (both softmaxes are fp32 on the same scores)
+        assert (r.top_log_prob[:, 0].double().exp() - best).abs().max() < \
+            64 * 2 ** -24
+
+
 def test_dgmc_log_probs_train_and_refuse_sinkhorn():
     args, y = _graphs('cpu')
     model = DGMC(GIN(16, 16, 2), GIN(8, 8, 2), num_steps=1)

@@ -566,6 +566,73 @@ def test_tiles_wider_than_a_buffers_range():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('D', [5, 20, 66])
+def test_padded_copies(dtype, D):
+    """Rows that are no 16-byte chunks: few rows over long segments (split
+    keys), long rows over few, and the step captured and replayed."""
+    for lq, lk in (([2, 0, 1], [900, 7, 1400]), ([300], [40])):
+        st = _case(lq, lk, 2, 1, D, dtype, axes=1, half=3, tail=2)
+        val, tol = _plain(st, cap=3.0, half=3)
+        _close(_run(st, 'cuda', cap=3.0), val, tol)
+    dev = {n: t.cuda() for n, t in st.items()}
+    leaves = [dev[n].requires_grad_(True) for n in ('q', 'k', 'v')]
+
+    def step():
+        out = segment_attention(*leaves, dev['ptr_q'], dev['ptr_k'])
+        return [out.detach()] + list(
+            torch.autograd.grad(out, leaves, dev['do']))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for seed in range(3):
+        with torch.no_grad():
+            for t in leaves:
+                t.mul_(0.9).add_(0.1 * seed)
+        eager = [t.clone() for t in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, eager):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_two_captured_graphs_and_eager_calls_share_nothing():
+    """Two captured calls with split keys and one eager call, replayed in
+    turn: no workspace of one is another's."""
+    st = [_case([2, 1], [3000, 2500], 4, 1, 64, torch.bfloat16, seed=s)
+          for s in range(3)]
+    dev = [{n: t.cuda() for n, t in d.items() if t is not None} for d in st]
+
+    def call(d):
+        return segment_attention(d['q'], d['k'], d['v'], d['ptr_q'],
+                                 d['ptr_k'])
+
+    want = [call(d).clone() for d in dev]
+    graphs, outs = [], []
+    for d in dev[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(d))
+        graphs.append(g)
+    for _ in range(3):
+        graphs[1].replay()
+        graphs[0].replay()
+        e = call(dev[2])
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0])
+        assert torch.equal(outs[1], want[1])
+        assert torch.equal(e, want[2])
+
+
+@pytest.mark.gpu
 def test_second_derivatives_are_refused():
     q = torch.randn(5, 1, 16, device='cuda', requires_grad=True)
     ptr = torch.tensor([0, 5], dtype=torch.int32, device='cuda')
