@@ -14,7 +14,7 @@ void fwd_f32(const Args& a, int axes, int nw, hipStream_t st);
 void fwd_x6(const Args& a, int axes, hipStream_t st);
 void dq_bf16(const Args& a, int axes, int nw, int nblk, hipStream_t st);
 void dq_f32(const Args& a, int axes, int nw, int nblk, hipStream_t st);
-void dq_x6(const Args& a, int axes, int nblk, hipStream_t st);
+void dq_x6(const Args& a, hipStream_t st);
 void dkv_bf16(const Args& a, int axes, int nw, hipStream_t st);
 void dkv_f32(const Args& a, int axes, int nw, hipStream_t st);
 void dkv_x6(const Args& a, int axes, hipStream_t st);
@@ -578,26 +578,33 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
   const int TQ = 32 / a.G * nwq;
   const bool six = f && takes_x6(a, x6);
   pick_bufs(a, f);
-  at::Tensor pq, pk;
+  at::Tensor pq, pk, wsq;
+  Args d = a;                         // of the dq kernel
   const at::Tensor ws = make_copies(a, six, q, k, v, dout);
-  if (split_axis(a, a.Nq / TQ, a.Nk, 32, nwq, 2))
-    pq = part_workspace(a, (int64_t)a.Nq * a.H, 1, false,
-                        (a.Nq + TQ - 1) / TQ, q);
+  // A table's gradient sums dz over all rows, whose rounding has to average
+  // out: x6 scores leave 4e-6 of it (1079 x 726 rows, 3 buckets), exact
+  // products 6e-7, so the kernel that sums it takes those.
+  const bool sixq = six && !axes;
+  if (six && axes) wsq = make_copies(d, false, q, k, v, dout);
+  else d = a;
+  if (split_axis(d, d.Nq / TQ, d.Nk, 32, nwq, 2))
+    pq = part_workspace(d, (int64_t)d.Nq * d.H, 1, false,
+                        (d.Nq + TQ - 1) / TQ, q);
   // Workgroups of the dq kernel with a table: each keeps its LDS columns
   // over all of its tiles.  2048 waves: ragged case 149 us (1024 222, 4096
   // 168), one graph of 4096 nodes 222 (331, 248).
   int nblk = 0;
   at::Tensor part;
   if (axes) {
-    const int items = (a.Nq + TQ - 1) / TQ * a.splits;
-    nblk = std::max(1, std::min(items, 2048 / (a.KV * nwq)));
-    part = at::empty({nblk, a.KV, a.G, a.slots}, f32);
-    a.part_bias = part.data_ptr<float>();
+    const int items = (d.Nq + TQ - 1) / TQ * d.splits;
+    nblk = std::max(1, std::min(items, 2048 / (d.KV * nwq)));
+    part = at::empty({nblk, d.KV, d.G, d.slots}, f32);
+    d.part_bias = part.data_ptr<float>();
   }
-  six ? dq_x6(a, axes, nblk, stream())
-  : f ? dq_f32(a, axes, nwq, nblk, stream())
-      : dq_bf16(a, axes, nwq, nblk, stream());
-  if (a.splits > 1) join<DQ>(a, f, TQ);
+  sixq ? dq_x6(d, stream())
+  : f  ? dq_f32(d, axes, nwq, nblk, stream())
+       : dq_bf16(d, axes, nwq, nblk, stream());
+  if (d.splits > 1) join<DQ>(d, f, TQ);
   if (a.Nk > 0) {
     if (split_axis(a, a.Nk / (32 * nwk), a.Nq, 32 / a.G, nwk, 2))
       pk = part_workspace(a, (int64_t)a.Nk * a.KV, 2, false,
@@ -609,7 +616,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
   }
   if (axes) {
     bias_sum_kernel<<<a.H, kSlots * kSumWays, 0, stream()>>>(
-        a.part_bias, dbias.data_ptr<float>(), nblk, a.KV, a.G, a.slots, a.nb,
+        d.part_bias, dbias.data_ptr<float>(), nblk, a.KV, a.G, a.slots, a.nb,
         a.half, axes);
     DGMC_CHECK_LAUNCH();
   }

@@ -589,9 +589,11 @@ void launch_dq(const Args& a, int axes, int nblk, hipStream_t st) {
                     (axes ? a.G * kTab * 4 +
                                 (size_t)NW * a.slots * hist_cols(NW) * 4
                           : 0);
-  auto kern = axes == 0   ? dq_kernel<P, DP, NW, 0>
-              : axes == 1 ? dq_kernel<P, DP, NW, 1>
-                          : dq_kernel<P, DP, NW, 2>;
+  auto kern = dq_kernel<P, DP, NW, 0>;
+  if constexpr (P::kPlanes == 1) {     // (x6: without a table only)
+    if (axes == 1) kern = dq_kernel<P, DP, NW, 1>;
+    if (axes == 2) kern = dq_kernel<P, DP, NW, 2>;
+  }
   allow_lds(reinterpret_cast<const void*>(kern), sm);
   kern<<<dim3((axes ? nblk : ntiles * a.splits) * a.KV), dim3(NW * 64), sm,
          st>>>(a, ntiles);

@@ -46,6 +46,11 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
   constexpr int NT = NW * 64;
   constexpr int TB = P::kPlanes * KT * CH * 16;  // bytes of one tile
   constexpr int UB = 32 * CH * 16;               // bytes of 32 rows
+  // Long fp32 rows with a table: 32 keys are summed from 0 and then added.
+  // The output's error is the backward's delta's, which misses the sum of a
+  // row's p dp by as much, and the table's gradient adds up what all rows
+  // miss (1079 x 726 rows, 3 buckets: 2e-6 of it, so 6e-7).
+  constexpr bool kBlocked = sizeof(T) == 4 && NW > 1 && POS > 0;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   DGMC_LDS char* lds = (DGMC_LDS char*)smem;
   const int NB = stage_bufs<P, NW>(a);
@@ -231,7 +236,18 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
         for (int r = 0; r < 16; ++r)
           z[u][r] = exp2_(fmaf(z[u][r], ex, -ms));
         l = P::template sum<FINE>(z[u], l);
-        P::template accum<DP, KT, FINE>(acc, lds + TB + u * UB, cols, z[u]);
+        if constexpr (kBlocked) {
+          f32x16 blk[DP / 32];
+#pragma unroll
+          for (int k = 0; k < DP / 32; ++k) blk[k] = f32x16{};
+          P::template accum<DP, KT, FINE>(blk, lds + TB + u * UB, cols, z[u]);
+#pragma unroll
+          for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[k][r] += blk[k][r];
+        } else {
+          P::template accum<DP, KT, FINE>(acc, lds + TB + u * UB, cols, z[u]);
+        }
       }
     }
     l = sum_half(l);
