@@ -13,8 +13,8 @@ never formed, the work list is derived from ``ptr`` on the device (no host
 copy; a captured graph may change ``ptr`` and the rows between replays) and
 every sum has a fixed order.  fp32 calls on long segments run as "x6" (three
 bf16 terms an operand, six products, fp32 sums: ``DGMC_AMD_X6``, as in
-:mod:`.gemm`), short ones on exact fp32 products.  CPU tensors use the oracle
-in :mod:`.reference`.
+:mod:`.gemm`), short ones - and the kernel that sums a table's gradient - on
+exact fp32 products.  CPU tensors use the oracle in :mod:`.reference`.
 """
 import torch
 
