@@ -194,9 +194,14 @@ struct Rows {
   __device__ __forceinline__ bool skip(int x, int n) const {
     return x >= l_hi || x + n <= f_lo;
   }
-  // Every row of the wave takes all of them.
-  __device__ __forceinline__ bool whole(int x, int n) const {
-    return x >= l_lo && x + n <= f_hi;
+  // Every row of the wave takes all of them, and all are staged: a pass ends
+  // at `end`, inside a tile where a segment of its own starts inside one.
+  __device__ __forceinline__ bool whole(int x, int n, int end) const {
+    return x >= l_lo && x + n <= min(f_hi, end);
+  }
+  // Other rows of the lane's own that are staged: [r_lo, min(r_hi, end)).
+  __device__ __forceinline__ unsigned count(int end) const {
+    return max(min(r_hi, end) - r_lo, 0);
   }
   // Pass `pass` of a tile cut to [s_lo, s_hi): all of it (pass < b0) or the
   // segment's own part.

@@ -255,8 +255,8 @@ dq_kernel(const Args a, int ntiles) {
           z = row_dot<P, CH, KT>(lds, rows, qf);
           dp = row_dot<P, CH, KT>(lds + TB, rows, gf);
         }
-        const bool whole = w.whole(k0, KT);
-        const unsigned n = w.r_hi - w.r_lo;
+        const bool whole = w.whole(k0, KT, p_hi);
+        const unsigned n = w.count(p_hi);
         const int j0 = k0 + 4 * h - w.r_lo;
         int one = 0;
         bool same = false;
@@ -500,8 +500,8 @@ dkv_kernel(const Args a) {
         z = row_dot<P, CH, QT>(lds, rows, kf);
         dp = row_dot<P, CH, QT>(lds + TB, rows, vf);
       }
-      const bool whole = w.whole(q0, QW);
-      const unsigned n = (w.r_hi - w.r_lo) * a.G;
+      const bool whole = w.whole(q0, QW, p_hi);
+      const unsigned n = w.count(p_hi) * a.G;
       const int j0 = (q0 - w.r_lo) * a.G + 4 * h;
       int one = 0;
       bool same = false;

@@ -203,8 +203,8 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
           }
         }
       }
-      if (!w.whole(k0, KT)) {
-        const unsigned n = w.r_hi - w.r_lo;
+      if (!w.whole(k0, KT, p_hi)) {
+        const unsigned n = w.count(p_hi);
         const int j0 = k0 + 4 * h - w.r_lo;
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u)
