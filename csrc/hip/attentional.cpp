@@ -54,11 +54,11 @@ struct SegmentAttention
                         const Tensor& ptr_k, const OptTensor& pos_q,
                         const OptTensor& pos_k, double scale, double cap,
                         int64_t half, int64_t mbits, double dmax, bool x6) {
-    auto [out, lo, lse] =
+    auto [out, lo, stat] =
         segattn::forward(q, k, v, ptr_q, ptr_k, scale, cap, bias, pos_q,
                          pos_k, {half, mbits, dmax}, x6, true);
     ctx->save_for_backward({q, k, v, def(bias), ptr_q, ptr_k, def(pos_q),
-                            def(pos_k), out, lo, lse});
+                            def(pos_k), out, lo, stat});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["cap"] = cap;
     ctx->saved_data["half"] = half;

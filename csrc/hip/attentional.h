@@ -21,8 +21,8 @@ struct BucketLayout {
 namespace segattn {
 
 // `x6`: long fp32 segments on the bf16 matrix cores, three terms an operand.
-// (out, lo, lse): lo (bf16 rest of out's rounding, bf16 only) and lse are
-// empty unless `train`.
+// (out, lo, stat): lo (bf16 rest of out's rounding, bf16 only) and stat (fp32
+// [Nq, H, 2], the softmax's maximum and 1 / sum) are empty unless `train`.
 std::tuple<at::Tensor, at::Tensor, at::Tensor> forward(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& ptr_q, const at::Tensor& ptr_k, double scale,
@@ -33,7 +33,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> forward(
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
     const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k,
     const at::Tensor& v, const at::Tensor& out, const at::Tensor& lo,
-    const at::Tensor& lse, const at::Tensor& ptr_q, const at::Tensor& ptr_k,
+    const at::Tensor& stat, const at::Tensor& ptr_q, const at::Tensor& ptr_k,
     double scale, double cap, const OptTensor& bias, const OptTensor& pos_q,
     const OptTensor& pos_k, const BucketLayout& layout, bool x6);
 

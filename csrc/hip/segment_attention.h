@@ -73,7 +73,10 @@ constexpr float kLowest = -1e38f;
 struct Args {
   const void *q, *k, *v, *o, *dout;
   void *out, *out_lo, *dq, *dk, *dv;  // out_lo: bf16 rest of out (training)
-  float *lse, *delta;                 // [Nq, H]
+  // Softmax statistics [Nq, H]: (maximum, 1 / sum) of 2^(z log2(e) - maximum).
+  // Apart: in one log-sum-exp a maximum of -1e9 would swallow the sum's log.
+  float2* stat;
+  float* delta;                       // [Nq, H]
   // Splits: [S][Nq, H, D] (dk, dv: [2][S][Nk, KV, D]), [S][Nq, H, 2] and
   // the number of every [tile, KV]'s.
   float *part_o, *part_ml;
@@ -292,6 +295,11 @@ __device__ __forceinline__ float sum_half(float v) {
 }
 __device__ __forceinline__ float exp2_(float x) {
   return __builtin_amdgcn_exp2f(x);
+}
+
+// A row's statistics; without a key of finite score p is 0 everywhere.
+__device__ __forceinline__ float2 row_stat(float m, float l) {
+  return l == 0.f ? make_float2(INFINITY, 0.f) : make_float2(m, 1.f / l);
 }
 
 // One 16-byte chunk of a row of D elements (zeros outside).

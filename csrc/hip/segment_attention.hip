@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int per_tile,
       __syncthreads();
     }
     if (!live || way != 0) continue;
-    const float f = MODE == FWD ? (L == 0.f ? 0.f : 1.f / L)
+    const float f = MODE == FWD ? row_stat(M, L).y
                     : MODE == DKV && blockIdx.y == 1 ? 1.f
                                                      : a.scale;
     T* out = (T*)(MODE == FWD  ? a.out
@@ -218,8 +218,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int per_tile,
       put4(lo_row, d0, a.D, v_lo);
       put4(lo_row, d0 + 4, a.D, v_lo + 4);
     }
-    if (MODE == FWD && a.lse && d0 == 0)
-      a.lse[row] = L == 0.f ? INFINITY : M + log2f(L);
+    if (MODE == FWD && a.stat && d0 == 0) a.stat[row] = row_stat(M, L);
   }
 }
 
@@ -499,14 +498,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> forward(
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   const auto f32 = q.options().dtype(at::kFloat);
   at::Tensor out = at::empty({a.Nq, a.H, a.D}, q.options());
-  at::Tensor lse = at::empty({train ? a.Nq : 0, a.H}, f32);
+  at::Tensor stat = at::empty({train ? a.Nq : 0, a.H, 2}, f32);
   // bf16 training keeps the rest of the output's rounding for delta.
   const bool f = q.scalar_type() == at::kFloat, fine = train && !f;
   at::Tensor lo = at::empty({fine ? a.Nq : 0, a.H, a.D}, q.options());
-  if (a.Nq == 0) return {out, lo, lse};
+  if (a.Nq == 0) return {out, lo, stat};
   a.out = out.data_ptr();
   a.out_lo = fine ? lo.data_ptr() : nullptr;
-  a.lse = train ? lse.data_ptr<float>() : nullptr;
+  a.stat = train ? (float2*)stat.data_ptr<float>() : nullptr;
   const int nw = waves_for((int64_t)a.Nq * a.G, a.B);
   const bool six = f && takes_x6(a, x6);
   pick_bufs(a, f);
@@ -523,13 +522,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> forward(
   : fine ? fwd_bf16_fine(a, axes, nw, stream())
          : fwd_bf16(a, axes, nw, stream());
   if (a.splits > 1) join<FWD>(a, f, TQ);
-  return {out, lo, lse};
+  return {out, lo, stat};
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
     const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k,
     const at::Tensor& v, const at::Tensor& out, const at::Tensor& lo,
-    const at::Tensor& lse, const at::Tensor& ptr_q, const at::Tensor& ptr_k,
+    const at::Tensor& stat, const at::Tensor& ptr_q, const at::Tensor& ptr_k,
     double scale, double cap, const OptTensor& bias, const OptTensor& pos_q,
     const OptTensor& pos_k, const BucketLayout& layout, bool x6) {
   int axes;
@@ -540,10 +539,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
                   out.scalar_type() == q.scalar_type() &&
                   out.device() == q.device() && out.is_contiguous(),
               "segment_attention: dout and out must have q's shape");
-  TORCH_CHECK(lse.device() == q.device() && lse.is_contiguous() &&
-                  lse.scalar_type() == at::kFloat && lse.dim() == 2 &&
-                  lse.size(0) == a.Nq && lse.size(1) == a.H,
-              "segment_attention: lse must be fp32 [nodes, heads]");
+  TORCH_CHECK(stat.device() == q.device() && stat.is_contiguous() &&
+                  stat.scalar_type() == at::kFloat && stat.dim() == 3 &&
+                  stat.size(0) == a.Nq && stat.size(1) == a.H &&
+                  stat.size(2) == 2,
+              "segment_attention: stat must be fp32 [nodes, heads, 2]");
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   const auto f32 = q.options().dtype(at::kFloat);
   at::Tensor dq = at::empty({a.Nq, a.H, a.D}, q.options());
@@ -567,7 +567,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> backward(
   a.dout = dout.data_ptr();
   a.g_sn = dout.stride(0); a.g_sh = dout.stride(1);
   a.vec_o = rows16(out);
-  a.lse = lse.data_ptr<float>();
+  a.stat = (float2*)stat.data_ptr<float>();
   a.delta = delta.data_ptr<float>();
   a.dq = dq.data_ptr();
   a.dk = dk.data_ptr();

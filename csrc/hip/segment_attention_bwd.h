@@ -1,5 +1,5 @@
 // Backward kernels of the segment attention (segment_attention.h): with
-// p_ij recomputed from the forward's log-sum-exp,
+// p_ij recomputed from the forward's row maximum and sum,
 //
 //   delta_i = <do_i, o_i>,  dz_ij = p_ij (<do_i, v_j> - delta_i)
 //   dT[h, b] = sum of dz_ij over the pairs in bucket b
@@ -191,7 +191,8 @@ dq_kernel(const Args a, int ntiles) {
       }
     }
     dl = sum_half(dl);
-    const float lse = live ? a.lse[row] : INFINITY;
+    // p / st.y, so also dz / st.y, is summed: 1 / sum is a row's own factor.
+    const float2 st = live ? a.stat[row] : make_float2(INFINITY, 0.f);
     if (live && h == 0 && split == 0) a.delta[row] = dl;
     float px = 0.f, py = 0.f;
     if (POS > 0 && live) {
@@ -299,7 +300,7 @@ dq_kernel(const Args a, int ntiles) {
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            v[r] = exp2_(v[r] - lse) * (dp[4 * r4 + r] - dl);
+            v[r] = exp2_(v[r] - st.x) * (dp[4 * r4 + r] - dl);
           if (!whole) {
             // (selected, not multiplied away: a masked key may hold NaN)
 #pragma unroll
@@ -307,15 +308,20 @@ dq_kernel(const Args a, int ntiles) {
               if ((unsigned)(j0 + 8 * r4 + r) >= n) v[r] = t[r] = 0.f;
           }
           if constexpr (POS > 0) {
-            if (same) sum1 += (v[0] + v[1]) + (v[2] + v[3]);
-            else if (pass < w.b0) add_slots<HC>(myhist, sl, v);
+            if (same) {
+              sum1 += (v[0] + v[1]) + (v[2] + v[3]);
+            } else if (pass < w.b0) {
+              const float dz[4] = {v[0] * st.y, v[1] * st.y, v[2] * st.y,
+                                   v[3] * st.y};
+              add_slots<HC>(myhist, sl, dz);
+            }
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             z[4 * r4 + r] = v[r] * fmaf(-t[r], t[r], 1.f);
         }
         if constexpr (POS == 1 && NW > 1) {
-          if (same && pass < w.b0) myhist[one * HC] += sum1;
+          if (same && pass < w.b0) myhist[one * HC] += sum1 * st.y;
         }
         P::template accum<DP, KT, NW == 1>(acc, lds, cols, z);
       }
@@ -324,9 +330,9 @@ dq_kernel(const Args a, int ntiles) {
       if (!redo && live && (pass < w.b0 || w.seg == pass)) {
         if (per < ntile)        // joined by join_kernel
           put_acc<DP>(a.part_o + ((int64_t)split * a.Nq * a.H + row) * a.D,
-                      acc, a.D, 1.f);
+                      acc, a.D, st.y);
         else
-          put_acc<DP>((T*)a.dq + row * a.D, acc, a.D, a.scale);
+          put_acc<DP>((T*)a.dq + row * a.D, acc, a.D, a.scale * st.y);
       }
       if (pass < w.b0 ? !redo : pass == w.b1) break;
     }
@@ -366,8 +372,9 @@ dkv_kernel(const Args a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   DGMC_LDS char* lds = (DGMC_LDS char*)smem;
   const int NB = stage_bufs<P, NW>(a);
-  DGMC_LDS float* rowv = (DGMC_LDS float*)(lds + 2 * NB * TB);  // [NB][4][QT]
-  DGMC_LDS int* toff = (DGMC_LDS int*)(rowv + 4 * NB * QT);     // [QT]
+  // Of every row: maximum, delta, 1 / sum, position.
+  DGMC_LDS float* rowv = (DGMC_LDS float*)(lds + 2 * NB * TB);  // [NB][5][QT]
+  DGMC_LDS int* toff = (DGMC_LDS int*)(rowv + 5 * NB * QT);     // [QT]
   // Wide heads: the lanes' own rows of V and the last KL chunks of K, too
   // many for the registers (a spilled one's load in the loop waits for the
   // next tile's, in order: 14 segments of 30 to 1350 nodes, 297 us; so 204).
@@ -425,7 +432,7 @@ dkv_kernel(const Args a) {
 
   const S* qbase = (const S*)a.q + (int64_t)kvh * a.G * a.q_sh;
   const S* gbase = (const S*)a.dout + (int64_t)kvh * a.G * a.g_sh;
-  float rv[2] = {INFINITY, 0.f};
+  float rv[3] = {INFINITY, 0.f, 0.f};
   int rp[2] = {0, 0};
   auto fetch = [&](int q0, int e, int buf) {
     using St = Stager<P, QT, CH, NT>;
@@ -441,8 +448,11 @@ dkv_kernel(const Args a) {
       const int i = div_group(a, tid), qi = q0 + i;
       const bool there = tid < RW && qi < e;
       const int64_t row = (int64_t)qi * a.H + kvh * a.G + tid - i * a.G;
-      rv[0] = there ? a.lse[row] : INFINITY;   // p = 0 in a row not there
+      // (p = 0 in a row not there)
+      const float2 st = there ? a.stat[row] : make_float2(INFINITY, 0.f);
+      rv[0] = st.x;
       rv[1] = there ? a.delta[row] : 0.f;
+      rv[2] = st.y;
       if (POS > 0) {
         // (rows not there: the first one's)
         const int64_t i = there ? qi : q0;
@@ -458,8 +468,8 @@ dkv_kernel(const Args a) {
   auto put_rows = [&](int buf) {
     if (tid < QT) {
 #pragma unroll
-      for (int k = 0; k < 2 + POS; ++k)
-        rowv[(buf * 4 + k) * QT + tid] = k < 2 ? rv[k] : to_pos(rp[k - 2]);
+      for (int k = 0; k < 3 + POS; ++k)
+        rowv[(buf * 5 + k) * QT + tid] = k < 3 ? rv[k] : to_pos(rp[k - 3]);
     }
   };
   const bool capped = a.cap > 0.f;
@@ -485,7 +495,7 @@ dkv_kernel(const Args a) {
       stage_barrier();
       if (NB == 2 && q0 + QW < p_hi) fetch(q0 + QW, p_hi, buf ^ 1);
       if (w.skip(q0, QW)) continue;
-      const DGMC_LDS float* rw = rowv + buf * 4 * QT;
+      const DGMC_LDS float* rw = rowv + buf * 5 * QT;
       const int rows = lane_base<CH>(rows0 + buf * 2 * TB);
       const int cols = lane_base<CH>(cols0 + buf * 2 * TB);
       f32x16 z, dp;
@@ -506,12 +516,13 @@ dkv_kernel(const Args a) {
       int one = 0;
       bool same = false;
       if constexpr (POS == 1 && NW > 1)
-        same = one_bucket<false>(bk, rw + 2 * QT, px, live, one);
+        same = one_bucket<false>(bk, rw + 3 * QT, px, live, one);
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
         const int o = 8 * r4 + 4 * h;
-        const f32x4 ls = *(const DGMC_LDS f32x4*)(rw + o);
+        const f32x4 mx = *(const DGMC_LDS f32x4*)(rw + o);
         const f32x4 de = *(const DGMC_LDS f32x4*)(rw + QT + o);
+        const f32x4 inv = *(const DGMC_LDS f32x4*)(rw + 2 * QT + o);
         float p[4], t[4] = {0.f, 0.f, 0.f, 0.f}, ds[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) p[r] = z[4 * r4 + r] * s1;
@@ -529,9 +540,9 @@ dkv_kernel(const Args a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) p[r] += tab[one + to[r]];
           } else {
-            const f32x4 qx = *(const DGMC_LDS f32x4*)(rw + 2 * QT + o);
+            const f32x4 qx = *(const DGMC_LDS f32x4*)(rw + 3 * QT + o);
             f32x4 qy = qx;
-            if (POS == 2) qy = *(const DGMC_LDS f32x4*)(rw + 3 * QT + o);
+            if (POS == 2) qy = *(const DGMC_LDS f32x4*)(rw + 4 * QT + o);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               int s = bk.slot(px - qx[r]);
@@ -542,7 +553,7 @@ dkv_kernel(const Args a) {
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          p[r] = exp2_(p[r] - ls[r]);
+          p[r] = exp2_(p[r] - mx[r]) * inv[r];
           ds[r] = p[r] * (dp[4 * r4 + r] - de[r]);
         }
         if (!whole) {
@@ -604,7 +615,7 @@ template <typename P, int DP, int NW>
 void launch_dkv(const Args& a, int axes, hipStream_t st) {
   constexpr int B = P::kPlanes * (int)sizeof(typename P::S);
   const int NB = NW == 1 ? a.bufs : 2;
-  const size_t sm = NB * (2 * 32 * DP * B + 4 * 32 * 4) + 32 * 4 +
+  const size_t sm = NB * (2 * 32 * DP * B + 5 * 32 * 4) + 32 * 4 +
                     (tight<P>(DP) ? (8 + 2) * NW * 64 * 16 : 0) +
                     (axes ? a.G * kTab * 4 : 0);
   auto kern = axes == 0   ? dkv_kernel<P, DP, NW, 0>

@@ -264,8 +264,8 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
         put_acc<DP>(a.part_o + prow * a.D, acc, a.D, 1.f);
       } else {
         // l is 0 only without a key of finite score: such a row is 0.
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (h == 0 && a.lse) a.lse[row] = l == 0.f ? INFINITY : m + log2f(l);
+        const float inv = row_stat(m, l).y;
+        if (h == 0 && a.stat) a.stat[row] = row_stat(m, l);
         T* orow = (T*)a.out + row * a.D;
 #pragma unroll
         for (int k = 0; k < DP / 32; ++k)

@@ -6,7 +6,7 @@ Inputs, the plain form in 64 bits and its element-wise bounds are those of
 import pytest
 import torch
 
-from test_segment_attention import _case, _close, _plain, _run
+from test_segment_attention import F, _case, _close, _plain, _run
 
 
 # --------------------------------------------------------------------------
@@ -60,3 +60,64 @@ def test_sick_graph_beside_low_scores(dtype):
     st['q'] = (st['q'].float() - 5).to(dtype)
     st['k'] = (st['k'].float() + 5).to(dtype)
     _sick(st, 'v', slice(2999, 3001))
+
+
+# --------------------------------------------------------------------------
+# Scores that swallow the log of their own sum
+# --------------------------------------------------------------------------
+MASKS = [torch.finfo(torch.float32).min, -1e9]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('low', MASKS)
+@pytest.mark.parametrize('lq,lk,D,axes', [
+    ([6, 40], [6, 40], 32, 1), ([6, 40], [6, 40], 32, 2),
+    ([300], [400], 64, 1), ([300], [400], 128, 1),
+    ([2, 1], [1300, 700], 64, 1)])
+def test_gradients_of_rows_masked_by_a_lowest_value(dtype, low, lq, lk, D,
+                                                    axes):
+    """Every key masked by a finite value: the row is uniform, and so are its
+    gradients.  With q = 0 the scores are the table's alone, so the plain
+    form with a table of zeros has the same weights 1 / n and its bounds do
+    not grow with the mask."""
+    st = _case(lq, lk, 2, 1, D, dtype, axes=axes, half=2)
+    st['q'].zero_()
+    st['bias'].zero_()
+    val, tol = _plain(st, half=2)
+    st['bias'].fill_(low)
+    got = _run(st, 'cuda')
+    _close(got, val, tol, 'q = 0')
+    # |q k| < 64: swallowed by a score of -1e9 (a unit of 64 there)
+    st['q'] = _case(lq, lk, 2, 1, D, dtype, axes=axes, half=2)['q']
+    st['q'] = (st['q'].float() * 0.5).to(dtype)
+    z = torch.einsum('ihd,jd->ihj', st['q'].float(), st['k'][:, 0].float())
+    assert z.abs().max() * D ** -0.5 * 1.45 < 32
+    more = _run(st, 'cuda')
+    for n in ('out', 'dq', 'dv', 'dbias'):
+        assert torch.equal(more[n], got[n]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('lq,lk', [([5, 9], [7, 30]), ([200], [300]),
+                                   ([2], [1500])])
+def test_weights_of_large_equal_scores_sum_to_one(dtype, lq, lk):
+    """All keys alike and scores of 2^23, where a unit of fp32 is one: p is 1
+    / n, dv the mean of do's columns, to the roundings of 1 / n, the product
+    (fp32 steps, bf16 weights) and the output."""
+    st = _case(lq, lk, 1, 1, 64, dtype)
+    st['q'].fill_(1024.0)
+    st['k'].fill_(1024.0)
+    got = _run(st, 'cuda')
+    u = torch.finfo(dtype).eps / 2
+    up = u if dtype == torch.bfloat16 else 0.0
+    for b in range(len(lq)):
+        sq = slice(*st['ptr_q'][b:b + 2].tolist())
+        sk = slice(*st['ptr_k'][b:b + 2].tolist())
+        n, m = sk.stop - sk.start, sq.stop - sq.start
+        g = st['do'][sq].double()
+        want = (g.sum(0, keepdim=True) / n).expand(n, 1, 64)
+        tol = (up + (n + m + 16) * F) * g.abs().sum(0, keepdim=True) / n + \
+            u * want.abs()
+        assert ((got['dv'][sk].double() - want).abs() <= tol).all()
