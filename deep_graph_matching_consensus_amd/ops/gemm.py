@@ -21,6 +21,7 @@ import os
 import torch
 
 from . import _backend
+from . import reference as ref
 from ..runtime import loopgrad
 from ..runtime.cache import cached
 
@@ -194,7 +195,8 @@ def _dense_tn_ok(a, b):
 
 
 def matmul_tn_fp32(a, b, out=None, accumulate=False):
-    """``a^T @ b`` (``a [K, M]``, ``b [K, N]``) with fp32 output, split-K.
+    """``a^T @ b`` (``a [K, M]``, ``b [K, N]``) with fp32 output (fp64 for
+    the oracle's fp64 inputs), split-K.
 
     With ``out`` (fp32 ``[M, N]``) the product is written (or added, when
     ``accumulate``) there; on the GPU the split-K combine does the
@@ -219,7 +221,8 @@ def matmul_tn_fp32(a, b, out=None, accumulate=False):
         # the deterministic fold writes / adds ``out`` directly).
         return tn_f32([a], [b], out=out, accumulate=accumulate)
     elif not a.is_cuda:
-        res = a.float().t() @ b.float()
+        acc = ref.sum_dtype(a.dtype)
+        res = a.to(acc).t() @ b.to(acc)
     else:
         # (low-precision inputs accumulate into fp32; fp32 / fp64 - the
         # reference-mode oracle - stay in their own dtype)
@@ -365,7 +368,7 @@ def loop_col_sum(loop, name, idx, src):
                                      src.size(1)), torch.float32, src.device)
         _backend.ops().col_sum(src.contiguous(), None, False, slot)
     else:
-        loop.add_to(name, src.float().sum(0))
+        loop.add_to(name, src.to(ref.sum_dtype(src.dtype)).sum(0))
 
 
 def loop_col_total(loop, name):
@@ -377,10 +380,11 @@ def loop_col_total(loop, name):
 
 
 def _col_sum(src, out=None, accumulate=False):
-    """Column sum of a 2-D tensor in fp32 (optionally into ``out``)."""
+    """Column sum of a 2-D tensor in fp32 - the oracle's fp64 in fp64 -
+    (optionally into ``out``)."""
     if _backend.use_hip(src):
         return _backend.ops().col_sum(src.contiguous(), out, accumulate)
-    res = src.float().sum(0)
+    res = src.to(ref.sum_dtype(src.dtype)).sum(0)
     if out is None:
         return res
     if accumulate:

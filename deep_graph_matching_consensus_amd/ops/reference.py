@@ -11,12 +11,18 @@ import torch
 # --------------------------------------------------------------------------
 # Message passing
 # --------------------------------------------------------------------------
+def sum_dtype(dtype):
+    """The type in which values of ``dtype`` are summed: fp64 ones in fp64
+    (a fp64 model's oracle keeps all its bits), all others in fp32."""
+    return dtype if dtype == torch.float64 else torch.float32
+
+
 def spmm(row, col, val, num_rows, x, self_x=None, self_scale=None,
          bias=None, relu=False, out_dtype=torch.float32):
     # 64-bit inputs (a 64-bit oracle) sum in 64 bits: index_add_ adds in any
     # order on the GPU, and in 32 bits that order decides the sign of a value
     # of 1e-7 - a ReLU, and with it a gradient, differently from run to run.
-    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+    acc = sum_dtype(x.dtype)
     xf = x.to(acc)
     out = torch.zeros(num_rows, x.size(1), dtype=acc, device=x.device)
     if col.numel() > 0:

@@ -204,6 +204,12 @@ def spmm_out(op, x, out, self_x=None, self_scale=None, bias=None,
     return out
 
 
+def _out_dtype(dtype):
+    """An operator's default output type: that of half and fp64 inputs."""
+    return dtype if dtype in (torch.bfloat16, torch.float16) else \
+        ref.sum_dtype(dtype)
+
+
 def _spmm_raw(op, x, self_x, self_scale, bias, relu, out_dtype):
     if _backend.use_hip(x) and op.balanced:
         x = x.contiguous()
@@ -244,7 +250,7 @@ class _SpMM(torch.autograd.Function):
             if need_bias:
                 gbias = db.to(ctx.bias_dtype)
         else:
-            g = grad.float()
+            g = grad.to(ref.sum_dtype(grad.dtype))
             if ctx.relu:
                 g = g * (out > 0)
             if need_bias:
@@ -254,11 +260,12 @@ class _SpMM(torch.autograd.Function):
             gx = _spmm_raw(ctx.op.t(), g, None, None, None, False,
                            ctx.x_dtype)
         if self_x is not None:
-            gf = g.float()
+            acc = ref.sum_dtype(g.dtype)
+            gf = g.to(acc)
             if ctx.needs_input_grad[1]:
-                gself = (gf * self_scale.float()).to(self_x.dtype)
+                gself = (gf * self_scale.to(acc)).to(self_x.dtype)
             if ctx.needs_input_grad[2]:
-                gscale = (gf * self_x.float()).sum().view_as(self_scale)
+                gscale = (gf * self_x.to(acc)).sum().view_as(self_scale)
                 gscale = gscale.to(self_scale.dtype)
         return gx, gself, gscale, gbias, None, None, None
 
@@ -270,15 +277,14 @@ def spmm(op, x, self_x=None, self_scale=None, bias=None, relu=False,
     ``x`` may be fp32 or bf16 (e.g. the output of a bf16 GEMM).  The result
     keeps bf16/fp16 inputs in their dtype (so the next GEMM needs no cast and
     the backward moves half the bytes) and is fp32 otherwise; override with
-    ``out_dtype``.  Gradients flow to ``x``, ``self_x``, ``self_scale`` and
-    ``bias``.
+    ``out_dtype``.  (The oracle keeps fp64 inputs in fp64 throughout.)
+    Gradients flow to ``x``, ``self_x``, ``self_scale`` and ``bias``.
     """
     assert x.dim() == 2 and x.size(0) == op.num_cols, (x.shape, op)
     if self_x is not None:
         assert self_x.size(0) == op.num_rows and self_scale is not None
     if out_dtype is None:
-        out_dtype = x.dtype if x.dtype in (torch.bfloat16, torch.float16) \
-            else torch.float32
+        out_dtype = _out_dtype(x.dtype)
     return _SpMM.apply(x, self_x, self_scale, bias, op, relu, out_dtype)
 
 
@@ -319,10 +325,8 @@ class _GemmSpMM(torch.autograd.Function):
                 y = nt_f32([xc], w_lp.t()).view(-1, C)
             else:
                 y = (xc @ w_lp).view(-1, C)
-            out_dtype = y.dtype if y.dtype in (torch.bfloat16,
-                                               torch.float16) \
-                else torch.float32
-            out = _spmm_raw(op, y, None, None, bias, relu, out_dtype)
+            out = _spmm_raw(op, y, None, None, bias, relu,
+                            _out_dtype(y.dtype))
         ctx.save_for_backward(xc, w_lp, out if relu else None)
         ctx.op, ctx.relu, ctx.C, ctx.loop = op, relu, C, loop
         ctx.x_dtype, ctx.w_dtype = x.dtype, w.dtype
@@ -421,7 +425,7 @@ class _GemmSpMM(torch.autograd.Function):
                 grad, out if ctx.relu else grad, ctx.relu, w_lp.dtype, None,
                 False, part)
         else:
-            g = grad.float()
+            g = grad.to(ref.sum_dtype(grad.dtype))
             if ctx.relu:
                 g = g * (out > 0)
             if need_b:

@@ -94,20 +94,21 @@ class LoopGrad(object):
     def stack(self, name):
         return self._stacks[name]
 
-    def acc(self, name, shape, device):
-        """``(buffer, accumulate)``: fp32 accumulator ``name``; ``accumulate``
-        is False for the first contribution (the producer overwrites)."""
+    def acc(self, name, shape, device, dtype=torch.float32):
+        """``(buffer, accumulate)``: fp32 accumulator ``name`` (``dtype`` of
+        an oracle's fp64); ``accumulate`` is False for the first contribution
+        (the producer overwrites)."""
         buf = self._accs.get(name)
         if buf is None:
-            buf = torch.empty(tuple(shape), dtype=torch.float32,
-                              device=device)
+            buf = torch.empty(tuple(shape), dtype=dtype, device=device)
             self._accs[name] = buf
             return buf, False
         return buf, True
 
     def add_to(self, name, value):
         """Accumulate a tensor computed elsewhere (fallback paths)."""
-        buf, accumulate = self.acc(name, value.shape, value.device)
+        buf, accumulate = self.acc(name, value.shape, value.device,
+                                   value.dtype)
         if accumulate:
             buf.add_(value)
         else:
