@@ -768,13 +768,14 @@ __device__ __forceinline__ float tanh_(float x) {
 
 // Bucket slot of offset d (float, exact) on one axis: 0 .. 2 half + 1.
 struct Bucket {
-  float dmax, dmul;
+  float dmin, dmax, dmul;
   int shift, width, K;
+  // (0 - dmax: +0 where there is one bucket, whose offsets so have no sign)
   __device__ __forceinline__ explicit Bucket(const Args& a)
-      : dmax(a.dmax), dmul(a.dmul), shift(23 - a.mbits), width(5 + a.mbits),
+      : dmin(0.f - a.dmax), dmax(a.dmax), dmul(a.dmul), shift(23 - a.mbits), width(5 + a.mbits),
         K(a.half + 1) {}
   __device__ __forceinline__ int slot(float d) const {
-    const float c = __builtin_amdgcn_fmed3f(d, -dmax, dmax);
+    const float c = __builtin_amdgcn_fmed3f(d, dmin, dmax);
     const float x = fmaf(fabsf(c), dmul, 2.f);
     const int t = __builtin_amdgcn_ubfe(__builtin_bit_cast(unsigned, x),
                                         shift, width);

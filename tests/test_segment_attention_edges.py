@@ -121,3 +121,19 @@ def test_weights_of_large_equal_scores_sum_to_one(dtype, lq, lk):
         tol = (up + (n + m + 16) * F) * g.abs().sum(0, keepdim=True) / n + \
             u * want.abs()
         assert ((got['dv'][sk].double() - want).abs() <= tol).all()
+
+
+# --------------------------------------------------------------------------
+# Bucket layouts and caps at their ends
+# --------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('axes', [1, 2])
+@pytest.mark.parametrize('lens', [[5, 20], [300]])
+def test_one_bucket(dtype, axes, lens):
+    """half = 0: one bucket for every offset, whatever its sign."""
+    st = _case(lens, None, 2, 2, 32, dtype, axes=axes, half=0)
+    assert (st['pos_q'] < 0).any() and (st['pos_q'] > 0).any()
+    st['bias'][:] = torch.tensor([[3.0], [-2.0]])
+    val, tol = _plain(st, cap=2.0, half=0)
+    _close(_run(st, 'cuda', cap=2.0), val, tol)
