@@ -746,10 +746,12 @@ __device__ __forceinline__ void put_acc(T* row, const f32x16 (&acc)[DP / 32],
 // Scores
 // --------------------------------------------------------------------------
 // tanh: v_exp / v_rcp (about 1 ulp each) of 1 - 2 / (e^2x + 1), whose
-// cancellation leaves an absolute error of 1e-7 near 0 - below a bf16
-// product's rounding.  fp32 (EXACT) takes the odd series up to |x| < 0.25
-// (to x^9; the next term is 8.5e-9 of x there) so small scores keep their
-// relative precision.
+// cancellation leaves an absolute error of 1e-7 near 0, times the cap in a
+// score.  bf16 takes that up to a cap of 64, where it is the 2^-17 that
+// weights of two terms are rounded to (wider caps are taken in fp32; the
+// series in these kernels cost 3 % of every capped call).  fp32 (EXACT) takes
+// the odd series up to |x| < 0.25 (to x^9; the next term is 8.5e-9 of x
+// there) so small scores keep their relative precision.
 template <bool EXACT>
 __device__ __forceinline__ float tanh_(float x) {
   const float e = exp2_(x * (2.f * kLog2e));

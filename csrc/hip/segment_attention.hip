@@ -269,6 +269,8 @@ __global__ __launch_bounds__(kSlots * kSumWays) void bias_sum_kernel(
   out[(int64_t)head * nb + c] = sum;
 }
 
+constexpr double kMaxCapBf16 = 64.0;      // see tanh_
+
 static void check_heads(const at::Tensor& t, const char* name,
                         const at::Tensor& like) {
   TORCH_CHECK(t.dim() == 3, "segment_attention: ", name,
@@ -315,6 +317,8 @@ static Args make_args(const at::Tensor& q, const at::Tensor& k,
   TORCH_CHECK(q.scalar_type() == at::kFloat ||
                   q.scalar_type() == at::kBFloat16,
               "segment_attention: unsupported dtype ", q.scalar_type());
+  TORCH_CHECK(q.scalar_type() == at::kFloat || cap <= kMaxCapBf16,
+              "segment_attention: caps over ", kMaxCapBf16, " need fp32");
   TORCH_CHECK(k.sizes() == v.sizes(), "segment_attention: k and v differ in "
               "shape");
   TORCH_CHECK(q.size(2) == k.size(2) && q.size(2) >= 1 && q.size(2) <= 128,

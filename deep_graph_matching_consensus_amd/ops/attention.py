@@ -26,6 +26,8 @@ from . import reference as ref
 MAX_DISTANCE = 1 << 22
 MAX_GROUP = 32
 MAX_DIM = 128
+#: Widest cap the bf16 kernels take; their tanh is off by 1e-7 of the cap.
+MAX_CAP_BF16 = 64.0
 
 
 def bucket_starts(half, octave_steps=1):
@@ -148,7 +150,9 @@ def segment_attention(q, k, v, ptr_q, ptr_k=None, scale=None, cap=0.0,
             the device (``ptr`` of a batch's dense layout).  ``ptr_k=None``:
             the queries' own segments.
         scale (float): default ``dim ** -0.5``.
-        cap (float): score cap, 0 for none.
+        cap (float): score cap, 0 for none.  (On the GPU a bf16 call with a
+            cap over 64 runs on fp32 copies of ``q``, ``k`` and ``v``, whose
+            kernels keep small scores' precision under any cap.)
         bias (Tensor): learned table ``[heads, (2 half + 1) ** axes]`` with
             ``half <= 31`` on one axis, ``half <= 3`` on two; accumulated in
             fp32.  Finite entries below -1e38 count as -1e38.
@@ -176,10 +180,13 @@ def segment_attention(q, k, v, ptr_q, ptr_k=None, scale=None, cap=0.0,
         return ref.segment_attention(
             q, k, v, ptr_q, ptr_k, scale, cap, bias, pos_q, pos_k,
             bucket_starts(layout[0], octave_steps))
+    dtype = q.dtype
+    if dtype == torch.bfloat16 and cap > MAX_CAP_BF16:
+        q, k, v = q.float(), k.float(), v.float()
     q, k, v = (t if t.stride(2) == 1 or t.size(2) == 1 else t.contiguous()
                for t in (q, k, v))
     if bias is not None:
         bias = bias.float().contiguous()
     return _backend.ops().segment_attention.default(
         q, k, v, bias, ptr_q.contiguous(), ptr_k.contiguous(), pos_q, pos_k,
-        scale, float(cap), *layout, gemm.NT_X6)
+        scale, float(cap), *layout, gemm.NT_X6).to(dtype)

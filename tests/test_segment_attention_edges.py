@@ -3,6 +3,8 @@
 Inputs, the plain form in 64 bits and its element-wise bounds are those of
 ``test_segment_attention.py``.
 """
+import math
+
 import pytest
 import torch
 
@@ -137,3 +139,21 @@ def test_one_bucket(dtype, axes, lens):
     st['bias'][:] = torch.tensor([[3.0], [-2.0]])
     val, tol = _plain(st, cap=2.0, half=0)
     _close(_run(st, 'cuda', cap=2.0), val, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('cap', [1e3, 1e5, 1e7, 1e9])
+@pytest.mark.parametrize('lens', [[5, 20], [300]])
+def test_wide_caps(dtype, cap, lens):
+    """A cap far above the scores changes nothing: its rounding follows the
+    score, not the cap.  Bounds: those of a cap at four times the largest
+    score, over the least slope 1 - tanh(1 / 4)^2 that form multiplies by."""
+    st = _case(lens, None, 2, 1, 64, dtype, axes=1, half=2)
+    z = torch.einsum('ihd,jd->ihj', st['q'].double(), st['k'][:, 0].double())
+    near = 4 * float(z.abs().max()) / 8
+    assert near < cap
+    val, _ = _plain(st, cap=cap, half=2)
+    _, tol = _plain(st, cap=near, half=2)
+    tol = {n: t / (1 - math.tanh(0.25) ** 2) for n, t in tol.items()}
+    _close(_run(st, 'cuda', cap=cap), val, tol)
