@@ -26,6 +26,9 @@ from . import reference as ref
 MAX_DISTANCE = 1 << 22
 MAX_GROUP = 32
 MAX_DIM = 128
+#: Largest scale and cap, and the smallest cap's reciprocal: fp32 holds what
+#: the kernels form of them.
+MAX_FACTOR = 1e30
 #: Widest cap the bf16 kernels take; their tanh is off by 1e-7 of the cap.
 MAX_CAP_BF16 = 64.0
 
@@ -47,7 +50,7 @@ def bias_width(half, axes=1):
     return (2 * half + 1) ** axes
 
 
-def _check(q, k, v, ptr_q, ptr_k, cap):
+def _check(q, k, v, ptr_q, ptr_k, cap, scale):
     for t, name in ((q, 'q'), (k, 'k'), (v, 'v')):
         if t.dim() != 3:
             raise ValueError('{} must be [nodes, heads, dim], got {}'.format(
@@ -81,8 +84,13 @@ def _check(q, k, v, ptr_q, ptr_k, cap):
     if ptr_q is ptr_k and q.size(0) != k.size(0):
         raise ValueError('ptr_k=None (self-attention) needs as many keys as '
                          'queries')
-    if not 0.0 <= cap < float('inf'):
-        raise ValueError('cap must be finite and >= 0 (0: none)')
+    if cap != 0.0 and not 1.0 / MAX_FACTOR <= cap <= MAX_FACTOR:
+        raise ValueError('cap must be 0 (none) or within {:g} and {:g}'.format(
+            1.0 / MAX_FACTOR, MAX_FACTOR))
+    if scale is not None and not abs(scale) <= MAX_FACTOR * min(
+            cap or 1.0, 1.0):
+        raise ValueError('scale must be at most {:g} in size, of a cap under '
+                         '1 that much of it'.format(MAX_FACTOR))
 
 
 def _check_bias(q, k, bias, pos_q, pos_k, octave_steps):
@@ -168,7 +176,7 @@ def segment_attention(q, k, v, ptr_q, ptr_k=None, scale=None, cap=0.0,
     """
     if ptr_k is None:
         ptr_k = ptr_q
-    _check(q, k, v, ptr_q, ptr_k, cap)
+    _check(q, k, v, ptr_q, ptr_k, cap, scale)
     scale = q.size(2) ** -0.5 if scale is None else float(scale)
     layout = (0, 0, 0.0)
     if bias is not None:

@@ -8,6 +8,7 @@ import math
 import pytest
 import torch
 
+from deep_graph_matching_consensus_amd.ops import segment_attention
 from test_segment_attention import F, _case, _close, _plain, _run
 
 
@@ -157,3 +158,31 @@ def test_wide_caps(dtype, cap, lens):
     _, tol = _plain(st, cap=near, half=2)
     tol = {n: t / (1 - math.tanh(0.25) ** 2) for n, t in tol.items()}
     _close(_run(st, 'cuda', cap=cap), val, tol)
+
+
+@pytest.mark.parametrize('kw', [
+    dict(cap=1e39), dict(cap=1e-40), dict(cap=1e-20, scale=1e20),
+    dict(scale=math.inf), dict(scale=math.nan), dict(scale=1e38),
+    dict(scale=-1e39)])
+def test_scores_past_fp32_are_refused(kw):
+    """A cap or scale that fp32 holds only as 0 or inf makes 0 times inf of
+    an ordinary score."""
+    q = torch.randn(4, 2, 8)
+    p = torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(ValueError):
+        segment_attention(q, q, q, p, **kw)
+
+
+@pytest.mark.parametrize('device', [
+    'cpu', pytest.param('cuda', marks=pytest.mark.gpu)])
+@pytest.mark.parametrize('cap,scale', [
+    (1e30, None), (1e-30, None), (0.0, 1e30), (0.0, -1e30), (0.0, 0.0),
+    (2.0, 0.0), (2.0, -0.3)])
+def test_caps_and_scales_at_their_ends_are_finite(cap, scale, device):
+    q = torch.randn(4, 2, 8, device=device, requires_grad=True)
+    p = torch.tensor([0, 4], dtype=torch.int32, device=device)
+    out = segment_attention(q, q, q, p, cap=cap, scale=scale)
+    g, = torch.autograd.grad(out.square().sum(), q)
+    assert torch.isfinite(out).all()
+    if abs(scale or 0.0) < 1:       # (else scores of 1e30 have such gradients)
+        assert torch.isfinite(g).all()
