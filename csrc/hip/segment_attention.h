@@ -296,6 +296,23 @@ __device__ __forceinline__ float sum_half(float v) {
 __device__ __forceinline__ float exp2_(float x) {
   return __builtin_amdgcn_exp2f(x);
 }
+// A product that is rounded before what is added to it.
+__device__ __forceinline__ float mul_(float x, float y) {
+#pragma clang fp contract(off)
+  return x * y;
+}
+
+// Weights are 2^(z ex - m), one fma: of plain scores (no cap, no table) z is
+// the product alone and ex its scale.  Where a maximum is past kFar, that
+// product's own rounding, which m has and the fma has not, would be an
+// exponent of its own (a score of 2^31: up to 128, the weight inf): such
+// scores are scaled and rounded first.  Forward and backward round alike, so
+// that no weight of a row passes the forward's largest.
+constexpr float kFar = 16777216.f;
+template <int POS>
+__device__ __forceinline__ bool plain_scores(const Args& a, float s1) {
+  return POS == 0 && a.cap <= 0.f && s1 > 0.f;
+}
 
 // A row's statistics; without a key of finite score p is 0 everywhere.
 __device__ __forceinline__ float2 row_stat(float m, float l) {
@@ -662,12 +679,14 @@ struct X6 {
 };
 
 // Row operand: chunks h, h + 2, .. of row c of a staged block of 32 rows.
+// KEYS: the staged rows are the keys (x6 adds its terms in one order of query
+// and key, so that a score has the same bits in every kernel).
 template <int CH>
 __device__ __forceinline__ int row_base() {
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   return c * CH * 16 + ((h ^ swz<CH>(c)) * 16);
 }
-template <typename P, int CH, int ROWS>
+template <typename P, int CH, int ROWS, bool KEYS>
 __device__ __forceinline__ f32x16 row_dot(
     const DGMC_LDS char* tile, int rows,
     const u32x4 (&f)[P::kPlanes][CH / 2]) {
@@ -684,7 +703,8 @@ __device__ __forceinline__ f32x16 row_dot(
     } else {
 #pragma unroll
       for (int t = 0; t < 6; ++t)
-        acc = Bf16::dot(a[x6_a(t)], f[x6_b(t)][s], acc);
+        acc = KEYS ? Bf16::dot(a[x6_a(t)], f[x6_b(t)][s], acc)
+                   : Bf16::dot(a[x6_b(t)], f[x6_a(t)][s], acc);
     }
   }
   return acc;

@@ -125,6 +125,8 @@ dq_kernel(const Args a, int ntiles) {
   const bool capped = a.cap > 0.f;
   const float s1 = capped ? a.scale / a.cap : a.scale * kLog2e;
   const float s2 = a.cap * kLog2e;
+  const bool plain = plain_scores<POS>(a, s1);
+  constexpr bool kOther = sizeof(S) == 4 && NW > 1 && POS > 0;
   const int rows0 = row_base<CH>(), cols0 = P::template cols<CH>();
 
   for (int it = blk; it < ntiles * a.splits; it += nblk) {
@@ -194,6 +196,8 @@ dq_kernel(const Args a, int ntiles) {
     // p / st.y, so also dz / st.y, is summed: 1 / sum is a row's own factor.
     const float2 st = live ? a.stat[row] : make_float2(INFINITY, 0.f);
     if (live && h == 0 && split == 0) a.delta[row] = dl;
+    const bool scaled = !plain || __any(st.x < INFINITY && fabsf(st.x) > kFar);
+    const float ex = scaled ? 1.f : s1;
     float px = 0.f, py = 0.f;
     if (POS > 0 && live) {
       px = load_pos(a.pos_q, qi, POS, 0);
@@ -253,8 +257,8 @@ dq_kernel(const Args a, int ntiles) {
               z, dp, lds, TB, rows, [&](int s) { return qf[0][s]; },
               [&](int s) { return gf[0][s]; });
         } else {
-          z = row_dot<P, CH, KT>(lds, rows, qf);
-          dp = row_dot<P, CH, KT>(lds + TB, rows, gf);
+          z = row_dot<P, CH, KT, true>(lds, rows, qf);
+          dp = row_dot<P, CH, KT, true>(lds + TB, rows, gf);
         }
         const bool whole = w.whole(k0, KT, p_hi);
         const unsigned n = w.count(p_hi);
@@ -271,12 +275,16 @@ dq_kernel(const Args a, int ntiles) {
           float v[4], t[4] = {0.f, 0.f, 0.f, 0.f};
           int sl[4] = {0, 0, 0, 0};
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = z[4 * r4 + r] * s1;
+          for (int r = 0; r < 4; ++r) v[r] = z[4 * r4 + r];
+          if (scaled) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = mul_(v[r], s1);
+          }
           if (capped) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               t[r] = tanh_<sizeof(T) == 4>(v[r]);
-              v[r] = s2 * t[r];
+              v[r] = mul_(s2, t[r]);
             }
           }
           if constexpr (POS > 0) {
@@ -299,8 +307,12 @@ dq_kernel(const Args a, int ntiles) {
             }
           }
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            v[r] = exp2_(v[r] - st.x) * (dp[4 * r4 + r] - dl);
+          for (int r = 0; r < 4; ++r) {
+            float x = fmaf(v[r], ex, -st.x);
+            // (the forward's scores were x6 products, other bits than these)
+            if (kOther) x = x > 9.f ? 9.f : x;
+            v[r] = exp2_(x) * (dp[4 * r4 + r] - dl);
+          }
           if (!whole) {
             // (selected, not multiplied away: a masked key may hold NaN)
 #pragma unroll
@@ -375,12 +387,13 @@ dkv_kernel(const Args a) {
   // Of every row: maximum, delta, 1 / sum, position.
   DGMC_LDS float* rowv = (DGMC_LDS float*)(lds + 2 * NB * TB);  // [NB][5][QT]
   DGMC_LDS int* toff = (DGMC_LDS int*)(rowv + 5 * NB * QT);     // [QT]
+  DGMC_LDS int* far_rows = toff + QT;              // [2, of 4: see kFar]
   // Wide heads: the lanes' own rows of V and the last KL chunks of K, too
   // many for the registers (a spilled one's load in the loop waits for the
   // next tile's, in order: 14 segments of 30 to 1350 nodes, 297 us; so 204).
   constexpr bool VL = tight<P>(DP);
   constexpr int KL = VL ? 2 : 0, OWN = VL ? CH / 2 + KL : 0;
-  DGMC_LDS u32x4* own = (DGMC_LDS u32x4*)(toff + QT);       // [OWN][NT]
+  DGMC_LDS u32x4* own = (DGMC_LDS u32x4*)(far_rows + 4);    // [OWN][NT]
   DGMC_LDS float* tab = (DGMC_LDS float*)(own + OWN * NT);  // [G][kTab]
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -467,6 +480,8 @@ dkv_kernel(const Args a) {
   };
   auto put_rows = [&](int buf) {
     if (tid < QT) {
+      const bool far = __any(rv[0] < INFINITY && fabsf(rv[0]) > kFar);
+      if (tid == 0) far_rows[buf] = far;
 #pragma unroll
       for (int k = 0; k < 3 + POS; ++k)
         rowv[(buf * 5 + k) * QT + tid] = k < 3 ? rv[k] : to_pos(rp[k - 3]);
@@ -475,6 +490,7 @@ dkv_kernel(const Args a) {
   const bool capped = a.cap > 0.f;
   const float s1 = capped ? a.scale / a.cap : a.scale * kLog2e;
   const float s2 = a.cap * kLog2e;
+  const bool plain = plain_scores<POS>(a, s1);
   const int rows0 = row_base<CH>(), cols0 = P::template cols<CH>();
 
   // Passes as in the forward.
@@ -496,6 +512,8 @@ dkv_kernel(const Args a) {
       if (NB == 2 && q0 + QW < p_hi) fetch(q0 + QW, p_hi, buf ^ 1);
       if (w.skip(q0, QW)) continue;
       const DGMC_LDS float* rw = rowv + buf * 5 * QT;
+      const bool scaled = !plain || far_rows[buf] != 0;
+      const float ex = scaled ? 1.f : s1;
       const int rows = lane_base<CH>(rows0 + buf * 2 * TB);
       const int cols = lane_base<CH>(cols0 + buf * 2 * TB);
       f32x16 z, dp;
@@ -507,8 +525,8 @@ dkv_kernel(const Args a) {
             },
             [&](int s) { return own[s * NT + tid]; });
       } else {
-        z = row_dot<P, CH, QT>(lds, rows, kf);
-        dp = row_dot<P, CH, QT>(lds + TB, rows, vf);
+        z = row_dot<P, CH, QT, false>(lds, rows, kf);
+        dp = row_dot<P, CH, QT, false>(lds + TB, rows, vf);
       }
       const bool whole = w.whole(q0, QW, p_hi);
       const unsigned n = w.count(p_hi) * a.G;
@@ -525,12 +543,16 @@ dkv_kernel(const Args a) {
         const f32x4 inv = *(const DGMC_LDS f32x4*)(rw + 2 * QT + o);
         float p[4], t[4] = {0.f, 0.f, 0.f, 0.f}, ds[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[r] = z[4 * r4 + r] * s1;
+        for (int r = 0; r < 4; ++r) p[r] = z[4 * r4 + r];
+        if (scaled) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) p[r] = mul_(p[r], s1);
+        }
         if (capped) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             t[r] = tanh_<sizeof(T) == 4>(p[r]);
-            p[r] = s2 * t[r];
+            p[r] = mul_(s2, t[r]);
           }
         }
         if constexpr (POS > 0) {
@@ -553,7 +575,7 @@ dkv_kernel(const Args a) {
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          p[r] = exp2_(p[r] - mx[r]) * inv[r];
+          p[r] = exp2_(fmaf(p[r], ex, -mx[r])) * inv[r];
           ds[r] = p[r] * (dp[4 * r4 + r] - de[r]);
         }
         if (!whole) {
@@ -615,7 +637,7 @@ template <typename P, int DP, int NW>
 void launch_dkv(const Args& a, int axes, hipStream_t st) {
   constexpr int B = P::kPlanes * (int)sizeof(typename P::S);
   const int NB = NW == 1 ? a.bufs : 2;
-  const size_t sm = NB * (2 * 32 * DP * B + 5 * 32 * 4) + 32 * 4 +
+  const size_t sm = NB * (2 * 32 * DP * B + 5 * 32 * 4) + 36 * 4 +
                     (tight<P>(DP) ? (8 + 2) * NW * 64 * 16 : 0) +
                     (axes ? a.G * kTab * 4 : 0);
   auto kern = axes == 0   ? dkv_kernel<P, DP, NW, 0>

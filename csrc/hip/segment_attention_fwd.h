@@ -129,8 +129,7 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
 
   const float s1 = a.cap > 0.f ? a.scale / a.cap : a.scale * kLog2e;
   const float s2 = a.cap * kLog2e;
-  // Plain scores stay unscaled: 2^(s1 z - m) is one fma and one exp2.
-  const bool plain = POS == 0 && a.cap <= 0.f && s1 > 0.f;
+  const bool plain = plain_scores<POS>(a, s1);
   const float ex = plain ? s1 : 1.f;
   const int rows0 = row_base<CH>(), cols0 = P::template cols<CH>();
 
@@ -159,18 +158,18 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
       f32x16 z[KT / 32];
 #pragma unroll
       for (int u = 0; u < KT / 32; ++u)
-        z[u] = row_dot<P, CH, KT>(lds + u * UB, rows, qf);
+        z[u] = row_dot<P, CH, KT, true>(lds + u * UB, rows, qf);
       if (!plain) {
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) z[u][r] *= s1;
+          for (int r = 0; r < 16; ++r) z[u][r] = mul_(z[u][r], s1);
         if (a.cap > 0.f) {
 #pragma unroll
           for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-              z[u][r] = s2 * tanh_<sizeof(T) == 4>(z[u][r]);
+              z[u][r] = mul_(s2, tanh_<sizeof(T) == 4>(z[u][r]));
         }
       }
       if constexpr (POS > 0) {
@@ -218,7 +217,7 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
       for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mt = fmaxf(mt, z[u][r]);
-      mt = max_half(mt) * ex;
+      mt = mul_(max_half(mt), ex);
       if (__any(mt > m + 8.f)) {
         const float mn = fmaxf(m, mt);
         const float al = mn == m ? 1.f : exp2_(m - mn);
@@ -230,11 +229,19 @@ __global__ __launch_bounds__(NW * 64, fwd_waves<P>(DP)) void fwd_kernel(
         m = mn;
       }
       const float ms = m == -INFINITY ? 0.f : m;
+      float e = ex;
+      if (plain && __any(fabsf(ms) > kFar)) {
+        e = 1.f;
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) z[u][r] = mul_(z[u][r], s1);
+      }
 #pragma unroll
       for (int u = 0; u < KT / 32; ++u) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          z[u][r] = exp2_(fmaf(z[u][r], ex, -ms));
+          z[u][r] = exp2_(fmaf(z[u][r], e, -ms));
         l = P::template sum<FINE>(z[u], l);
         if constexpr (kBlocked) {
           f32x16 blk[DP / 32];

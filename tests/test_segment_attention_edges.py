@@ -186,3 +186,66 @@ def test_caps_and_scales_at_their_ends_are_finite(cap, scale, device):
     assert torch.isfinite(out).all()
     if abs(scale or 0.0) < 1:       # (else scores of 1e30 have such gradients)
         assert torch.isfinite(g).all()
+
+
+# --------------------------------------------------------------------------
+# Scores past fp32's integers
+# --------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('lq,lk,D', [([5, 9], [7, 30], 64), ([200], [300], 64),
+                                     ([200], [300], 128), ([2], [1500], 64)])
+@pytest.mark.parametrize('axes,scale', [(0, None), (0, -0.125), (1, None)])
+def test_scores_of_2_to_the_31(dtype, lq, lk, D, axes, scale):
+    """Multiples of 2^31 / sqrt(D) that every type here holds: a row's largest
+    scores share its weight, whatever rounds their product with log2(e).
+
+    Bounds: weights 1 / n are exact to the sum's and the division's steps
+    (and the type's, where they enter a product in it); <do, v>, <do, o> and
+    the sums over rows as in the plain form."""
+    st = _case(lq, lk, 2, 1, D, dtype, axes=axes, half=1)
+    g = torch.Generator().manual_seed(9)
+    st['q'] = (torch.randint(-3, 4, st['q'].shape, generator=g) *
+               2.0 ** 17).to(dtype)
+    st['k'] = (torch.randint(-3, 4, st['k'].shape, generator=g) *
+               2.0 ** 14).to(dtype)
+    if axes:
+        st['bias'].zero_()
+    got = _run(st, 'cuda', scale=scale)
+    s = D ** -0.5 if scale is None else scale
+    u = torch.finfo(dtype).eps / 2
+    up = u if dtype == torch.bfloat16 else 0.0
+    for b in range(len(lq)):
+        sq = slice(*st['ptr_q'][b:b + 2].tolist())
+        sk = slice(*st['ptr_k'][b:b + 2].tolist())
+        K, V = st['k'][sk, 0].double(), st['v'][sk, 0].double()
+        n, m = K.size(0), sq.stop - sq.start
+        dk, dv = torch.zeros_like(K), torch.zeros_like(V)
+        edk, edv = torch.zeros_like(K), torch.zeros_like(V)
+        for h in range(2):
+            Q, G = st['q'][sq, h].double(), st['do'][sq, h].double()
+            z = s * Q @ K.t()
+            assert z.abs().max() > 2.0 ** 31 / D ** 0.5
+            p = torch.softmax(z, dim=-1)
+            rp = up + (n + 16) * F
+            o, pv = p @ V, p @ V.abs()
+            eo = rp * pv + u * o.abs()
+            assert ((got['out'][sq, h].double() - o).abs() <= eo).all()
+            dp = G @ V.t()
+            delta = (G * o).sum(1, keepdim=True)
+            edp = (D + 2) * F * G.abs() @ V.abs().t() + \
+                (G.abs() * eo).sum(1, keepdim=True) + \
+                D * F * (G * o).abs().sum(1, keepdim=True)
+            ds = s * p * (dp - delta)
+            eds = abs(s) * p * (rp * (dp - delta).abs() + edp) + \
+                (up + 4 * F) * ds.abs()
+            dq = ds @ K
+            edq = eds @ K.abs() + n * F * ds.abs() @ K.abs() + u * dq.abs()
+            assert ((got['dq'][sq, h].double() - dq).abs() <= edq).all()
+            dk += ds.t() @ Q
+            edk += (eds.t() + 2 * m * F * ds.t().abs()) @ Q.abs()
+            dv += p.t() @ G
+            edv += ((rp + 2 * m * F) * p).t() @ G.abs()
+        for t, e, x in ((dk, edk, 'dk'), (dv, edv, 'dv')):
+            err = (got[x][sk, 0].double() - t).abs()
+            assert (err <= e + u * t.abs()).all(), x
