@@ -21,8 +21,15 @@ using torch::autograd::variable_list;
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants(const OptTensor& t) { return t.has_value() && wants(*t); }
 
+bool dual(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool dual(const OptTensor& t) { return t.has_value() && dual(*t); }
+
+// (A tangent is refused: these nodes, and the calls that need none, know no
+// forward mode and would drop it.)
 template <typename... A>
-bool wants_grad(const A&... a) {
+bool wants_grad(const char* name, const A&... a) {
+  TORCH_CHECK(!(dual(a) || ...), name,
+              ": forward-mode differentiation is not supported");
   return at::GradMode::is_enabled() && (wants(a) || ...);
 }
 
@@ -102,7 +109,7 @@ Tensor segment_attention_autograd(const Tensor& q, const Tensor& k,
                                   const OptTensor& pos_k, double scale,
                                   double cap, int64_t half, int64_t mbits,
                                   double dmax, bool x6) {
-  if (wants_grad(q, k, v, bias))
+  if (wants_grad("segment_attention", q, k, v, bias))
     return SegmentAttention::apply(q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k,
                                    scale, cap, half, mbits, dmax, x6);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -154,7 +161,7 @@ std::vector<Tensor> layer_norm_autograd(const Tensor& x,
                                         const OptTensor& residual,
                                         const OptTensor& weight,
                                         const OptTensor& bias, double eps) {
-  if (wants_grad(x, residual, weight, bias))
+  if (wants_grad("layer_norm", x, residual, weight, bias))
     return LayerNorm::apply(x, residual, weight, bias, eps);
   at::AutoDispatchBelowADInplaceOrView below;
   return layer_norm(x, residual, weight, bias, eps);
@@ -195,7 +202,7 @@ std::vector<Tensor> match_logprob(const Tensor& z, const Tensor& y,
 
 std::vector<Tensor> match_logprob_autograd(const Tensor& z, const Tensor& y,
                                            const OptTensor& n, int64_t k) {
-  if (wants_grad(z)) return MatchLogProb::apply(z, y, n, k);
+  if (wants_grad("match_log_probs", z)) return MatchLogProb::apply(z, y, n, k);
   at::AutoDispatchBelowADInplaceOrView below;
   return match_logprob(z, y, n, k);
 }
