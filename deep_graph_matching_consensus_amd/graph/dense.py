@@ -80,6 +80,8 @@ class MaskLayout(object):
         counts.scatter_add_(0, batch, torch.ones_like(batch))
         self.N = int(counts.max().item()) if self.B > 0 else 0
         self.counts = counts.to(torch.int32)
+        self.ptr = torch.cat([counts.new_zeros(1), counts.cumsum(0)]).to(
+            torch.int32)
         self.num_nodes = num_nodes
         self.device = device
         ar = torch.arange(self.N, device=device).view(1, -1)
