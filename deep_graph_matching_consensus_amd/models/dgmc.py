@@ -780,7 +780,8 @@ class DGMC(torch.nn.Module):
         return self.loss_stats(S_0, y, mask)
 
     def log_probs(self, x_s, edge_index_s, edge_attr_s, batch_s, x_t,
-                  edge_index_t, edge_attr_t, batch_t, y_col=None, top=0):
+                  edge_index_t, edge_attr_t, batch_t, y_col=None, top=0,
+                  y=None):
         r"""How sure the model is: log-probabilities of the given matches,
         the rows' entropies and the best alternatives, for the initial and
         the refined correspondences (an extension; inputs as in
@@ -797,6 +798,11 @@ class DGMC(torch.nn.Module):
                 :meth:`objective`), -1 for none.
             top (int): number of alternatives per row (sparse models: of the
                 candidates).
+            y (Tensor, optional): ground truth ``[2, num_pairs]`` as in
+                :meth:`forward`: in training a sparse model's candidates then
+                hold it and random negatives.  Without it they are the best
+                ``k`` alone, and a given match outside of them is ``-inf``
+                and has no gradient - a loss on it needs ``y``.
 
         Returns ``(first, last)``, two
         :class:`~..ops.logprob.MatchLogProbs`.  Sparse models: a given match
@@ -805,7 +811,7 @@ class DGMC(torch.nn.Module):
             raise ValueError('log_probs needs the softmax normalization')
         with forward_cache():
             out = self._forward(x_s, edge_index_s, edge_attr_s, batch_s, x_t,
-                                edge_index_t, edge_attr_t, batch_t, None,
+                                edge_index_t, edge_attr_t, batch_t, y,
                                 raw='scores')
         if y_col is None:
             y_col = torch.full((x_s.size(0), ), -1, dtype=torch.long,

@@ -105,3 +105,38 @@ def test_model_answers_in_reference_mode(device, k):
         # (a probability of at most 1, from the same scores)
         assert (r.top_log_prob[:, 0].exp() - best).abs().max() < \
             64 * 2.0 ** -24
+
+
+@pytest.mark.parametrize('device', [
+    'cpu', pytest.param('cuda', marks=pytest.mark.gpu)])
+def test_sparse_models_train_on_log_probs(device):
+    """With the ground truth among the candidates every given match has a
+    finite log-probability, that of ``forward`` on the same draws, and psi_1
+    a gradient from it."""
+    torch.manual_seed(0)
+    model = DGMC(GIN(16, 16, 2), GIN(8, 8, 2), num_steps=1, k=2).to(device)
+    model.train()
+    x = [torch.randn(n, 16, device=device) for n in (40, 60)]
+    ei = [torch.randint(0, n, (2, 3 * n), device=device) for n in (40, 60)]
+    args = (x[0], ei[0], None, None, x[1], ei[1], None, None)
+    y_col = torch.randperm(60, device=device)[:40]
+    y = torch.stack([torch.arange(40, device=device), y_col])
+    torch.manual_seed(1)
+    none, _ = model.log_probs(*args, y_col=y_col)
+    assert torch.isinf(none.log_prob).any()      # (outside the best two)
+    torch.manual_seed(1)
+    S = model(*args, y=y)
+    torch.manual_seed(1)
+    res = model.log_probs(*args, y_col=y_col, top=3, y=y)
+    for s, r in zip(S, res):
+        want = torch.stack([v[i == c][0].log() for v, i, c in zip(
+            s.__val__.double(), s.__idx__, y_col)])
+        # (the probability is rounded, its log here is not)
+        assert (r.log_prob.double() - want).abs().max() < 64 * 2.0 ** -24
+        assert r.top_index.shape == (40, 3)
+    loss = -(res[0].log_prob + res[1].log_prob).mean()
+    grads = torch.autograd.grad(loss, list(model.psi_1.parameters()),
+                                allow_unused=True)
+    grads = [g for g in grads if g is not None]
+    assert grads and all(torch.isfinite(g).all() for g in grads)
+    assert any((g != 0).any() for g in grads)
