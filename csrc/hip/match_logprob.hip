@@ -467,17 +467,20 @@ __device__ __forceinline__ float lp_grad(const LpRow& w, float z, int j) {
   return j < w.nv ? g : 0.f;
 }
 
-// One value a thread (short rows, rows whose score and gradient vectors do
-// not fall on the same 16-byte boundaries).
+// One value a thread at a time (short rows, rows whose score and gradient
+// vectors do not fall on the same 16-byte boundaries).
+constexpr int64_t kLpFlatBlocks = 1 << 23;     // (2^31 threads)
+
 template <typename T>
 __global__ __launch_bounds__(256) void lp_bwd_flat_kernel(const LpArgs a) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= a.rows * a.V) return;
-  const int64_t r = e / a.V;
-  const int j = (int)(e - r * a.V);
-  const LpRow w = lp_row(a, r);
-  ((T*)a.dz)[e] = Cvt<T>::from_f(
-      lp_grad(w, Cvt<T>::to_f(((const T*)a.z)[r * a.stride + j]), j));
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+       e < a.rows * a.V; e += (int64_t)gridDim.x * 256) {
+    const int64_t r = e / a.V;
+    const int j = (int)(e - r * a.V);
+    const LpRow w = lp_row(a, r);
+    ((T*)a.dz)[e] = Cvt<T>::from_f(
+        lp_grad(w, Cvt<T>::to_f(((const T*)a.z)[r * a.stride + j]), j));
+  }
 }
 
 // One workgroup per 4 vectors a lane of one row.
@@ -668,9 +671,8 @@ at::Tensor match_logprob_bwd(const OptTensor& gl,
       lp_bwd_kernel<T>
           <<<dim3((unsigned)(R * a.parts)), 256, 0, st>>>(a);
     } else {
-      const int64_t blocks = (R * a.V + 255) / 256;
-      TORCH_CHECK(blocks < (1 << 24),
-                  "match_log_probs: too many scores for one call");
+      const int64_t blocks =
+          std::min<int64_t>((R * a.V + 255) / 256, kLpFlatBlocks);
       lp_bwd_flat_kernel<T><<<dim3((unsigned)blocks), 256, 0, st>>>(a);
     }
     DGMC_CHECK_LAUNCH();

@@ -140,3 +140,25 @@ def test_sparse_models_train_on_log_probs(device):
     grads = [g for g in grads if g is not None]
     assert grads and all(torch.isfinite(g).all() for g in grads)
     assert any((g != 0).any() for g in grads)
+
+
+@pytest.mark.gpu
+def test_log_probs_train_on_more_than_2_to_32_scores():
+    """Short rows, more scores than one launch has threads: what the forward
+    takes, the backward takes."""
+    R, V = (1 << 24) + 5, 257 - 1
+    if torch.cuda.mem_get_info()[0] < 48 << 30:
+        pytest.skip('needs 48 GB')
+    z = torch.zeros(R, V, dtype=torch.bfloat16, device='cuda')
+    z[-1, :5] = 3.0
+    z.requires_grad_(True)
+    y = torch.full((R, ), 2, dtype=torch.long, device='cuda')
+    r = match_log_probs(z, y)
+    g, = torch.autograd.grad(r.log_prob, z, torch.ones(R, device='cuda'))
+    for i in (0, R // 2, (1 << 32) // V, R - 2, R - 1):
+        row = z[i].detach().double().cpu()
+        want = -torch.softmax(row, 0)
+        want[2] += 1
+        # bf16: half a step of the value, after fp32's exp and sums
+        tol = (2.0 ** -8 + (V + 16) * 2.0 ** -24) * want.abs()
+        assert ((g[i].double().cpu() - want).abs() <= tol).all(), i
