@@ -327,6 +327,9 @@ static Args make_args(const at::Tensor& q, const at::Tensor& k,
                   q.size(1) % k.size(1) == 0 && q.size(1) / k.size(1) <= 32,
               "segment_attention: query heads must be a multiple (at most "
               "32) of the key heads");
+  // (a tile's rows, also of a copy in eights, lie within 2^31 bytes)
+  TORCH_CHECK(q.size(1) * ((q.size(2) + 7) / 8 * 8) <= 1 << 21,
+              "segment_attention: rows of more than 2^21 values");
   check_index(ptr_q, "ptr_q", 1, q);
   check_index(ptr_k, "ptr_k", 1, q);
   TORCH_CHECK(ptr_q.size(0) >= 1 && ptr_q.size(0) == ptr_k.size(0),

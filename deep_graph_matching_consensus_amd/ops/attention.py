@@ -26,6 +26,9 @@ from . import reference as ref
 MAX_DISTANCE = 1 << 22
 MAX_GROUP = 32
 MAX_DIM = 128
+#: Values of one row (heads times the dimension, in eights): the kernels
+#: address the 128 rows of a tile within 2^31 bytes of its first.
+MAX_ROW = 1 << 21
 #: Largest scale and cap, and the smallest cap's reciprocal: fp32 holds what
 #: the kernels form of them.
 MAX_FACTOR = 1e30
@@ -74,6 +77,9 @@ def _check(q, k, v, ptr_q, ptr_k, cap, scale):
         raise ValueError('{} query heads over {} key heads: need a multiple '
                          'of at most {}'.format(q.size(1), k.size(1),
                                                 MAX_GROUP))
+    if q.size(1) * (-(-q.size(2) // 8) * 8) > MAX_ROW:
+        raise ValueError('{} heads of {} are more than {} values a '
+                         'row'.format(q.size(1), q.size(2), MAX_ROW))
     for t in (ptr_q, ptr_k):
         if t.dtype != torch.int32 or t.dim() != 1 or t.numel() < 1 or \
                 t.device != q.device:

@@ -249,3 +249,19 @@ def test_scores_of_2_to_the_31(dtype, lq, lk, D, axes, scale):
         for t, e, x in ((dk, edk, 'dk'), (dv, edv, 'dv')):
             err = (got[x][sk, 0].double() - t).abs()
             assert (err <= e + u * t.abs()).all(), x
+
+
+def test_rows_wider_than_a_buffers_range_are_refused():
+    """A tile of 128 rows has to lie within 2^31 bytes, whatever its copy."""
+    p = torch.zeros(1, dtype=torch.int32)
+    q, k = torch.zeros(0, 16416, 128), torch.zeros(0, 513, 128)
+    with pytest.raises(ValueError, match='row'):
+        segment_attention(q, k, k, p)
+    q, k = torch.zeros(0, 16384, 128), torch.zeros(0, 512, 128)
+    assert segment_attention(q, k, k, p).shape == q.shape
+    # 1 to 8 wide heads take 8 values in a copy
+    q = torch.zeros(0, 1 << 18, 3)
+    assert segment_attention(q, q, q, p).shape == q.shape
+    q = torch.zeros(0, (1 << 18) + 32, 3)
+    with pytest.raises(ValueError, match='row'):
+        segment_attention(q, q, q, p)
