@@ -63,6 +63,12 @@ class AttentionConv(torch.nn.Module):
         graph) and, for a layer with a bias, int32 positions ``pos [sum N,
         axes]``; ``other = (x_o, batch_o, pos_o)``: the paired graphs to
         attend to (``x``'s own otherwise)."""
+        if self.axes:
+            for p in (pos, ) if other is None else (pos, other[2]):
+                axes = 0 if p is None else 1 if p.dim() == 1 else p.size(-1)
+                if axes != self.axes:
+                    raise ValueError('{} needs positions pos [nodes, '
+                                     '{}]'.format(self, self.axes))
         ptr = dense_layout(batch, x.size(0), x.device).ptr
         h = layer_norm(x, self.norm_weight, self.norm_bias, self.eps)
         q = linear(h, self.query.weight, self.query.bias)

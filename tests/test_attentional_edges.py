@@ -162,3 +162,24 @@ def test_log_probs_train_on_more_than_2_to_32_scores():
         # bf16: half a step of the value, after fp32's exp and sums
         tol = (2.0 ** -8 + (V + 16) * 2.0 ** -24) * want.abs()
         assert ((g[i].double().cpu() - want).abs() <= tol).all(), i
+
+
+@pytest.mark.parametrize('axes,given', [(2, 1), (2, None), (1, 2), (1, 3)])
+def test_layer_refuses_positions_of_other_axes(axes, given):
+    """A table of 49 buckets is 7 x 7 or 49 on a line: positions do not say
+    which."""
+    conv = AttentionConv(32, 4, axes=axes, half=3 if axes == 2 else 4,
+                         octave_steps=2)
+    shape = (5, ) if given is None else (5, given)
+    pos = torch.zeros(shape, dtype=torch.int32)
+    x = torch.randn(5, 32)
+    with pytest.raises(ValueError, match='positions'):
+        conv(x, None, pos)
+    ok = torch.zeros((5, axes), dtype=torch.int32)
+    with pytest.raises(ValueError, match='positions'):
+        conv(x, None, ok, other=(x, None, pos))
+    assert conv(x, None, ok, other=(x, None, ok)).shape == x.shape
+    if axes == 1:
+        assert torch.equal(conv(x, None, ok[:, 0]), conv(x, None, ok))
+    with pytest.raises(ValueError, match='pos'):
+        conv(x)
