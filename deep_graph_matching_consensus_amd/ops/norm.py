@@ -20,7 +20,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
         x (Tensor): ``[..., C]`` fp32, bf16 or fp16, ``C <= 8192``.
         weight, bias (Tensor, optional): ``[C]``, any floating dtype (fp32
             arithmetic and gradients); ``bias`` needs ``weight``.
-        eps (float): variance floor, > 0.
+        eps (float): variance floor, > 0 in fp32.
         residual (Tensor, optional): like ``x``; the norm is then of ``s = x
             + residual`` (in ``x``'s dtype) and ``(y, s)`` is returned.
 
@@ -38,8 +38,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
                              'x'.format(name, C))
     if bias is not None and weight is None:
         raise ValueError('bias needs weight')
-    if not eps > 0.0:
-        raise ValueError('eps must be > 0')
+    if not torch.finfo(ref.sum_dtype(x.dtype)).tiny <= eps < float('inf'):
+        raise ValueError('eps must be finite, > 0 and a normal number of '
+                         'fp32')
     if residual is not None and (residual.shape != x.shape or
                                  residual.dtype != x.dtype or
                                  residual.device != x.device):

@@ -183,3 +183,21 @@ def test_layer_refuses_positions_of_other_axes(axes, given):
         assert torch.equal(conv(x, None, ok[:, 0]), conv(x, None, ok))
     with pytest.raises(ValueError, match='pos'):
         conv(x)
+
+
+@pytest.mark.parametrize('eps', [1e-46, 1e-39, float('inf'), float('nan')])
+def test_norm_refuses_a_floor_that_fp32_does_not_hold(eps):
+    """(a constant row's deviation would be divided by 0)"""
+    with pytest.raises(ValueError, match='eps'):
+        layer_norm(torch.ones(2, 4), eps=eps)
+
+
+@pytest.mark.parametrize('device', [
+    'cpu', pytest.param('cuda', marks=pytest.mark.gpu)])
+def test_norm_of_constant_rows_at_the_least_floor(device):
+    x = torch.full((2, 8), 3.0, device=device, requires_grad=True)
+    y = layer_norm(x, eps=torch.finfo(torch.float32).tiny)
+    g, = torch.autograd.grad(y.sum(), x)
+    assert (y == 0).all() and (g == 0).all()
+    if device == 'cpu':          # fp64 holds more
+        assert (layer_norm(x.detach().double(), eps=1e-100) == 0).all()
