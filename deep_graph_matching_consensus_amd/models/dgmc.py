@@ -235,10 +235,12 @@ class DGMC(torch.nn.Module):
 
     Args:
         psi_1 (torch.nn.Module): GNN computing node embeddings
-            ``psi_1(x, edge_index, edge_attr)``.
-        psi_2 (torch.nn.Module): GNN validating neighbourhood consensus; must
-            expose ``in_channels`` (size of the random node indicators) and
-            ``out_channels``.
+            ``psi_1(x, edge_index, edge_attr)`` - or ``psi_1(x, batch)`` for
+            a module that ``takes_batch`` (:class:`~..nn.AttentionConv`
+            without a position bias).
+        psi_2 (torch.nn.Module): GNN validating neighbourhood consensus,
+            called likewise; must expose ``in_channels`` (size of the random
+            node indicators) and ``out_channels``.
         num_steps (int): number of consensus iterations.
         k (int, optional): sparsity.  ``-1`` keeps dense correspondences.
         detach (bool, optional): stop gradients into ``psi_1``.
@@ -277,10 +279,13 @@ class DGMC(torch.nn.Module):
             return False
         return bool(getattr(psi, 'pair_fusable', False))
 
-    def _encode(self, psi, pair, x_s, x_t, ei_s, ea_s, ei_t, ea_t):
+    def _encode(self, psi, pair, x_s, x_t, ei_s, ea_s, ei_t, ea_t, batch_s,
+                batch_t):
         if pair is not None and self._fusable(psi):
             h = psi(_cat_rows(x_s, x_t), pair.edge_index, pair.edge_attr)
             return h[:pair.n_s], h[pair.n_s:]
+        if getattr(psi, 'takes_batch', False):
+            return psi(x_s, batch_s), psi(x_t, batch_t)
         return psi(x_s, ei_s, ea_s), psi(x_t, ei_t, ea_t)
 
     # ------------------------------------------------------------------
@@ -374,7 +379,8 @@ class DGMC(torch.nn.Module):
 
         with trace_range('dgmc.psi_1'):
             h_s, h_t = self._encode(self.psi_1, pair, x_s, x_t, edge_index_s,
-                                    edge_attr_s, edge_index_t, edge_attr_t)
+                                    edge_attr_s, edge_index_t, edge_attr_t,
+                                    batch_s, batch_t)
         if self.detach:
             h_s, h_t = h_s.detach(), h_t.detach()
 
@@ -438,8 +444,9 @@ class DGMC(torch.nn.Module):
                         if isinstance(o, CatParts):
                             return None, None, o
                         return o[:pair.n_s], o[pair.n_s:], o
-                    o_s = self.psi_2(r_s, edge_index_s, edge_attr_s)
-                    o_t = self.psi_2(r_t, edge_index_t, edge_attr_t)
+                    o_s, o_t = self._encode(
+                        self.psi_2, None, r_s, r_t, edge_index_s, edge_attr_s,
+                        edge_index_t, edge_attr_t, batch_s, batch_t)
                     return o_s, o_t, None
 
             if self.k < 1 and self.normalization == 'sinkhorn':

@@ -27,7 +27,12 @@ class AttentionConv(torch.nn.Module):
         half (int): signed buckets per axis, ``2 half + 1``.
         octave_steps (int): buckets per octave of distance.
         eps (float): of the norm.
+
+    Without a position bias it is an encoder of :class:`~..models.DGMC`, which
+    calls it with the graphs' ``batch`` vector in place of their edges.
     """
+
+    takes_batch = True
 
     def __init__(self, channels, heads, key_heads=None, cap=0.0, axes=0,
                  half=3, octave_steps=1, eps=1e-5):
@@ -36,6 +41,7 @@ class AttentionConv(torch.nn.Module):
         assert channels % heads == 0 and heads % key_heads == 0
         assert axes in (0, 1, 2)
         self.channels, self.heads, self.key_heads = channels, heads, key_heads
+        self.in_channels = self.out_channels = channels
         self.dim = channels // heads
         self.cap, self.axes, self.eps = cap, axes, eps
         self.octave_steps = octave_steps

@@ -201,3 +201,60 @@ def test_norm_of_constant_rows_at_the_least_floor(device):
     assert (y == 0).all() and (g == 0).all()
     if device == 'cpu':          # fp64 holds more
         assert (layer_norm(x.detach().double(), eps=1e-100) == 0).all()
+
+
+def _two_graphs(device):
+    g = torch.Generator().manual_seed(3)
+    x = [torch.randn(n, 16, generator=g).to(device) for n in (9, 11)]
+    ei = [torch.randint(0, 4, (2, 12), generator=g).to(device)
+          for _ in range(2)]
+    b = [torch.tensor([0] * 4 + [1] * (n - 4), device=device)
+         for n in (9, 11)]
+    return x[0], ei[0], None, b[0], x[1], ei[1], None, b[1]
+
+
+@pytest.mark.parametrize('device', [
+    'cpu', pytest.param('cuda', marks=pytest.mark.gpu)])
+@pytest.mark.parametrize('k', [-1, 3])
+@pytest.mark.parametrize('plain', [False, True])
+def test_model_of_attention_layers(device, k, plain):
+    """AttentionConv as psi_1 and psi_2: every graph attends to itself, and
+    all parameters that reach the scores train."""
+    torch.manual_seed(0)
+    model = DGMC(AttentionConv(16, 4), AttentionConv(8, 2), num_steps=2,
+                 k=k).to(device).eval()
+    args = _two_graphs(device)
+    with reference_mode(plain):
+        def scores(args):
+            torch.manual_seed(1)
+            return [S.to_dense() if S.is_sparse else S for S in model(*args)]
+
+        with torch.no_grad():
+            S = scores(args)
+            # S_0 straight from the layer
+            h = [model.psi_1(args[4 * i], args[4 * i + 3]) for i in (0, 1)]
+            z = h[0][:4] @ h[1][:4].t()
+            if k < 1:
+                assert (torch.softmax(z, -1) - S[0][:4, :4]).abs().max() < \
+                    64 * 16 * 2.0 ** -24
+            # the second pair's nodes do not reach the first one's rows
+            other = list(args)
+            other[0] = torch.cat([args[0][:4], args[0][4:].flip(0) * 2])
+            if k < 1:
+                far = scores(other)
+                for a, b in zip(S, far):
+                    assert torch.equal(a[:4], b[:4])
+        y = torch.arange(9, device=device)
+        y[4:] -= 4
+        torch.manual_seed(1)
+        first, last = model.log_probs(*args, y_col=y)
+        live = torch.isfinite(last.log_prob)
+        loss = -(first.log_prob + last.log_prob)[live].mean()
+        params = [p for n, p in model.named_parameters()]
+        grads = torch.autograd.grad(loss, params, allow_unused=True)
+    for (n, _), g in zip(model.named_parameters(), grads):
+        if n == 'mlp.2.bias':       # (a constant of a row's scores)
+            continue
+        assert g is not None and torch.isfinite(g).all(), n
+        if 'key_value.bias' not in n:
+            assert (g != 0).any(), n
