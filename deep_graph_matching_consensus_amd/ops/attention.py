@@ -60,9 +60,6 @@ def _check(q, k, v, ptr_q, ptr_k, cap, scale):
                 name, tuple(t.shape)))
         if t.dtype != q.dtype or t.device != q.device:
             raise ValueError('q, k and v must share dtype and device')
-    if q.is_cuda and q.dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError('segment_attention takes fp32 and bf16, got '
-                         '{}'.format(q.dtype))
     if not q.dtype.is_floating_point:
         raise ValueError('q, k and v must be floating')
     if k.shape != v.shape or k.size(2) != q.size(2):
@@ -195,6 +192,9 @@ def segment_attention(q, k, v, ptr_q, ptr_k=None, scale=None, cap=0.0,
             q, k, v, ptr_q, ptr_k, scale, cap, bias, pos_q, pos_k,
             bucket_starts(layout[0], octave_steps))
     dtype = q.dtype
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError('segment_attention takes fp32 and bf16, got '
+                         '{}'.format(dtype))
     if dtype == torch.bfloat16 and cap > MAX_CAP_BF16:
         q, k, v = q.float(), k.float(), v.float()
     q, k, v = (t if t.stride(2) == 1 or t.size(2) == 1 else t.contiguous()

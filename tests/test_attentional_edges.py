@@ -258,3 +258,22 @@ def test_model_of_attention_layers(device, k, plain):
         assert g is not None and torch.isfinite(g).all(), n
         if 'key_value.bias' not in n:
             assert (g != 0).any(), n
+
+
+@pytest.mark.gpu
+def test_fp64_layer_in_reference_mode():
+    """The oracles take fp64 on the GPU too; the kernels refuse it."""
+    torch.manual_seed(0)
+    conv = AttentionConv(32, 4, key_heads=2, axes=1).double()
+    conv.table.data.normal_()
+    x = torch.randn(11, 32, dtype=torch.float64)
+    pos = torch.arange(11, dtype=torch.int32)
+    want = conv(x, None, pos)
+    conv, x, pos = conv.cuda(), x.cuda(), pos.cuda()
+    with reference_mode():
+        got = conv(x, None, pos)
+    assert (got.cpu() - want).abs().max() < 1e-13 * 32
+    ptr = torch.tensor([0, 11], dtype=torch.int32, device='cuda')
+    q = x.view(11, 4, 8)
+    with pytest.raises(ValueError, match='fp32 and bf16'):
+        segment_attention(q, q, q, ptr)
