@@ -16,8 +16,9 @@
 // every run.
 //
 // Measured (38960 x 256 bf16 with residual, 80 MB each way; a large copy runs
-// at 4.8 TB/s): forward 24 us, 3.3 TB/s, backward 20 and its fold 4.  20 x
-// 256 fp32: 10 us, a launch.
+// at 4.8 TB/s): forward 24 us, 3.3 TB/s, backward 20 and its fold 4; no load
+// is in flight while a row is reduced, and 4870 groups of rows are 2.4 rounds
+// of 2048 workgroups that take the time of 3.  20 x 256 fp32: 10 us, a launch.
 #include "attentional.h"
 #include "common.h"
 

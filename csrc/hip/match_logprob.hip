@@ -22,9 +22,9 @@
 // Rows past one workgroup's registers are cut into parts; a second kernel
 // joins the parts' maxima, sums and selections.
 //
-// Measured (4500 x 19572 fp32, ten alternatives): forward 105 us for 352 MB
-// (3.4 TB/s: two workgroups a CU, whose loads stop while they rank), backward
-// 106 us for 705 MB, part of it still cached.  4608 x 19: 5 and 3 us.
+// Measured (4500 x 19572 fp32, ten alternatives): forward 109 us for 352 MB
+// (3.2 TB/s: two workgroups a CU, whose loads stop while they rank), backward
+// 110 us for 705 MB, part of it still cached.  4608 x 19: 5 and 3 us.
 #include "attentional.h"
 #include "common.h"
 

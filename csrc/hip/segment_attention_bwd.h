@@ -20,13 +20,15 @@
 // order); a workgroup keeps its columns over all the tiles it walks and sums
 // them once, a last kernel adds the workgroups' parts in order.
 //
-// Measured (dq / dkv).  4847 x 4893 rows, fp32 as x6, 4 heads of 64: 229 /
-// 304 us, 160 TFLOP/s of fp32 products - the matrix cores, six products for
-// one.  24 graphs of 1 to 1350 nodes, bf16, 8 heads on 2 key heads of
-// 128, cap and table: 149 / 147 us; the longest graph's tiles and, per 32 x
-// 32 scores, 90 vector cycles a score against 1024 matrix cycles.  1024
-// graphs of 3 to 19 nodes, fp32, two position axes: 42 / 40 us, 512 pairs of
-// 30 to 80 nodes, bf16: 55 / 41 us; latency of one wave's chain.
+// Measured (dq / dkv).  4847 x 4893 rows, fp32 as x6, 4 heads of 64: 231 /
+// 316 us, 156 TFLOP/s of fp32 products - the matrix cores, six products for
+// one; with a table dq takes exact products: 579 us.  24 graphs of 1 to 1350
+// nodes, bf16, 8 heads on 2 key heads of 128, cap and table: 151 / 165 us;
+// vector units busy 34 / 26 % of it, matrix cores 9 / 12 %: the time is that
+// of the workgroups with the most tiles (dq: 42 against 23 on average).  1024
+// graphs of 3 to 19 nodes, fp32, two position axes: 42 / 39 us (dq: vector
+// units busy 18 %, matrix cores 15 %), 512 pairs of 30 to 80 nodes, bf16: 54 /
+// 40 us; latency of one wave's chain.
 #pragma once
 
 #include "segment_attention.h"

@@ -16,14 +16,16 @@
 // 2 of bf16's 8 bits); and on short segments, whose few keys average nothing
 // out and whose time is latency, not products.
 //
-// Measured.  19388 x 19572 rows, 4 heads of 64, bf16: 463 us with its join,
-// 0.84 PFLOP/s - the vector unit bounds it (exp2 takes 16 cycles a wave: per
-// 32 x 64 scores it has 830 cycles of work, the matrix cores 512).  4847 x
-// 4893 rows, fp32 as x6: 146 us, 166 TFLOP/s, matrix cores.  One row in each of
-// four graphs of 14000 to 20000 nodes, bf16, heads of 128: 23 us, 75 MB at
-// 3.3 TB/s (474 workgroups of one wave).  1024 graphs of 3 to 19 nodes, fp32,
-// heads of 64: 27 us, the chain of dependent loads (segment search, rows,
-// tiles) and 64 matrix cycles for every fp32 product.
+// Measured.  19388 x 19572 rows, 4 heads of 64, bf16: 470 us with its join,
+// 0.83 PFLOP/s.  Per 32 x 64 scores the vector unit has 830 cycles of work
+// (exp2 takes 16 a wave) and the matrix cores 512; counters find them busy 65
+// and 40 % of the time: for the most part one runs after the other.  4847 x
+// 4893 rows, fp32 as x6: 148 us, 164 TFLOP/s, matrix cores; with a table 184.
+// One row in each of four graphs of 14000 to 20000 nodes, bf16, heads of 128:
+// 23 us, 75 MB at 3.2 TB/s (474 workgroups of one wave, a tile in flight
+// each).  1024 graphs of 3 to 19 nodes, fp32, heads of 64: 27 us, the chain of
+// dependent loads (segment search, rows, tiles) and 64 matrix cycles for every
+// fp32 product.
 #pragma once
 
 #include "segment_attention.h"

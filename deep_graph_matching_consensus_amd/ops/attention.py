@@ -175,7 +175,11 @@ def segment_attention(q, k, v, ptr_q, ptr_k=None, scale=None, cap=0.0,
         octave_steps (int): buckets per octave of distance.
 
     Returns ``[N_q, heads, dim]`` in ``q``'s dtype; softmax statistics and
-    all sums are fp32.
+    all sums are fp32.  bf16 products take weights (and in the backward
+    scores' gradients) as one bf16 term where the mean segment is long, as two
+    where it is short and in a training forward; that rule and the others of
+    the work's layout follow the batch's mean segment.  Forward-mode and
+    second derivatives are refused.
     """
     if ptr_k is None:
         ptr_k = ptr_q
