@@ -794,8 +794,8 @@ struct Bucket {
   int shift, width, K;
   // (0 - dmax: +0 where there is one bucket, whose offsets so have no sign)
   __device__ __forceinline__ explicit Bucket(const Args& a)
-      : dmin(0.f - a.dmax), dmax(a.dmax), dmul(a.dmul), shift(23 - a.mbits), width(5 + a.mbits),
-        K(a.half + 1) {}
+      : dmin(0.f - a.dmax), dmax(a.dmax), dmul(a.dmul), shift(23 - a.mbits),
+        width(5 + a.mbits), K(a.half + 1) {}
   __device__ __forceinline__ int slot(float d) const {
     const float c = __builtin_amdgcn_fmed3f(d, dmin, dmax);
     const float x = fmaf(fabsf(c), dmul, 2.f);
